@@ -65,6 +65,12 @@ EXPORTED_SYMBOLS = (
     "grx_comm_create",
     "grx_comm_destroy",
     "grx_comm_allgather",
+    "grx_token_logps_scratch_bytes",
+    "grx_token_logps",
+    "grx_token_logps_backward",
+    "grx_policy_loss_scratch_bytes",
+    "grx_policy_loss",
+    "grx_policy_loss_backward",
 )
 
 
@@ -229,6 +235,57 @@ class GrxBeamInitArgs(C.Structure):
     ]
 
 
+class GrxTokenLogpsArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("row_stride", C.c_int64),
+        ("pos_stride", C.c_int64),
+        ("token_ids", C.c_void_p),
+        ("ids_stride", C.c_int64),
+        ("B", C.c_int32),
+        ("T", C.c_int32),
+        ("V", C.c_int32),
+        ("dtype", C.c_int32),
+        ("temperature", C.c_float),
+        ("reserved", C.c_int32),
+        ("logps", C.c_void_p),
+        ("row_stats", C.c_void_p),
+        ("entropy", C.c_void_p),
+        ("grad_logps", C.c_void_p),
+        ("grad_entropy", C.c_void_p),
+        ("grad_logits", C.c_void_p),
+    ]
+
+
+class GrxPolicyLossArgs(C.Structure):
+    _fields_ = [
+        ("logps", C.c_void_p),
+        ("logps_stride", C.c_int64),
+        ("old_logps", C.c_void_p),
+        ("old_stride", C.c_int64),
+        ("ref_logps", C.c_void_p),
+        ("ref_stride", C.c_int64),
+        ("advantages", C.c_void_p),
+        ("adv_row_stride", C.c_int64),
+        ("adv_pos_stride", C.c_int64),
+        ("mask", C.c_void_p),
+        ("mask_stride", C.c_int64),
+        ("mask_type", C.c_int32),
+        ("R", C.c_int32),
+        ("T", C.c_int32),
+        ("sequence_level", C.c_int32),
+        ("row_mean", C.c_int32),
+        ("beta", C.c_float),
+        ("epsilon_low", C.c_double),
+        ("epsilon_high", C.c_double),
+        ("delta", C.c_double),
+        ("normalizer", C.c_double),
+        ("loss", C.c_void_p),
+        ("stats", C.c_void_p),
+        ("unit_grad", C.c_void_p),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -341,6 +398,18 @@ def _declare(lib: C.CDLL) -> None:
     lib.grx_group_normalize_tokenwise.argtypes = [vp, vp, i32, i32, i32, f32, vp, vp]
     lib.grx_token_prefix_advantages.restype = C.c_int
     lib.grx_token_prefix_advantages.argtypes = [C.POINTER(GrxTokenPrefixArgs), vp]
+    lib.grx_token_logps_scratch_bytes.restype = C.c_size_t
+    lib.grx_token_logps_scratch_bytes.argtypes = [i64, i32, i32]
+    lib.grx_token_logps.restype = C.c_int
+    lib.grx_token_logps.argtypes = [C.POINTER(GrxTokenLogpsArgs), vp, C.c_size_t, vp]
+    lib.grx_token_logps_backward.restype = C.c_int
+    lib.grx_token_logps_backward.argtypes = [C.POINTER(GrxTokenLogpsArgs), vp]
+    lib.grx_policy_loss_scratch_bytes.restype = C.c_size_t
+    lib.grx_policy_loss_scratch_bytes.argtypes = [i32, i32]
+    lib.grx_policy_loss.restype = C.c_int
+    lib.grx_policy_loss.argtypes = [C.POINTER(GrxPolicyLossArgs), vp, C.c_size_t, vp]
+    lib.grx_policy_loss_backward.restype = C.c_int
+    lib.grx_policy_loss_backward.argtypes = [vp, vp, vp, i64, vp, vp]
 
 
 def lib() -> C.CDLL:

@@ -1,0 +1,316 @@
+// Clipped policy loss with a KL term, and its gradient, on per-token log-probabilities.  Per valid token, with
+// d = logp - old (or its mean over the row's valid tokens: one ratio per sequence), w = exp(d), A the advantage:
+//   l = -min(min(w, delta) A, clip(w, 1 - e_low, 1 + e_high) A) + beta (exp(q) - 1 - q),      q = ref - logp
+//   dl/dlogp = -w A where the clipped term is not the smaller one, + -beta (exp(q) - 1)
+// and the loss is the sum of l under one of four weights: 1 / (rows x tokens of the row), 1 / tokens of the batch,
+// or a constant.  About 20 bytes a token; a launcher's batch is 320 tokens, so small calls are launch latency (one
+// workgroup, one launch) and large ones HBM.
+//
+// Differences are taken, and compared with log(1 - e_low), log(1 + e_high), log(delta), in 64 bits: which side of a
+// bound a token is on does not depend on the rounding of exp.  Terms are fp32, all sums 64 bits, in a fixed order.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <string.h>
+
+#include "common.h"
+
+#define PL_THREADS 256
+#define PL_BIG 1024
+#define PL_SINGLE_TOKENS 4096   // up to here one workgroup does the whole call
+#define PL_MAX_WGS 1024
+#define PL_SUMS 5               // loss, kl, clipped below, clipped above, valid tokens
+
+struct PlArgs {
+    grx_policy_loss_args p;
+    double log_low, log_high, log_delta;
+    float low, high, delta;
+    double constant;            // the weight all tokens share; 0: 1 / valid tokens of the batch
+    double* partials;           // [gridDim][PL_SUMS]; null: this launch is one workgroup and finishes the call
+    int n_partials;
+};
+
+__device__ __forceinline__ bool pl_valid(const grx_policy_loss_args& p, int64_t r, int t) {
+    const int64_t i = r * p.mask_stride + t;
+    switch (p.mask_type) {
+        case GRX_MASK_U8: return static_cast<const uint8_t*>(p.mask)[i] != 0;
+        case GRX_MASK_I32: return static_cast<const int32_t*>(p.mask)[i] > 0;
+        case GRX_MASK_I64: return static_cast<const int64_t*>(p.mask)[i] > 0;
+        default: return static_cast<const float*>(p.mask)[i] > 0.f;
+    }
+}
+
+// exp(q) - 1 - q without the cancellation near 0: its Taylor series (the first term left out is below 2^-26 of the
+// sum for |q| < 1), the difference itself elsewhere.
+__device__ __forceinline__ float pl_kl(float q) {
+    if (fabsf(q) < 1.f) {
+        float s = 1.f / 39916800.f;
+        s = fmaf(s, q, 1.f / 3628800.f);
+        s = fmaf(s, q, 1.f / 362880.f);
+        s = fmaf(s, q, 1.f / 40320.f);
+        s = fmaf(s, q, 1.f / 5040.f);
+        s = fmaf(s, q, 1.f / 720.f);
+        s = fmaf(s, q, 1.f / 120.f);
+        s = fmaf(s, q, 1.f / 24.f);
+        s = fmaf(s, q, 1.f / 6.f);
+        s = fmaf(s, q, 0.5f);
+        return s * q * q;
+    }
+    return expf(q) - 1.f - q;
+}
+
+// Sum over the LANES lanes that share a row; every lane gets it.  LANES > 64: a whole workgroup.
+template <int LANES>
+__device__ __forceinline__ double pl_row_sum(double v, double* lds) {
+#pragma unroll
+    for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (LANES > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = 0.0;
+#pragma unroll
+        for (int w = 0; w < LANES / 64; ++w) v += lds[w];
+    }
+    return v;
+}
+
+// What the call returns, from the sums over all tokens.  global: the factor that the stored gradient still lacks.
+__device__ __forceinline__ void pl_finish(const PlArgs& a, const double* s) {
+    const double tokens = s[4] > 1.0 ? s[4] : 1.0;
+    const double global = a.constant != 0.0 ? a.constant : 1.0 / tokens;
+    a.p.loss[0] = (float)(s[0] * global);
+    a.p.stats[0] = (float)(s[1] / tokens);
+    a.p.stats[1] = (float)(s[2] / tokens);
+    a.p.stats[2] = (float)(s[3] / tokens);
+    a.p.stats[3] = (float)global;
+}
+
+// LANES lanes share a row; a workgroup of THREADS threads holds THREADS / LANES rows at a time.
+template <int LANES, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_loss_kernel(PlArgs a) {
+    __shared__ double lds[16 * PL_SUMS];
+    const grx_policy_loss_args& p = a.p;
+    constexpr int ROWS = THREADS / LANES;
+    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
+    double sum[PL_SUMS] = {0.0, 0.0, 0.0, 0.0, 0.0};
+    // every thread of the workgroup makes the same number of turns (barriers inside): rows past the end are empty
+    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < p.R; base += (int64_t)gridDim.x * ROWS) {
+        const int64_t r = base + slot;
+        const bool live = r < p.R;
+        const float* lp = p.logps + r * p.logps_stride;
+        const float* old = p.old_logps ? p.old_logps + r * p.old_stride : nullptr;
+        const float* ref = p.ref_logps ? p.ref_logps + r * p.ref_stride : nullptr;
+        float* grad = p.unit_grad ? p.unit_grad + r * p.T : nullptr;
+        double row_w = 1.0, row_d = 0.0, inv_n = 1.0;
+        if (p.row_mean || p.sequence_level) {
+            double n = 0.0, d = 0.0;
+            if (live)
+                for (int t = lane; t < p.T; t += LANES)
+                    if (pl_valid(p, r, t)) {
+                        n += 1.0;
+                        if (p.sequence_level && old) d += (double)lp[t] - (double)old[t];
+                    }
+            n = pl_row_sum<LANES>(n, lds);
+            inv_n = 1.0 / (n > 1.0 ? n : 1.0);
+            if (p.sequence_level) row_d = pl_row_sum<LANES>(d, lds) * inv_n;
+            if (p.row_mean) row_w = inv_n;
+        }
+        float seq_w = 1.f;
+        double seq_slope = 0.0;
+        if (p.sequence_level) seq_w = expf((float)row_d);
+        for (int pass = 0; pass < (p.sequence_level && grad ? 2 : 1); ++pass) {
+            // second pass (one ratio per sequence): every token of the row carries the row's slope
+            if (pass == 1) seq_slope = pl_row_sum<LANES>(seq_slope, lds) * inv_n;
+            if (live)
+                for (int t = lane; t < p.T; t += LANES) {
+                    if (!pl_valid(p, r, t)) {
+                        if (grad && pass == 0) grad[t] = 0.f;
+                        continue;
+                    }
+                    const float x = lp[t];
+                    float kl = 0.f, kl_slope = 0.f;
+                    if (ref) {
+                        const float q = (float)((double)ref[t] - (double)x);
+                        kl = pl_kl(q);
+                        kl_slope = -p.beta * expm1f(q);
+                    }
+                    if (pass == 1) {
+                        grad[t] = (float)(row_w * (seq_slope + (double)kl_slope));
+                        continue;
+                    }
+                    double d = row_d;
+                    float w = seq_w;
+                    if (!p.sequence_level) {
+                        d = old ? (double)x - (double)old[t] : 0.0;
+                        w = expf((float)d);
+                    }
+                    const float adv = p.advantages[r * p.adv_row_stride + (int64_t)t * p.adv_pos_stride];
+                    const bool below = d < a.log_low, above = d > a.log_high, capped = d > a.log_delta;
+                    const float first = (capped ? a.delta : w) * adv;
+                    const float second = (below ? a.low : above ? a.high : w) * adv;
+                    const float l = fmaf(p.beta, kl, -(second < first ? second : first));  // a NaN of either stays
+                    const bool cut_low = below && adv < 0.f, cut_high = above && adv > 0.f;
+                    const float slope = (cut_low || cut_high || capped) ? 0.f : -w * adv;
+                    sum[0] += row_w * (double)l;
+                    sum[1] += (double)kl;
+                    sum[2] += cut_low ? 1.0 : 0.0;
+                    sum[3] += cut_high ? 1.0 : 0.0;
+                    sum[4] += 1.0;
+                    if (!grad) continue;
+                    if (p.sequence_level)
+                        seq_slope += (double)slope;
+                    else
+                        grad[t] = (float)(row_w * ((double)slope + (double)kl_slope));
+                }
+        }
+    }
+    // totals of the workgroup, waves in order
+#pragma unroll
+    for (int i = 0; i < PL_SUMS; ++i) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum[i] += __shfl_xor(sum[i], o, 64);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < PL_SUMS; ++i) lds[(threadIdx.x >> 6) * PL_SUMS + i] = sum[i];
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < THREADS / 64; ++w)
+            for (int i = 0; i < PL_SUMS; ++i) sum[i] += lds[w * PL_SUMS + i];
+        if (a.partials == nullptr) {
+            pl_finish(a, sum);
+        } else {
+            for (int i = 0; i < PL_SUMS; ++i) a.partials[(int64_t)blockIdx.x * PL_SUMS + i] = sum[i];
+        }
+    }
+}
+
+__global__ __launch_bounds__(PL_THREADS) void policy_loss_join_kernel(PlArgs a) {
+    __shared__ double lds[PL_THREADS / 64][PL_SUMS];
+    double sum[PL_SUMS] = {0.0, 0.0, 0.0, 0.0, 0.0};
+    for (int j = threadIdx.x; j < a.n_partials; j += PL_THREADS)
+#pragma unroll
+        for (int i = 0; i < PL_SUMS; ++i) sum[i] += a.partials[(int64_t)j * PL_SUMS + i];
+#pragma unroll
+    for (int i = 0; i < PL_SUMS; ++i) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum[i] += __shfl_xor(sum[i], o, 64);
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6][i] = sum[i];
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < PL_THREADS / 64; ++w)
+            for (int i = 0; i < PL_SUMS; ++i) sum[i] += lds[w][i];
+        pl_finish(a, sum);
+    }
+}
+
+// dL/dlogps = unit gradient x the factor that was known only at the end x what came from behind the loss
+__global__ __launch_bounds__(PL_THREADS) void policy_loss_grad_kernel(const float* __restrict__ unit,
+                                                                      const float* __restrict__ stats,
+                                                                      const float* __restrict__ upstream, int64_t n,
+                                                                      float* __restrict__ out) {
+    const float f = stats[3] * upstream[0];
+    for (int64_t i = ((int64_t)blockIdx.x * PL_THREADS + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * PL_THREADS * 4) {
+        if (i + 4 <= n) {
+            const float4 v = *reinterpret_cast<const float4*>(unit + i);
+            float4 w;
+            w.x = v.x == 0.f ? 0.f : v.x * f;  // padding keeps its 0 under an infinite or NaN factor
+            w.y = v.y == 0.f ? 0.f : v.y * f;
+            w.z = v.z == 0.f ? 0.f : v.z * f;
+            w.w = v.w == 0.f ? 0.f : v.w * f;
+            *reinterpret_cast<float4*>(out + i) = w;
+        } else {
+            for (int64_t j = i; j < n; ++j) out[j] = unit[j] == 0.f ? 0.f : unit[j] * f;
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+static int pl_lanes(int T) { return T <= 8 ? 8 : T <= 2048 ? 64 : PL_BIG; }
+
+static int pl_groups(int R, int T) {
+    if ((int64_t)R * T <= PL_SINGLE_TOKENS) return 1;
+    const int lanes = pl_lanes(T);
+    const int rows = lanes == PL_BIG ? 1 : PL_THREADS / lanes;
+    const int64_t g = ((int64_t)R + rows - 1) / rows;
+    return g < PL_MAX_WGS ? (int)g : PL_MAX_WGS;
+}
+
+extern "C" size_t grx_policy_loss_scratch_bytes(int32_t R, int32_t T) {
+    if (R <= 0 || T <= 0) return 0;
+    const int g = pl_groups(R, T);
+    return g > 1 ? (size_t)g * PL_SUMS * sizeof(double) : 0;
+}
+
+extern "C" int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, size_t scratch_bytes, void* stream_) {
+    const char* who = "grx_policy_loss";
+    GRX_REQUIRE(args != nullptr, GRX_E_INVALID, "%s: null args", who);
+    PlArgs a;
+    memset(&a, 0, sizeof(a));
+    a.p = *args;
+    const grx_policy_loss_args& p = a.p;
+    GRX_REQUIRE(p.R >= 0 && p.T >= 0, GRX_E_INVALID, "%s: bad shape", who);
+    GRX_REQUIRE(p.loss != nullptr && p.stats != nullptr, GRX_E_INVALID, "%s: null output", who);
+    const bool any = (int64_t)p.R * p.T > 0;
+    GRX_REQUIRE(!any || (p.logps != nullptr && p.advantages != nullptr && p.mask != nullptr), GRX_E_INVALID,
+                "%s: null input", who);
+    GRX_REQUIRE(p.mask_type >= GRX_MASK_U8 && p.mask_type <= GRX_MASK_F32, GRX_E_INVALID, "%s: mask type %d", who, p.mask_type);
+    GRX_REQUIRE(p.epsilon_low >= 0.0 && p.epsilon_low < 1.0 && p.epsilon_high >= 0.0 && isfinite(p.epsilon_high), GRX_E_INVALID,
+                "%s: epsilon_low must lie in [0, 1) and epsilon_high must not be negative", who);
+    GRX_REQUIRE(p.delta == 0.0 || (isfinite(p.delta) && p.delta > 1.0 + p.epsilon_high), GRX_E_INVALID,
+                "%s: delta must be 0 (off) or above 1 + epsilon_high", who);
+    GRX_REQUIRE(isfinite(p.beta) && (p.beta == 0.f || !any || p.ref_logps != nullptr), GRX_E_INVALID,
+                "%s: a KL term needs reference log-probabilities", who);
+    GRX_REQUIRE(p.normalizer >= 0.0 && isfinite(p.normalizer), GRX_E_INVALID, "%s: normalizer must not be negative", who);
+    GRX_REQUIRE(p.unit_grad == nullptr || ((uintptr_t)p.unit_grad & 15) == 0, GRX_E_INVALID, "%s: misaligned unit_grad", who);
+    a.log_low = log1p(-p.epsilon_low);
+    a.log_high = log1p(p.epsilon_high);
+    a.log_delta = p.delta == 0.0 ? (double)INFINITY : log(p.delta);
+    a.delta = (float)p.delta;
+    a.low = (float)(1.0 - p.epsilon_low);
+    a.high = (float)(1.0 + p.epsilon_high);
+    a.constant = p.row_mean ? 1.0 / (double)(p.R > 0 ? p.R : 1) : p.normalizer > 0.0 ? 1.0 / p.normalizer : 0.0;
+    hipStream_t stream = (hipStream_t)stream_;
+    const int lanes = pl_lanes(p.T);
+    const int groups = any ? pl_groups(p.R, p.T) : 1;
+    a.n_partials = groups;
+    if (groups > 1) {
+        const size_t need = grx_policy_loss_scratch_bytes(p.R, p.T);
+        GRX_REQUIRE(scratch != nullptr && scratch_bytes >= need && ((uintptr_t)scratch & 7) == 0, GRX_E_WORKSPACE,
+                    "%s: scratch of %zu bytes, need %zu", who, scratch_bytes, need);
+        a.partials = reinterpret_cast<double*>(scratch);
+    }
+    if (lanes == PL_BIG) {
+        hipLaunchKernelGGL((policy_loss_kernel<PL_BIG, PL_BIG>), dim3(groups), dim3(PL_BIG), 0, stream, a);
+    } else if (groups == 1) {
+        if (lanes == 8) hipLaunchKernelGGL((policy_loss_kernel<8, PL_BIG>), dim3(1), dim3(PL_BIG), 0, stream, a);
+        else hipLaunchKernelGGL((policy_loss_kernel<64, PL_BIG>), dim3(1), dim3(PL_BIG), 0, stream, a);
+    } else {
+        if (lanes == 8) hipLaunchKernelGGL((policy_loss_kernel<8, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a);
+        else hipLaunchKernelGGL((policy_loss_kernel<64, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a);
+    }
+    GRX_CHECK_HIP(hipGetLastError());
+    if (groups > 1) {
+        hipLaunchKernelGGL(policy_loss_join_kernel, dim3(1), dim3(PL_THREADS), 0, stream, a);
+        GRX_CHECK_HIP(hipGetLastError());
+    }
+    return GRX_OK;
+}
+
+extern "C" int grx_policy_loss_backward(const float* unit_grad, const float* stats, const float* upstream, int64_t n,
+                                        float* grad_logps, void* stream_) {
+    const char* who = "grx_policy_loss_backward";
+    GRX_REQUIRE(n >= 0, GRX_E_INVALID, "%s: bad size", who);
+    if (n == 0) return GRX_OK;
+    GRX_REQUIRE(unit_grad != nullptr && stats != nullptr && upstream != nullptr && grad_logps != nullptr, GRX_E_INVALID,
+                "%s: null buffer", who);
+    GRX_REQUIRE((((uintptr_t)unit_grad | (uintptr_t)grad_logps) & 15) == 0, GRX_E_INVALID, "%s: misaligned buffer", who);
+    int64_t wgs = (n / 4 + PL_THREADS - 1) / PL_THREADS;
+    wgs = wgs < 1 ? 1 : wgs > 2048 ? 2048 : wgs;
+    hipLaunchKernelGGL(policy_loss_grad_kernel, dim3((unsigned)wgs), dim3(PL_THREADS), 0, (hipStream_t)stream_, unit_grad,
+                       stats, upstream, n, grad_logps);
+    GRX_CHECK_HIP(hipGetLastError());
+    return GRX_OK;
+}

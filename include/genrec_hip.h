@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GRX_ABI_VERSION 15
+#define GRX_ABI_VERSION 16
 
 #if defined(GRX_BUILDING)
 #define GRX_API __attribute__((visibility("default")))
@@ -699,6 +699,89 @@ typedef struct grx_token_prefix_args {
     float* token_advantages;
 } grx_token_prefix_args;
 GRX_API int grx_token_prefix_advantages(const grx_token_prefix_args* args, void* stream);
+
+/* --------------------------------------------------------- policy training --- */
+
+/*
+ * Log-probabilities and entropies of given tokens from logits, and the gradient of the logits
+ * (what the reference's trainers compute behind the rollout inside GRPOTrainer, whose advantages
+ * fixed_hint_grpo_trainer.py:382-408 and token_prefix_grpo_trainer.py:196-278 produce).  Rows are
+ * the positions (b, t), b < B, t < T: V logits from logits + b * row_stride + t * pos_stride
+ * (elements; consecutive in memory; any alignment), token token_ids[b * ids_stride + t].  With
+ * x the row divided by `temperature`:
+ *   logps = x[token] - lse,  entropy = lse - sum_v p_v x_v,  lse = log sum_v exp(x_v), p = exp(x - lse)
+ * A negative token marks padding: the row is not read, logps = entropy = 0 and its gradient is 0.
+ * A token >= V yields NaN.  Entries of -inf count as probability 0 (gradient 0 unless the token
+ * itself is one: its log-probability is -inf).
+ * Forward writes logps, row_stats and, if not null, entropy, [B * T] each (row_stats two floats per
+ * row, 8-byte aligned: the row's maximum and its sum of exponentials).  Backward reads logits,
+ * token_ids and row_stats as the forward call left them, grad_logps / grad_entropy (either may be
+ * null; grad_entropy needs the forward call's entropy) and writes all of grad_logits
+ * [B * T, V], contiguous, in the logits' type; rows whose gradients are both 0 are not read.
+ * scratch: grx_token_logps_scratch_bytes(B * T, V, dtype) bytes (0 for many rows), 16-byte aligned,
+ * contents need no initialisation; calls that may overlap must not share it.
+ */
+#define GRX_MAX_TOKEN_ROWS (1 << 23)
+typedef struct grx_token_logps_args {
+    const void* logits;
+    int64_t row_stride, pos_stride;
+    const int64_t* token_ids;
+    int64_t ids_stride;
+    int32_t B, T, V;
+    int32_t dtype;             /* GRX_F32 / GRX_BF16 / GRX_F16                        */
+    float temperature;         /* > 0                                                 */
+    int32_t reserved;
+    float* logps;
+    float* row_stats;
+    float* entropy;
+    const float* grad_logps;   /* backward only, as the two below                     */
+    const float* grad_entropy;
+    void* grad_logits;
+} grx_token_logps_args;
+GRX_API size_t grx_token_logps_scratch_bytes(int64_t rows, int32_t V, int32_t dtype);
+GRX_API int grx_token_logps(const grx_token_logps_args* args, void* scratch, size_t scratch_bytes, void* stream);
+GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* stream);
+
+/*
+ * Clipped policy loss with a KL term on [R, T] fp32 log-probabilities.  Per valid token (mask > 0),
+ * with d = logps - old_logps (null: 0) -- or, sequence_level = 1, the mean of that over the row's
+ * valid tokens -- w = exp(d), A the advantage, q = ref_logps - logps (null: no KL):
+ *   l = -min(min(w, delta) A, clip(w, 1 - epsilon_low, 1 + epsilon_high) A) + beta (exp(q) - 1 - q)
+ *   loss = sum over valid tokens of l times: 1 / (R * valid tokens of the row) (row_mean = 1),
+ *          1 / normalizer (normalizer > 0), or 1 / valid tokens of the batch; empty sums are 0.
+ * old_logps, ref_logps and advantages are constants (no gradient).  Masked positions are never
+ * read.  Outputs: loss [1]; stats [4] = mean KL, shares of valid tokens cut at the lower (w below,
+ * A < 0) and upper bound (w above, A > 0), and a factor; unit_grad (fp32 [R, T] contiguous, 16-byte
+ * aligned, or null): grx_policy_loss_backward multiplies it by stats[3] and by the device scalar
+ * `upstream` (dL/dloss) into grad_logps [R * T].
+ * scratch: grx_policy_loss_scratch_bytes(R, T) bytes (0 for small calls), 8-byte aligned, contents
+ * need no initialisation; calls that may overlap must not share it.
+ */
+#define GRX_MASK_U8 0 /* also bool */
+#define GRX_MASK_I32 1
+#define GRX_MASK_I64 2
+#define GRX_MASK_F32 3
+typedef struct grx_policy_loss_args {
+    const float* logps;       int64_t logps_stride;  /* row strides in elements        */
+    const float* old_logps;   int64_t old_stride;
+    const float* ref_logps;   int64_t ref_stride;
+    const float* advantages;  int64_t adv_row_stride, adv_pos_stride; /* 0 position stride: one per row */
+    const void* mask;         int64_t mask_stride;
+    int32_t mask_type;         /* GRX_MASK_*                                          */
+    int32_t R, T;
+    int32_t sequence_level, row_mean;
+    float beta;
+    double epsilon_low, epsilon_high;
+    double delta;              /* 0: off; else above 1 + epsilon_high                 */
+    double normalizer;
+    float* loss;
+    float* stats;
+    float* unit_grad;
+} grx_policy_loss_args;
+GRX_API size_t grx_policy_loss_scratch_bytes(int32_t R, int32_t T);
+GRX_API int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, size_t scratch_bytes, void* stream);
+GRX_API int grx_policy_loss_backward(const float* unit_grad, const float* stats, const float* upstream, int64_t n,
+                                     float* grad_logps, void* stream);
 
 #ifdef __cplusplus
 }

@@ -68,6 +68,10 @@ EXPORTED_SYMBOLS = (
     "grx_token_logps_scratch_bytes",
     "grx_token_logps",
     "grx_token_logps_backward",
+    "grx_lm_token_logps_scratch_bytes",
+    "grx_lm_token_logps_backward_scratch_bytes",
+    "grx_lm_token_logps",
+    "grx_lm_token_logps_backward",
     "grx_policy_loss_scratch_bytes",
     "grx_policy_loss",
     "grx_policy_loss_backward",
@@ -257,6 +261,27 @@ class GrxTokenLogpsArgs(C.Structure):
     ]
 
 
+class GrxLmTokenLogpsArgs(C.Structure):
+    _fields_ = [
+        ("hidden", C.c_void_p),
+        ("hidden_stride", C.c_int64),
+        ("weight", C.c_void_p),
+        ("weight_stride", C.c_int64),
+        ("token_ids", C.c_void_p),
+        ("N", C.c_int32),
+        ("H", C.c_int32),
+        ("V", C.c_int32),
+        ("temperature", C.c_float),
+        ("logps", C.c_void_p),
+        ("row_stats", C.c_void_p),
+        ("entropy", C.c_void_p),
+        ("grad_logps", C.c_void_p),
+        ("grad_entropy", C.c_void_p),
+        ("grad_hidden", C.c_void_p),
+        ("grad_weight", C.c_void_p),
+    ]
+
+
 class GrxPolicyLossArgs(C.Structure):
     _fields_ = [
         ("logps", C.c_void_p),
@@ -404,6 +429,14 @@ def _declare(lib: C.CDLL) -> None:
     lib.grx_token_logps.argtypes = [C.POINTER(GrxTokenLogpsArgs), vp, C.c_size_t, vp]
     lib.grx_token_logps_backward.restype = C.c_int
     lib.grx_token_logps_backward.argtypes = [C.POINTER(GrxTokenLogpsArgs), vp]
+    lib.grx_lm_token_logps_scratch_bytes.restype = C.c_size_t
+    lib.grx_lm_token_logps_scratch_bytes.argtypes = [i32, i32, i32, i32]
+    lib.grx_lm_token_logps_backward_scratch_bytes.restype = C.c_size_t
+    lib.grx_lm_token_logps_backward_scratch_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.grx_lm_token_logps.restype = C.c_int
+    lib.grx_lm_token_logps.argtypes = [C.POINTER(GrxLmTokenLogpsArgs), vp, C.c_size_t, vp]
+    lib.grx_lm_token_logps_backward.restype = C.c_int
+    lib.grx_lm_token_logps_backward.argtypes = [C.POINTER(GrxLmTokenLogpsArgs), vp, C.c_size_t, vp]
     lib.grx_policy_loss_scratch_bytes.restype = C.c_size_t
     lib.grx_policy_loss_scratch_bytes.argtypes = [i32, i32]
     lib.grx_policy_loss.restype = C.c_int

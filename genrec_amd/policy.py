@@ -66,6 +66,14 @@ def _token_ids(ids: torch.Tensor, dev) -> torch.Tensor:
     return _rows_2d(ids.detach().to(torch.int64), "token_ids")
 
 
+def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
+    """[N, H] with rows of consecutive elements that start on 16 bytes."""
+    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _grad_rows(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if g is None else g.to(torch.float32).contiguous()
 
@@ -145,6 +153,96 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
         logits = logits.contiguous()
     out = _TokenLogps.apply(logits, ids, temperature, bool(return_entropy))
     if len(shape) == 2:
+        return out
+    return tuple(t.reshape(shape) for t in out) if return_entropy else out.reshape(shape)
+
+
+class _LmTokenLogps(torch.autograd.Function):
+    @staticmethod
+    def _args(hidden, weight, ids, temperature):
+        a = _lib.GrxLmTokenLogpsArgs()
+        a.hidden, a.hidden_stride = hidden.data_ptr(), hidden.stride(0) if hidden.shape[0] > 1 else hidden.shape[1]
+        a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0) if weight.shape[0] > 1 else weight.shape[1]
+        a.token_ids, a.temperature = ids.data_ptr(), temperature
+        (a.N, a.H), a.V = hidden.shape, weight.shape[0]
+        return a
+
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, temperature, entropy):
+        N = hidden.shape[0]
+        dev = hidden.device
+        a = _LmTokenLogps._args(hidden, weight, ids, temperature)
+        out = torch.empty((2, N) if entropy else (1, N), dtype=torch.float32, device=dev)
+        stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
+        a.logps, a.row_stats = out.data_ptr(), stats.data_ptr()
+        logps, ent = out[0], None
+        if entropy:
+            ent = out[1]
+            a.entropy = ent.data_ptr()
+        index = dev.index
+        lib = _lib.lib()
+        n = lib.grx_lm_token_logps_scratch_bytes(N, a.H, a.V, int(entropy))
+        scratch = _scratch(n, dev)
+        with _lib.on_device(index):
+            _lib.check(lib.grx_lm_token_logps(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
+        ctx.save_for_backward(hidden, weight, ids, stats, *((ent,) if entropy else ()))
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        return (logps, ent) if entropy else logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logps, g_entropy=None):
+        hidden, weight, ids, stats, *rest = ctx.saved_tensors
+        dev = hidden.device
+        a = _LmTokenLogps._args(hidden, weight, ids, ctx.temperature)
+        want_h, want_w = ctx.needs_input_grad[:2]
+        grad_h = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
+        grad_w = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
+        if a.N == 0 and want_w:
+            grad_w.zero_()
+        g_logps, g_entropy = _grad_rows(g_logps), _grad_rows(g_entropy)
+        a.row_stats, a.entropy = stats.data_ptr(), (_ptr(rest[0]) if rest else None)
+        a.grad_logps, a.grad_entropy = _ptr(g_logps), _ptr(g_entropy)
+        a.grad_hidden, a.grad_weight = _ptr(grad_h), _ptr(grad_w)
+        index = dev.index
+        lib = _lib.lib()
+        n = lib.grx_lm_token_logps_backward_scratch_bytes(a.N, a.H, a.V, int(want_h), int(want_w))
+        scratch = _scratch(n, dev)
+        with _lib.on_device(index):
+            _lib.check(lib.grx_lm_token_logps_backward(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
+        return grad_h, grad_w, None, None, None
+
+
+def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor, temperature: float = 1.0,
+                        return_entropy: bool = False):
+    """:func:`token_logps` of ``logits = hidden @ weight.T`` without the logits: the product runs on the matrix cores
+    and is consumed tile by tile, forward and backward (the backward pass forms it again).
+
+    ``hidden`` [B, T, H] or [N, H] and ``weight`` [V, H] (``lm_head.weight``, no bias), bf16, H a multiple of 64, on
+    the GPU; ``token_ids`` [B, T] or [N], negative for padding.  Differentiable in both; a frozen weight costs
+    nothing.  The logits' gradient passes through bf16 on its way to the two products, as it does under autograd.
+    The backward pass takes a scratch tensor of about 1 GB at many rows.  A pass recorded into a HIP graph needs
+    leaves of its own (``detach().requires_grad_()`` inside the recording)."""
+    temperature = _temperature(temperature)
+    if hidden.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
+        raise TypeError(f"hidden states and weight must be bfloat16, got {hidden.dtype} and {weight.dtype}")
+    if hidden.dim() not in (2, 3) or token_ids.shape != hidden.shape[:-1]:
+        raise ValueError(f"hidden must be [..., H] with one row per token id: got {tuple(hidden.shape)} for ids "
+                         f"{tuple(token_ids.shape)}")
+    if weight.dim() != 2 or weight.shape[1] != hidden.shape[-1] or weight.shape[0] < 1:
+        raise ValueError(f"weight must be [V, {hidden.shape[-1]}], got {tuple(weight.shape)}")
+    H = hidden.shape[-1]
+    if H < 64 or H % 64 or H > 1 << 16 or weight.shape[0] > 1 << 24:
+        raise ValueError(f"the hidden size must be a multiple of 64 up to 2^16 and the vocabulary at most 2^24, got "
+                         f"{H}, {weight.shape[0]}")
+    shape = token_ids.shape
+    ids = _token_ids(token_ids, hidden.device).reshape(-1).contiguous()
+    _same_device(hidden.device, weight=weight)
+    _lib.require_cuda(hidden, "hidden")
+    rows = _aligned_rows(hidden.reshape(-1, H))
+    out = _LmTokenLogps.apply(rows, _aligned_rows(weight), ids, temperature, bool(return_entropy))
+    if len(shape) == 1:
         return out
     return tuple(t.reshape(shape) for t in out) if return_entropy else out.reshape(shape)
 

@@ -743,6 +743,39 @@ GRX_API int grx_token_logps(const grx_token_logps_args* args, void* scratch, siz
 GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* stream);
 
 /*
+ * The same from hidden states and the output projection, without logits: x = hidden [N, H] x
+ * weight^T [H, V] / temperature (bf16 operands, fp32 sums; nn.Linear.weight, no bias).  Outputs and
+ * padding as above, [N] each.  Backward writes grad_hidden [N, H] and / or grad_weight [V, H], bf16,
+ * contiguous, 16-byte aligned, all of them (a null one is not computed); the logits' gradient in
+ * between is bf16.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
+ * H a multiple of 64, operand rows 16-byte aligned.  scratch: the bytes that the matching size
+ * function names (backward: a chunk of the logits' gradient, about 1 GB at many rows), 16-byte
+ * aligned, contents need no initialisation; calls that may overlap must not share it.
+ */
+typedef struct grx_lm_token_logps_args {
+    const void* hidden;
+    int64_t hidden_stride;     /* elements                                            */
+    const void* weight;
+    int64_t weight_stride;
+    const int64_t* token_ids;  /* [N], contiguous                                     */
+    int32_t N, H, V;
+    float temperature;
+    float* logps;
+    float* row_stats;
+    float* entropy;
+    const float* grad_logps;   /* backward only, as the three below                   */
+    const float* grad_entropy;
+    void* grad_hidden;
+    void* grad_weight;
+} grx_lm_token_logps_args;
+GRX_API size_t grx_lm_token_logps_scratch_bytes(int32_t N, int32_t H, int32_t V, int32_t entropy);
+GRX_API size_t grx_lm_token_logps_backward_scratch_bytes(int32_t N, int32_t H, int32_t V, int32_t want_hidden,
+                                                         int32_t want_weight);
+GRX_API int grx_lm_token_logps(const grx_lm_token_logps_args* args, void* scratch, size_t scratch_bytes, void* stream);
+GRX_API int grx_lm_token_logps_backward(const grx_lm_token_logps_args* args, void* scratch, size_t scratch_bytes,
+                                        void* stream);
+
+/*
  * Clipped policy loss with a KL term on [R, T] fp32 log-probabilities.  Per valid token (mask > 0),
  * with d = logps - old_logps (null: 0) -- or, sequence_level = 1, the mean of that over the row's
  * valid tokens -- w = exp(d), A the advantage, q = ref_logps - logps (null: no KL):

@@ -1,0 +1,218 @@
+"""GPU: log-probabilities from hidden states and the output projection (``policy.lm_head_token_logps``), against the
+definition in 64 bits.
+
+Tolerances.  u = 2^-24.  A logit is a sum of H exact products of bf16 numbers, added in fp32: off by at most
+H u S, S = sum |hidden weight|.  From there as with logits: the row's sums carry (V / 256 + 160) u, and an error e
+of the logits moves log-probabilities by at most 2 e / T and probabilities by that factor.  The logits' gradient G is
+rounded to bf16 (2^-8 of each element), the products of it with the weight (the hidden states) are added in fp32 over
+V (N) terms and rounded to bf16 once: element by element at most
+    (2^-8 + relative error of G + (terms) u) (|G| |operand|) + 2^-8 |result|."""
+
+import math
+
+import pytest
+import torch
+
+from genrec_amd.policy import lm_head_token_logps, policy_loss, token_logps
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = 2.0 ** -8  # half a step of bf16
+
+
+def _inputs(shape, H, V, seed, pad=0.15):
+    dev = torch.device("cuda", 0)
+    g = torch.Generator(device=dev).manual_seed(seed)
+    hidden = torch.randn((*shape, H), generator=g, device=dev).to(torch.bfloat16)
+    weight = (torch.randn((V, H), generator=g, device=dev) * (2.5 / math.sqrt(H))).to(torch.bfloat16)
+    ids = torch.randint(0, V, shape, generator=g, device=dev)
+    ids[torch.rand(shape, generator=g, device=dev) < pad] = -1
+    gl = torch.randn(shape, generator=g, device=dev)
+    ge = torch.randn(shape, generator=g, device=dev) * 0.2
+    return hidden, weight, ids, gl, ge
+
+
+def _definition(hidden, weight, ids, temperature, g, h):
+    H, V = hidden.shape[-1], weight.shape[0]
+    flat, w, t = hidden.double().reshape(-1, H), weight.double(), ids.reshape(-1)
+    use = t >= 0
+    flat = torch.where(use[:, None], flat, 0.0)
+    x = flat @ w.T / temperature
+    lp = x - x.max(1, keepdim=True).values
+    lp = lp - lp.exp().sum(1, keepdim=True).log()
+    p = lp.exp()
+    at = t.clamp(min=0)[:, None]
+    logps = torch.where(use, lp.gather(1, at)[:, 0], 0.0)
+    ent = torch.where(use, -(p * lp).sum(1), 0.0)
+    G = -p * g.double().reshape(-1, 1)
+    if h is not None:
+        G = G - h.double().reshape(-1, 1) * p * (lp + ent[:, None])
+    G.scatter_add_(1, at, g.double().reshape(-1, 1))
+    G = torch.where(use[:, None], G, 0.0) / temperature
+    err = H * U * float((flat.abs() @ w.abs().T).max()) / temperature
+    return logps, ent, G, flat, w, err, p, lp
+
+
+def _check(hidden, weight, ids, g, h=None, temperature=1.0):
+    x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    made = lm_head_token_logps(x, w, ids, temperature, return_entropy=h is not None)
+    logps, ent = made if h is not None else (made, None)
+    assert logps.dtype == torch.float32 and logps.shape == ids.shape
+    dh, dw = torch.autograd.grad([logps] + ([ent] if h is not None else []), [x, w], [g] + ([h] if h is not None else []))
+    want, want_ent, G, flat, wd, err, p, lp = _definition(hidden, weight, ids, temperature, g, h)
+    N, V = G.shape
+    rel = (V / 256 + 160) * U
+    assert ((logps.double().reshape(-1) - want).abs() <= 2 * err + rel + 6 * U * want.abs()).all()
+    if h is not None:
+        assert ((ent.double().reshape(-1) - want_ent).abs() <= 2 * (2 * err + rel) * (math.log(V) + 2)).all()
+    # an element of G: p (a few factors), its argument error and the row's
+    size = g.double().abs().reshape(-1, 1)
+    if h is not None:
+        size = size + h.double().abs().reshape(-1, 1) * (2 * lp.abs() + math.log(V) + 4)
+    dG = p * size / temperature * (2 * err + rel + 3 * U * (lp.abs() + 20)) * 2 + HALF * G.abs()
+    if h is not None:
+        dG = dG + p * h.double().abs().reshape(-1, 1) / temperature * 4 * (2 * err + rel) * (math.log(V) + 2)
+    dG = dG + 8 * U * size.max() / temperature * (G.abs() > 0)
+    dG[ids.reshape(-1) < 0] = 0.0
+    bound_h = dG @ wd.abs() + V * U * (G.abs() @ wd.abs())
+    bound_w = dG.T @ flat.abs() + N * U * (G.abs().T @ flat.abs())
+    want_h, want_w = G @ wd, G.T @ flat
+    assert dh.shape == hidden.shape and dw.shape == weight.shape and dh.dtype == dw.dtype == torch.bfloat16
+    off = (dh.double().reshape(N, -1) - want_h).abs() - HALF * want_h.abs() - bound_h * (1 + HALF) - 1e-37
+    assert (off <= 0).all(), float(off.max())
+    off = (dw.double() - want_w).abs() - HALF * want_w.abs() - bound_w * (1 + HALF) - 1e-37
+    assert (off <= 0).all(), float(off.max())
+    assert (dh[ids < 0] == 0).all()
+    return logps, ent, dh, dw
+
+
+# row tiles of 64, 128 and 256, tails of both axes, H below and above one tile, several chunks of columns are below
+@pytest.mark.parametrize("shape,H,V", [((1,), 64, 1), ((1, 1), 64, 255), ((3, 5), 128, 300), ((64,), 192, 1000), ((65,), 320, 257),
+                                       ((5, 13), 256, 4099), ((128,), 128, 2048), ((129,), 576, 777), ((7, 40), 64, 5001),
+                                       ((300,), 448, 1531), ((513,), 256, 2500), ((1500,), 128, 513)])
+def test_logps_and_gradients(shape, H, V):
+    hidden, weight, ids, g, h = _inputs(shape, H, V, seed=H + V)
+    _check(hidden, weight, ids, g, None, 1.0)
+    _check(hidden, weight, ids, g, h, 0.8)
+
+
+@pytest.mark.parametrize("N", [5, 320])
+def test_real_vocabulary(N):
+    hidden, weight, ids, g, h = _inputs((N,), 256, 151669, seed=N)
+    _check(hidden, weight, ids, g, h, 1.2)
+
+
+def test_strided_operands_and_one_gradient_only():
+    hidden, weight, ids, g, h = _inputs((6, 9), 192, 1003, seed=4)
+    lp, ent, dh, dw = _check(hidden, weight, ids, g, h)
+    wide_h = torch.zeros((6, 11, 264), dtype=torch.bfloat16, device=hidden.device)
+    wide_w = torch.zeros((1003, 200), dtype=torch.bfloat16, device=hidden.device)
+    for off in (8, 3):  # rows that start on 16 bytes, and rows that do not
+        vh, vw = wide_h[:, 1:10, off : off + 192], wide_w[:, 8:200] if off == 8 else wide_w[:, 3:195]
+        vh.copy_(hidden)
+        vw.copy_(weight)
+        got = _check(vh, vw, ids, g, h)
+        assert torch.equal(got[0], lp) and torch.equal(got[2], dh) and torch.equal(got[3], dw)
+    for need in ((True, False), (False, True)):
+        x, w = hidden.detach().requires_grad_(need[0]), weight.detach().requires_grad_(need[1])
+        a, b = lm_head_token_logps(x, w, ids, return_entropy=True)
+        grads = torch.autograd.grad([a, b], [t for t in (x, w) if t.requires_grad], [g, h])
+        assert torch.equal(grads[0], dh if need[0] else dw)
+
+
+def test_padding_may_hold_anything():
+    hidden, weight, ids, g, h = _inputs((4, 20), 128, 900, seed=5, pad=0.4)
+    g = torch.where(torch.rand(g.shape, device=g.device) < 0.2, torch.zeros_like(g), g)
+    clean = _check(hidden, weight, ids, g)
+    for bad in (math.nan, math.inf):
+        dirty = hidden.clone()
+        dirty[ids < 0] = bad
+        got = _check(dirty, weight, ids, g)
+        assert all(torch.equal(a, b) for a, b in zip((clean[0], clean[2], clean[3]), (got[0], got[2], got[3])))
+    ids = torch.full_like(ids, -1)
+    x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    lp = lm_head_token_logps(x, w, ids)
+    lp.sum().backward()
+    assert (lp == 0).all() and (x.grad == 0).all() and (w.grad == 0).all()
+    ids[0, 0] = 900  # outside the vocabulary
+    assert torch.isnan(lm_head_token_logps(hidden, weight, ids)[0, 0])
+    empty = torch.zeros((0, 128), dtype=torch.bfloat16, device=hidden.device, requires_grad=True)
+    out = lm_head_token_logps(empty, w, torch.zeros(0, dtype=torch.int64, device=hidden.device))
+    (gw,) = torch.autograd.grad(out.sum(), w)
+    assert out.shape == (0,) and (gw == 0).all()
+
+
+def test_agrees_with_the_logits_form():
+    """The same call on the materialised product: log-probabilities to the summation order of the products."""
+    hidden, weight, ids, g, h = _inputs((3, 50), 512, 3001, seed=6)
+    logits = hidden.float() @ weight.float().T
+    a, b = lm_head_token_logps(hidden, weight, ids, 0.9, True), token_logps(logits, ids, 0.9, True)
+    tol = 512 * U * float((hidden.float().abs().reshape(-1, 512) @ weight.float().abs().T).max()) / 0.9
+    assert (a[0] - b[0]).abs().max() <= 4 * tol + 1e-5 and (a[1] - b[1]).abs().max() <= 40 * tol + 1e-4
+
+
+def test_several_chunks_of_columns(monkeypatch):
+    """More rows than one chunk of the logits' gradient holds at this vocabulary: 16,000 x 40,000."""
+    hidden, weight, ids, g, h = _inputs((16000,), 64, 40000, seed=7)
+    x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    lp = lm_head_token_logps(x, w, ids)
+    dh, dw = torch.autograd.grad(lp, [x, w], [g])
+    rows = torch.arange(0, 16000, 61, device=ids.device)
+    want, _, G, flat, wd, err, p, lpa = _definition(hidden[rows], weight, ids[rows], 1.0, g[rows], None)
+    assert ((lp[rows].double() - want).abs() <= 2 * err + (40000 / 256 + 160) * U + 6 * U * want.abs()).all()
+    dG = HALF * G.abs() * 1.01 + 8 * U * g[rows].abs().double()[:, None] * (G.abs() > 0)
+    want_h = G @ wd
+    assert ((dh[rows].double() - want_h).abs() <= HALF * want_h.abs() + dG @ wd.abs() * 1.01 + 40000 * U * (G.abs() @ wd.abs())).all()
+    # a few rows of the weight's gradient from all rows
+    vs = torch.tensor([0, 1, 17000, 33553, 33554, 39999], device=ids.device)
+    flat = torch.where(ids[:, None] >= 0, hidden.double(), 0.0)
+    lse = torch.logsumexp(hidden.double() @ weight.double().T, 1)
+    pv = (hidden.double() @ weight[vs].double().T - lse[:, None]).exp()
+    Gv = torch.where(ids[:, None] >= 0, g.double()[:, None] * ((ids[:, None] == vs[None]).double() - pv), 0.0)
+    want_w = Gv.T @ flat
+    bound = HALF * want_w.abs() + (Gv.abs().T @ flat.abs()) * (HALF * 1.02 + 16000 * U)
+    assert ((dw[vs].double() - want_w).abs() <= bound).all()
+
+
+def _step(hidden, weight, ids, mask, adv, old):
+    x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    lp, ent = lm_head_token_logps(x, w, ids.masked_fill(mask == 0, -1), 0.9, return_entropy=True)
+    res = policy_loss(lp, adv, mask, old, loss_type="bnpo")
+    return res.loss.detach(), *torch.autograd.grad(res.loss - 0.01 * (ent * mask).sum(), [x, w])
+
+
+def test_step_recorded_into_a_graph_and_on_two_streams():
+    def make(seed):
+        hidden, weight, ids, g, h = _inputs((16, 5), 256, 3001, seed=seed, pad=0.0)
+        mask = (torch.arange(5, device=ids.device)[None] < torch.randint(0, 6, (16, 1), device=ids.device)).long()
+        return [hidden, weight, ids, mask, g[:, 0].contiguous(), lm_head_token_logps(hidden, weight, ids) + 0.1 * h]
+
+    bufs = make(10)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(*bufs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        made = _step(*bufs)
+    for seed in (11, 12, 13):
+        new = make(seed)
+        for b, n in zip(bufs, new):
+            b.copy_(n)
+        want = _step(*new)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(made, want))
+    pair = [make(14), make(15)]
+    want = [_step(*p) for p in pair]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got[i] = _step(*pair[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))

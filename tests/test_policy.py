@@ -132,3 +132,58 @@ def test_policy_loss_backward_c_entry_refuses():
     assert lib.grx_policy_loss_backward(0x10000, 0x20000, None, 5, 0x30000, None) == -1
     assert lib.grx_policy_loss_backward(0x10004, 0x20000, 0x20010, 5, 0x30000, None) == -1
     assert b"misaligned" in lib.grx_last_error()
+
+
+def _bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("hidden,weight,ids,error,match", [
+    (torch.zeros(2, 64), _bf(8, 64), torch.zeros(2, dtype=torch.int64), TypeError, "bfloat16"),
+    (_bf(2, 64), _bf(8, 64).float(), torch.zeros(2, dtype=torch.int64), TypeError, "bfloat16"),
+    (_bf(2, 64), _bf(8, 64), torch.zeros(3, dtype=torch.int64), ValueError, "one row per token"),
+    (_bf(2, 64), _bf(8, 128), torch.zeros(2, dtype=torch.int64), ValueError, "weight must be"),
+    (_bf(2, 64), _bf(0, 64), torch.zeros(2, dtype=torch.int64), ValueError, "weight must be"),
+    (_bf(2, 96), _bf(8, 96), torch.zeros(2, dtype=torch.int64), ValueError, "multiple of 64"),
+    (_bf(2, 0), _bf(8, 0), torch.zeros(2, dtype=torch.int64), ValueError, "multiple of 64"),
+    (_bf(2, 64), _bf(8, 64), torch.zeros(2), TypeError, "integers"),
+    (_bf(2, 64), _bf(8, 64), torch.zeros(2, dtype=torch.int64), _lib.GenrecHipError, "must live on the GPU"),
+])
+def test_lm_head_token_logps_refuses(hidden, weight, ids, error, match):
+    with pytest.raises(error, match=match):
+        policy.lm_head_token_logps(hidden, weight, ids)
+
+
+@pytest.mark.parametrize("over,code,match", [
+    (dict(V=0), -1, b"bad shape"),
+    (dict(H=96), -3, b"multiple of 64"),
+    (dict(H=1 << 17, hidden_stride=1 << 17, weight_stride=1 << 17), -3, b"2^16"),
+    (dict(N=(1 << 23) + 1), -3, b"rows"),
+    (dict(temperature=-1.0), -1, b"temperature"),
+    (dict(hidden_stride=100), -1, b"operand rows"),
+    (dict(weight_stride=56), -1, b"operand rows"),
+    (dict(weight=None), -1, b"null buffer"),
+    (dict(hidden=0x10008), -1, b"misaligned"),
+])
+def test_lm_head_c_entries_refuse(over, code, match):
+    lib = _lib.lib()
+    a = _lib.GrxLmTokenLogpsArgs()
+    a.hidden, a.weight, a.token_ids, a.logps, a.row_stats, a.grad_hidden = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 0x60000
+    a.N, a.H, a.V, a.temperature, a.hidden_stride, a.weight_stride = 4, 64, 100, 1.0, 64, 64
+    for k, v in over.items():
+        setattr(a, k, v)
+    assert lib.grx_lm_token_logps(C.byref(a), None, 0, None) == code and match in lib.grx_last_error()
+    assert lib.grx_lm_token_logps_backward(C.byref(a), None, 0, None) == code and match in lib.grx_last_error()
+
+
+def test_lm_head_c_entries_refuse_short_scratch():
+    lib = _lib.lib()
+    a = _lib.GrxLmTokenLogpsArgs()
+    a.hidden, a.weight, a.token_ids, a.logps, a.row_stats, a.grad_hidden = 0x10000, 0x20000, 0x30000, 0x40000, 0x50000, 0x60000
+    a.N, a.H, a.V, a.temperature, a.hidden_stride, a.weight_stride = 4, 64, 100, 1.0, 64, 64
+    n = lib.grx_lm_token_logps_scratch_bytes(4, 64, 100, 0)
+    assert n > 0 and lib.grx_lm_token_logps(C.byref(a), 0x70000, n - 1, None) == -4
+    n = lib.grx_lm_token_logps_backward_scratch_bytes(4, 64, 100, 1, 0)
+    assert n > 0 and lib.grx_lm_token_logps_backward(C.byref(a), 0x70000, n - 1, None) == -4
+    a.grad_entropy = 0x80000
+    assert lib.grx_lm_token_logps_backward(C.byref(a), 0x70000, n, None) == -1 and b"entropies" in lib.grx_last_error()

@@ -15,108 +15,129 @@
 #include "lse_math.h"
 #include "mfma_tile.h"
 
-#define LL_FLOOR (-200.f)
+#define LL_FLOOR (-200.f)           // 2^-200 is 0 in fp32: keeps 0 * -inf out of the entropy sums
+#define LL_CUS 256
+#ifndef LL_CHUNK_BYTES
 #define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk
+#endif
+
+struct LlOperands {
+    const uint16_t* weight;     // [V, H]
+    int64_t weight_ld;
+    const uint16_t* hidden;     // [N, H]
+    int64_t hidden_ld;
+    int N, H, V;
+};
 
 struct LlArgs {
-    MtOperand w, h;             // weight [V, H], hidden [N, H]
-    int N, H, V;
+    LlOperands o;
     int m_tiles, n_tiles;
     float k;                    // log2(e) / temperature
     const int64_t* ids;         // [N]
-    float2* partials;           // [m_tiles][n_pad] (max, sum)
-    float* weighted;            // [m_tiles][n_pad], with entropies
+    float2* partials;           // [parts][n_pad] (max, sum), parts = m_tiles x waves along m
+    float* weighted;            // [parts][n_pad], with entropies
     int64_t n_pad;
     float* chosen;              // [N] logit of the row's token
 };
 
 template <int BN>
+using LlLogits = MtPipe<BN, MtAlong<MT_BM>, MtReadAlong, MtAlong<BN>, MtReadAlong>;
+
+template <int BN>
+__device__ __forceinline__ void ll_begin(LlLogits<BN>& pipe, const LlOperands& o, int v0, int r0) {
+    pipe.begin(MtAlong<MT_BM>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN>(o.hidden, o.hidden_ld, o.N, r0, 0), o.H / MT_BK);
+}
+
+// As many workgroups as run at a time; each takes every gridDim-th tile and starts the next one's copies before it
+// turns to its own results.  Those stay inside the wave: a row's sums over the wave's columns are one partial.
+template <int BN, bool ENT>
 __global__ __launch_bounds__(MT_THREADS) void lm_logps_kernel(LlArgs a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = mt_wave();
+    const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    const int tiles = a.m_tiles * a.n_tiles;
+    LlLogits<BN> pipe(lds);
     int tm, tn;
     mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    const int v0 = tm * MT_BM, r0 = tn * BN;
-    mt_f32x16 acc[S::MA][S::NB];
-    mt_multiply<BN, false, false>(acc, lds, a.w, v0, a.h, r0, 0, a.H / MT_BK);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
-    float* red = reinterpret_cast<float*>(lds);  // [3][WM][BN]
-    const bool ent = a.weighted != nullptr;
+    ll_begin(pipe, a.o, tm * MT_BM, tn * BN);
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int v0 = tm * MT_BM, r0 = tn * BN, part = tm * S::WM + wm;
+        int64_t id[S::NB];
 #pragma unroll
-    for (int n = 0; n < S::NB; ++n) {
-        const int in_tile = wn * S::NB * 32 + n * 32 + (lane & 31);
-        const int r = r0 + in_tile;
-        float mx = -INFINITY;
+        for (int n = 0; n < S::NB; ++n) {
+            const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+            id[n] = r < a.o.N ? a.ids[r] : -1;
+        }
+        typename LlLogits<BN>::Acc acc;
+        pipe.run(acc);
+        if (tile + (int)gridDim.x < tiles) {
+            mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
+            ll_begin(pipe, a.o, tm * MT_BM, tn * BN);
+        }
         const int vw = v0 + wm * S::MA * 32 + 4 * half;  // vocabulary entry of m = 0, e = 0
 #pragma unroll
-        for (int m = 0; m < S::MA; ++m)
+        for (int n = 0; n < S::NB; ++n) {
+            const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+            if (v0 + MT_BM > a.o.V) {  // the last tile
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                if (vw + m * 32 + (e & 3) + 8 * (e >> 2) >= a.V) acc[m][n][e] = -INFINITY;
-                mx = fmaxf(mx, acc[m][n][e]);
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (vw + m * 32 + (e & 3) + 8 * (e >> 2) >= a.o.V) acc[m][n][e] = -INFINITY;
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));  // the other half of the lanes holds the same row
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        float s = 0.f, u = 0.f;
-#pragma unroll
-        for (int m = 0; m < S::MA; ++m)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float t = (acc[m][n][e] - ref) * a.k;
-                const float w = fast_exp2(t);
-                s += w;
-                if (ent) u = fmaf(w, fmaxf(t, LL_FLOOR), u);
-            }
-        s += __shfl_xor(s, 32, 64);
-        u += __shfl_xor(u, 32, 64);
-        if (half == 0) {
-            red[wm * BN + in_tile] = mx;
-            red[(S::WM + wm) * BN + in_tile] = s;
-            red[(2 * S::WM + wm) * BN + in_tile] = u;
-        }
-        const int64_t id = r < a.N ? a.ids[r] : -1;
-        const int64_t off = id - vw;  // 4 consecutive entries, every 8
-        if (off >= 0 && off < S::MA * 32 && (off & 4) == 0) {
-            const int at = (int)(off >> 5) * 16 + (int)((off & 31) >> 3) * 4 + (int)(off & 3);
+            float mx = -INFINITY;
 #pragma unroll
             for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (m * 16 + e == at) a.chosen[r] = acc[m][n][e];
-        }
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < BN) {
-        const int i = threadIdx.x;
-        float m = red[i];
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, acc[m][n][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));  // the other half of the lanes holds the same row
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            float s0 = 0.f, s1 = 0.f, u = 0.f;
 #pragma unroll
-        for (int w = 1; w < S::WM; ++w) m = fmaxf(m, red[w * BN + i]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float s = 0.f, u = 0.f;
+            for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-        for (int w = 0; w < S::WM; ++w) {
-            const float d = fmaxf((red[w * BN + i] - ref) * a.k, LL_FLOOR), f = fast_exp2(d), sw = red[(S::WM + w) * BN + i];
-            s = fmaf(sw, f, s);
-            u += (red[(2 * S::WM + w) * BN + i] + sw * d) * f;
+                for (int e = 0; e < 16; ++e) {
+                    const float t = (acc[m][n][e] - ref) * a.k;
+                    const float w = fast_exp2(t);
+                    if (e & 1) s1 += w; else s0 += w;
+                    if (ENT) u = fmaf(w, fmaxf(t, LL_FLOOR), u);
+                }
+            float s = s0 + s1;
+            s += __shfl_xor(s, 32, 64);
+            if (ENT) u += __shfl_xor(u, 32, 64);
+            if (half == 0) {
+                a.partials[(int64_t)part * a.n_pad + r] = make_float2(mx, s);
+                if (ENT) a.weighted[(int64_t)part * a.n_pad + r] = u;
+            }
+            const int64_t off = id[n] - vw;  // runs of four entries, every eight
+            if (off >= 0 && off < S::MA * 32 && (off & 4) == 0) {
+                const int at = (int)(off >> 5) * 16 + (int)((off & 31) >> 3) * 4 + (int)(off & 3);
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (m * 16 + e == at) a.chosen[r] = acc[m][n][e];
+            }
         }
-        a.partials[(int64_t)tm * a.n_pad + r0 + i] = make_float2(m, s);
-        if (ent) a.weighted[(int64_t)tm * a.n_pad + r0 + i] = u;
     }
 }
 
 struct LlJoin {
     LlArgs g;
+    int parts;
     float* logps;
     float2* stats;
     float* entropy;
 };
 
-// Joins a row's column tiles: 16 rows per workgroup, 16 threads a row.
+// Joins a row's partials, ROWS rows per workgroup.
+template <int ROWS>
 __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
-    __shared__ float sm[16][17], ss[16][17], su[16][17];
-    const int i = threadIdx.x & 15, j = threadIdx.x >> 4;
-    const int r = blockIdx.x * 16 + i;
+    constexpr int PER = 256 / ROWS;  // threads a row
+    __shared__ float sm[PER][ROWS + 1], ss[PER][ROWS + 1], su[PER][ROWS + 1];
+    const int i = threadIdx.x % ROWS, j = threadIdx.x / ROWS;
+    const int r = blockIdx.x * ROWS + i;  // n_pad is a multiple of 64: rows past N read what a clamped row left
     const float k = a.g.k;
     float m = -INFINITY, s = 0.f, u = 0.f;
     auto add = [&](float pm, float ps, float pu) {
@@ -128,16 +149,24 @@ __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
         s = s * fa + ps * fb;
         m = mn;
     };
-    for (int t = j; t < a.g.m_tiles; t += 16) {  // n_pad is a multiple of 64: rows past N read what a clamped row left
+    for (int t = j; t < a.parts; t += PER) {
         const float2 p = a.g.partials[(int64_t)t * a.g.n_pad + r];
         add(p.x, p.y, a.entropy ? a.g.weighted[(int64_t)t * a.g.n_pad + r] : 0.f);
     }
     sm[j][i] = m;
     ss[j][i] = s;
     su[j][i] = u;
-    __syncthreads();
-    if (j != 0 || r >= a.g.N) return;
-    for (int w = 1; w < 16; ++w) add(sm[w][i], ss[w][i], su[w][i]);
+#pragma unroll
+    for (int half = PER / 2; half > 0; half >>= 1) {  // in a fixed order
+        __syncthreads();
+        if (j < half) {
+            add(sm[j + half][i], ss[j + half][i], su[j + half][i]);
+            sm[j][i] = m;
+            ss[j][i] = s;
+            su[j][i] = u;
+        }
+    }
+    if (j != 0 || r >= a.g.o.N) return;
     const int64_t id = a.g.ids[r];
     const float ln2 = 0.69314718055994531f;
     const float ls = log2f(s);
@@ -147,7 +176,7 @@ __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
         if (a.entropy) a.entropy[r] = 0.f;
         return;
     }
-    a.logps[r] = id < a.g.V ? ((a.g.chosen[r] - m) * k - ls) * ln2 : NAN;
+    a.logps[r] = id < a.g.o.V ? ((a.g.chosen[r] - m) * k - ls) * ln2 : NAN;
     a.stats[r] = make_float2(m, s);
     if (a.entropy) a.entropy[r] = (ls - u / s) * ln2;
 }
@@ -162,106 +191,147 @@ struct LlRow {
 };
 
 struct LlPrep {
+    LlOperands o;
     const int64_t* ids;
     const float2* stats;
     const float* entropy;
     const float* g;
     const float* h;
     float inv_t;
-    int N, V, H;
-    LlRow* rows;               // [n_pad]
-    const uint16_t* hidden;
-    int64_t hidden_ld;
-    uint16_t* copy;            // [n_pad][H]: hidden with 0 in the rows that do not count; null: not needed
+    LlRow* rows;               // one per row of the n tiles
+    char* copy;                // hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4]; null: not needed
 };
 
+// Workgroup (64 rows, 32 h).  The copy holds 0 in the rows that do not count.
 __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
-    const int r = blockIdx.x;
-    float g = 0.f, h = 0.f;
-    int64_t id = -1;
-    if (r < a.N) {
-        id = a.ids[r];
-        if (id >= 0) {
-            g = a.g ? a.g[r] : 0.f;
-            h = a.h ? a.h[r] : 0.f;
+    __shared__ bool live[64];
+    const int r0 = blockIdx.x * 64;
+    if (threadIdx.x < 64) {
+        const int r = r0 + threadIdx.x;
+        float g = 0.f, h = 0.f;
+        int64_t id = -1;
+        if (r < a.o.N) {
+            id = a.ids[r];
+            if (id >= 0) {
+                g = a.g ? a.g[r] : 0.f;
+                h = a.h ? a.h[r] : 0.f;
+            }
+        }
+        const bool counts = g != 0.f || h != 0.f;
+        live[threadIdx.x] = counts;
+        if (blockIdx.y == 0) {
+            LlRow o = {0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}};
+            if (counts) {
+                const float2 st = a.stats[r];
+                const float ln2 = 0.69314718055994531f;
+                o.m = st.x;
+                o.alpha = -(g + (a.h ? h * (a.entropy[r] - log2f(st.y) * ln2) : 0.f)) * a.inv_t / st.y;
+                o.beta = -h * ln2 * a.inv_t / st.y;
+                o.at = g * a.inv_t;
+                if (id >= a.o.V) o.alpha = NAN;
+                o.tok = id < a.o.V ? (int)id : 0;
+            }
+            a.rows[r] = o;
         }
     }
-    const bool live = g != 0.f || h != 0.f;
-    if (threadIdx.x == 0) {
-        LlRow o = {0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}};
-        if (live) {
-            const float2 st = a.stats[r];
-            const float ln2 = 0.69314718055994531f;
-            o.m = st.x;
-            o.alpha = -(g + (a.h ? h * (a.entropy[r] - log2f(st.y) * ln2) : 0.f)) * a.inv_t / st.y;
-            o.beta = -h * ln2 * a.inv_t / st.y;
-            o.at = id < a.V ? g * a.inv_t : NAN;
-            if (id >= a.V) o.alpha = NAN;
-            o.tok = id < a.V ? (int)id : 0;
-        }
-        a.rows[r] = o;
-    }
-    if (a.copy) {
-        uint4* d = reinterpret_cast<uint4*>(a.copy + (int64_t)r * a.H);
-        const uint4* s = reinterpret_cast<const uint4*>(a.hidden + (int64_t)r * a.hidden_ld);
-        for (int i = threadIdx.x; i < a.H / 8; i += 256) d[i] = live ? s[i] : make_uint4(0, 0, 0, 0);
-    }
+    if (a.copy == nullptr || r0 >= a.o.N) return;
+    __syncthreads();
+    const int lane = threadIdx.x & 63, n0 = (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = live[n0 + j] ? a.o.hidden[(int64_t)(r0 + n0 + j) * a.o.hidden_ld + h] : (uint16_t)0;
+    *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
+// G of a chunk of columns, in fragment blocks of 32 n x 16 v, [tile of BN n][64 v][BN / 32][4]: a wave's results are
+// such blocks already, so a store is 1 KB in one piece, and both products read it in pieces of 8 KB and more.
 struct LlGrad {
-    MtOperand w, h;
-    int N, H, V;
+    LlOperands o;
     int m_tiles, n_tiles;
-    int v_begin;               // first column of the chunk
+    int v_begin, v64;          // first column of the chunk, its width in 64s
     float k;
     const LlRow* rows;
-    uint16_t* out;             // [n_pad][ld]
-    int64_t ld;
-    int n_pad;
+    char* out;
 };
 
-template <int BN>
+template <int BN, bool ENT>
 __global__ __launch_bounds__(MT_THREADS) void lm_logps_dlogits_kernel(LlGrad a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = mt_wave();
+    const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    const int tiles = a.m_tiles * a.n_tiles;
+    LlLogits<BN> pipe(lds);
     int tm, tn;
     mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    const int c0 = tm * MT_BM, v0 = a.v_begin + c0, r0 = tn * BN;
-    mt_f32x16 acc[S::MA][S::NB];
-    mt_multiply<BN, false, false>(acc, lds, a.w, v0, a.h, r0, 0, a.H / MT_BK);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int v0 = a.v_begin + tm * MT_BM, r0 = tn * BN;
+        char* const out = a.out + ((int64_t)tn * a.v64 + tm * 4) * (BN * 128) + lane * 16;
+        LlRow row[S::NB];
 #pragma unroll
-    for (int n = 0; n < S::NB; ++n) {
-        const int r = r0 + wn * S::NB * 32 + n * 32 + (lane & 31);
-        if (r >= a.n_pad) continue;
-        const LlRow row = a.rows[r];
-        uint16_t* out = a.out + (int64_t)r * a.ld + c0 + wm * S::MA * 32 + 4 * half;
+        for (int n = 0; n < S::NB; ++n) row[n] = a.rows[r0 + (wn * S::NB + n) * 32 + (lane & 31)];
+        typename LlLogits<BN>::Acc acc;
+        pipe.run(acc);
+        if (tile + (int)gridDim.x < tiles) {
+            mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
+            ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
+        }
         const int vw = v0 + wm * S::MA * 32 + 4 * half;
-        const int tok = row.tok - vw;
 #pragma unroll
-        for (int m = 0; m < S::MA; ++m)
+        for (int n = 0; n < S::NB; ++n) {
+            const float m0 = row[n].m, alpha = row[n].alpha, beta = row[n].beta;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                mt_f32x4 d;
+            for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int off = m * 32 + 8 * q + j;
-                    const float t = (acc[m][n][q * 4 + j] - row.m) * a.k;
-                    float v = fast_exp2(t) * fmaf(row.beta, fmaxf(t, LL_FLOOR), row.alpha);
-                    if (off == tok) v += row.at;
-                    d[j] = row.tok >= 0 && vw + off < a.V ? v : 0.f;
+                for (int e = 0; e < 16; ++e) {
+                    const float t = (acc[m][n][e] - m0) * a.k;
+                    acc[m][n][e] = fast_exp2(t) * (ENT ? fmaf(beta, fmaxf(t, LL_FLOOR), alpha) : alpha);
                 }
-                *reinterpret_cast<mt_b16x4*>(out + m * 32 + 8 * q) = __builtin_convertvector(d, mt_b16x4);
+            const int off = row[n].tok - vw;  // runs of four entries, every eight
+            if (row[n].tok >= 0 && off >= 0 && off < S::MA * 32 && (off & 4) == 0) {
+                const int at = (off >> 5) * 16 + ((off & 31) >> 3) * 4 + (off & 3);
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (m * 16 + e == at) acc[m][n][e] += row[n].at;
             }
+            const bool dead = row[n].tok < 0;
+            if (__any(dead)) {
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) acc[m][n][e] = dead ? 0.f : acc[m][n][e];
+            }
+            if (v0 + MT_BM > a.o.V) {  // the last tile
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if (vw + m * 32 + (e & 3) + 8 * (e >> 2) >= a.o.V) acc[m][n][e] = 0.f;
+            }
+#pragma unroll
+            for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const mt_f32x16& c = acc[m][n];
+                    const mt_f32x4 x = {c[8 * q], c[8 * q + 1], c[8 * q + 2], c[8 * q + 3]};
+                    const mt_f32x4 y = {c[8 * q + 4], c[8 * q + 5], c[8 * q + 6], c[8 * q + 7]};
+                    const int v16 = (wm * S::MA + m) * 2 + q;
+                    *reinterpret_cast<mt_u32x4*>(out + (v16 >> 2) * (BN * 128) + ((wn * S::NB + n) * 4 + (v16 & 3)) * 1024) =
+                        mt_pack8(x, y);
+                }
+        }
     }
 }
 
 // d hidden: C[n][h] = sum over the chunk's columns of G[n][v] weight[v][h], fp32 slabs, one per split of the columns.
 struct LlDh {
-    MtOperand w, g;            // weight rows of the chunk (k across), G (k along)
-    int N, H;
-    int m_tiles, n_tiles, splits, steps, steps_per;
+    LlOperands o;
+    const char* g;
+    int m_tiles, n_tiles, splits, steps, steps_per, v_begin, v64;
     int add;                   // 1: add to what the chunk before left
     float* slabs;              // [splits][N][H]
 };
@@ -270,26 +340,32 @@ template <int BN>
 __global__ __launch_bounds__(MT_THREADS) void lm_logps_dhidden_kernel(LlDh a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
-    const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
-    const int tm = tile % a.m_tiles, tn = tile / a.m_tiles;
+    // one XCD takes neighbouring tiles: all h tiles of a few n tiles, which share G
+    const int total = a.splits * a.m_tiles * a.n_tiles, xcd = blockIdx.x & 7;
+    const int id = xcd * (total >> 3) + (xcd < (total & 7) ? xcd : total & 7) + (int)(blockIdx.x >> 3);
+    const int tm = id % a.m_tiles, rest = id / a.m_tiles;
+    const int tn = rest % a.n_tiles, split = rest / a.n_tiles;
     const int h0 = tm * MT_BM, r0 = tn * BN;
     const int s0 = split * a.steps_per, s1 = s0 + a.steps_per < a.steps ? s0 + a.steps_per : a.steps;
-    mt_f32x16 acc[S::MA][S::NB];
-    mt_multiply<BN, true, false>(acc, lds, a.w, h0, a.g, r0, s0 * MT_BK, s1 - s0);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    MtPipe<BN, MtAcross, MtReadAcross, MtBlocksAlong<BN>, MtReadBlocksAlong> pipe(lds);
+    typename decltype(pipe)::Acc acc;
+    pipe.begin(MtAcross(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
+               MtBlocksAlong<BN>(a.g + ((int64_t)tn * a.v64 + s0) * (BN * 128), BN * 128, BN / 32), s1 - s0);
+    pipe.run(acc);
+    const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
-    float* slab = a.slabs + (int64_t)split * a.N * a.H;
+    float* slab = a.slabs + (int64_t)split * a.o.N * a.o.H;
 #pragma unroll
     for (int n = 0; n < S::NB; ++n) {
-        const int r = r0 + wn * S::NB * 32 + n * 32 + (lane & 31);
-        if (r >= a.N) continue;
+        const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+        if (r >= a.o.N) continue;
 #pragma unroll
         for (int m = 0; m < S::MA; ++m)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int h = h0 + wm * S::MA * 32 + m * 32 + 8 * q + 4 * half;
-                if (h >= a.H) continue;
-                mt_f32x4* o = reinterpret_cast<mt_f32x4*>(slab + (int64_t)r * a.H + h);
+                const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
+                if (h >= a.o.H) continue;
+                mt_f32x4* o = reinterpret_cast<mt_f32x4*>(slab + (int64_t)r * a.o.H + h);
                 mt_f32x4 v = {acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
                 if (a.add) v += *o;
                 *o = v;
@@ -310,36 +386,55 @@ __global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(const float*
 
 // d weight of the chunk: C[v][h] = sum over the rows of G[n][v] hidden[n][h].
 struct LlDw {
-    MtOperand h, g;            // hidden copy (k across), G (k across)
-    int H, V;
-    int m_tiles, n_tiles, steps;
-    int v_begin;
+    const char* copy;
+    const char* g;
+    int H, V, bn;
+    int m_tiles, n_tiles, steps, v_begin, v64;
     uint16_t* out;             // [V][H]
 };
+
+typedef MtPipe<256, MtBlocksAlong<MT_BM>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross> LlDwPipe;
+
+// Eight v tiles at a time, one per XCD, all h tiles of each: G is read by one XCD.
+__device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int tile, int& h0, int& c0) {
+    const int group = tile / (8 * a.m_tiles), left = a.n_tiles - group * 8, wide = left < 8 ? left : 8;
+    const int rest = tile - group * 8 * a.m_tiles;
+    h0 = rest / wide * MT_BM;
+    c0 = (group * 8 + rest % wide) * 256;
+    pipe.begin(MtBlocksAlong<MT_BM>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, a.H / 32 - h0 / 32),
+               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * (a.bn * 128), (int64_t)a.v64 * (a.bn * 128), a.bn), a.steps);
+}
 
 __global__ __launch_bounds__(MT_THREADS) void lm_logps_dweight_kernel(LlDw a) {
     typedef MtShape<256> S;
     extern __shared__ __align__(16) unsigned char lds[];
-    int tm, tn;
-    mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    const int h0 = tm * MT_BM, c0 = tn * 256;
-    mt_f32x16 acc[S::MA][S::NB];
-    mt_multiply<256, true, true>(acc, lds, a.h, h0, a.g, c0, 0, a.steps);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    const int tiles = a.m_tiles * a.n_tiles;
+    LlDwPipe pipe(lds);
+    int h_next, c_next;
+    ll_dw_begin(pipe, a, blockIdx.x, h_next, c_next);
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int h0 = h_next, c0 = c_next;
+        LlDwPipe::Acc acc;
+        pipe.run(acc);
+        if (tile + (int)gridDim.x < tiles) ll_dw_begin(pipe, a, tile + gridDim.x, h_next, c_next);
 #pragma unroll
-    for (int n = 0; n < S::NB; ++n) {
-        const int v = a.v_begin + c0 + wn * S::NB * 32 + n * 32 + (lane & 31);
-        if (v >= a.V) continue;
+        for (int n = 0; n < S::NB; ++n) {
+            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
+            uint16_t* const out = a.out + (int64_t)v * a.H;
 #pragma unroll
-        for (int m = 0; m < S::MA; ++m)
+            for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int h = h0 + wm * S::MA * 32 + m * 32 + 8 * q + 4 * half;
-                if (h >= a.H) continue;
-                const mt_f32x4 x = {acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
-                *reinterpret_cast<mt_b16x4*>(a.out + (int64_t)v * a.H + h) = __builtin_convertvector(x, mt_b16x4);
-            }
+                for (int q = 0; q < 2; ++q) {
+                    const mt_f32x16& c = acc[m][n];
+                    const mt_f32x4 x = {c[8 * q], c[8 * q + 1], c[8 * q + 2], c[8 * q + 3]};
+                    const mt_f32x4 y = {c[8 * q + 4], c[8 * q + 5], c[8 * q + 6], c[8 * q + 7]};
+                    const mt_u32x4 packed = mt_pack8(x, y);
+                    const int h = h0 + (wm * S::MA + m) * 32 + 16 * q + 8 * half;
+                    if (v < a.V && h < a.H) *reinterpret_cast<mt_u32x4*>(out + h) = packed;
+                }
+        }
     }
 }
 
@@ -350,40 +445,43 @@ static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 static int ll_bn(int N) { return N <= 64 ? 64 : N <= 128 ? 128 : 256; }
 
 struct LlForward {
-    int bn, m_tiles, n_tiles;
+    int bn, m_tiles, n_tiles, parts;
     int64_t n_pad;
     size_t partials, weighted, chosen, total;  // byte offsets, total size
 };
+
+static int ll_wm(int bn) { return bn == 64 ? MtShape<64>::WM : bn == 128 ? MtShape<128>::WM : MtShape<256>::WM; }
 
 static LlForward ll_forward(int N, int V, bool ent) {
     LlForward f;
     f.bn = ll_bn(N);
     f.m_tiles = (V + MT_BM - 1) / MT_BM;
     f.n_tiles = (N + f.bn - 1) / f.bn;
+    f.parts = f.m_tiles * ll_wm(f.bn);
     f.n_pad = (int64_t)f.n_tiles * f.bn;
     f.partials = 0;
-    f.weighted = (size_t)f.m_tiles * f.n_pad * sizeof(float2);
-    f.chosen = f.weighted + (ent ? (size_t)f.m_tiles * f.n_pad * sizeof(float) : 0);
+    f.weighted = (size_t)f.parts * f.n_pad * sizeof(float2);
+    f.chosen = f.weighted + (ent ? (size_t)f.parts * f.n_pad * sizeof(float) : 0);
     f.total = f.chosen + (size_t)N * sizeof(float);
     return f;
 }
 
 struct LlBackward {
     int bn, n_tiles, h_tiles;
-    int64_t n_pad;             // rows of G: a multiple of 64, the step of d weight's sum
+    int64_t n_pad;             // rows of G: whole tiles
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
     int splits;
     size_t rows, copy, g, slabs, total;
 };
 
-// Splits of d hidden's sum: as many as fill the 256 CUs evenly, each at least eight steps long.
-static int ll_splits(int tiles, int64_t steps) {
+// Splits of d hidden's sum: as many as fill the CUs evenly, each at least eight steps long.
+static int ll_splits(int64_t tiles, int64_t steps) {
     int best = 1;
     double best_use = 0.0;
     for (int s = 1; s <= 64 && (s == 1 || steps / s >= 8); ++s) {
-        const int64_t wgs = (int64_t)tiles * s;
-        const double use = (double)wgs / (double)(ll_up(wgs, 256));
+        const int64_t wgs = tiles * s;
+        const double use = (double)wgs / (double)(ll_up(wgs, LL_CUS));
         if (use > best_use + 0.04) {
             best_use = use;
             best = s;
@@ -397,18 +495,18 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.bn = ll_bn(N);
     b.n_tiles = (N + b.bn - 1) / b.bn;
     b.h_tiles = (H + MT_BM - 1) / MT_BM;
-    b.n_pad = ll_up(N, MT_BK);
+    b.n_pad = (int64_t)b.n_tiles * b.bn;
     const int64_t v_pad = ll_up(V, MT_BM);
     int64_t most = LL_CHUNK_BYTES / 2 / b.n_pad / MT_BM * MT_BM;
     if (most < MT_BM) most = MT_BM;
     b.n_chunks = (int)((v_pad + most - 1) / most);
     b.chunk = ll_up((v_pad + b.n_chunks - 1) / b.n_chunks, MT_BM);
     b.n_chunks = (int)((v_pad + b.chunk - 1) / b.chunk);
-    b.splits = ll_splits(b.h_tiles * b.n_tiles, b.chunk / MT_BK);
+    b.splits = ll_splits((int64_t)b.h_tiles * b.n_tiles, b.chunk / MT_BK);
     b.rows = 0;
     b.copy = (size_t)ll_up(b.n_pad * sizeof(LlRow), 256);
-    b.g = b.copy + (want_w ? (size_t)ll_up(b.n_pad * H * 2, 256) : 0);
-    b.slabs = b.g + (size_t)ll_up(b.n_pad * b.chunk * 2, 256);
+    b.g = b.copy + (want_w ? (size_t)ll_up(N, MT_BK) * H * 2 : 0);
+    b.slabs = b.g + (size_t)(b.n_pad * b.chunk * 2);
     b.total = b.slabs + (want_h ? (size_t)b.splits * N * H * sizeof(float) : 0);
     return b;
 }
@@ -433,6 +531,8 @@ static int ll_check(const char* who, const grx_lm_token_logps_args* p) {
     GRX_REQUIRE(p->temperature > 0.f && p->temperature < INFINITY, GRX_E_INVALID, "%s: temperature must be positive", who);
     GRX_REQUIRE(p->hidden_stride >= p->H && p->weight_stride >= p->H && p->hidden_stride % 8 == 0 && p->weight_stride % 8 == 0,
                 GRX_E_INVALID, "%s: operand rows must be 16-byte aligned and at least H long", who);
+    GRX_REQUIRE(p->hidden_stride <= (1 << 22) && p->weight_stride <= (1 << 22), GRX_E_UNSUPPORTED,
+                "%s: operand rows more than 2^22 elements apart", who);
     if (p->N == 0) return GRX_OK;
     GRX_REQUIRE(p->hidden != nullptr && p->weight != nullptr && p->token_ids != nullptr && p->row_stats != nullptr, GRX_E_INVALID,
                 "%s: null buffer", who);
@@ -454,54 +554,83 @@ static int ll_allow_lds(K kernel, int bytes, std::atomic<uint64_t>& done) {
     return GRX_OK;
 }
 
-#define LL_LAUNCH(kernel, BN, grid, args)                                                                       \
-    do {                                                                                                        \
-        static std::atomic<uint64_t> done_{0};                                                                  \
-        const int rc_ = ll_allow_lds(kernel, mt_lds_bytes<BN>(), done_);                                        \
-        if (rc_ != GRX_OK) return rc_;                                                                          \
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(grid)), dim3(MT_THREADS), mt_lds_bytes<BN>(), stream, args); \
-        GRX_CHECK_HIP(hipGetLastError());                                                                       \
+template <int BN, typename K, typename A>
+static int ll_launch(K kernel, int64_t grid, const A& args, hipStream_t stream, std::atomic<uint64_t>& done) {
+    const int rc = ll_allow_lds(kernel, mt_lds_bytes<BN>(), done);
+    if (rc != GRX_OK) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(MT_THREADS), mt_lds_bytes<BN>(), stream, args);
+    GRX_CHECK_HIP(hipGetLastError());
+    return GRX_OK;
+}
+
+// Workgroups of a kernel that walks its tiles: as many as are resident (two per CU where the LDS holds two).
+static int64_t ll_resident(int bn, int64_t tiles) {
+    const int64_t most = bn == 64 ? 2 * LL_CUS : LL_CUS;
+    return tiles < most ? tiles : most;
+}
+
+#define LL_ONE(BN, kernel, grid, args)                                     \
+    do {                                                                   \
+        static std::atomic<uint64_t> done_{0};                             \
+        const int rc_ = ll_launch<BN>(kernel, grid, args, stream, done_);  \
+        if (rc_ != GRX_OK) return rc_;                                     \
+    } while (0)
+#define LL_EACH(bn, kernel, grid, args)                     \
+    do {                                                    \
+        if ((bn) == 64) LL_ONE(64, (kernel<64>), grid, args);        \
+        else if ((bn) == 128) LL_ONE(128, (kernel<128>), grid, args); \
+        else LL_ONE(256, (kernel<256>), grid, args);        \
+    } while (0)
+#define LL_EACH_ENT(bn, ent, kernel, grid, args)                                  \
+    do {                                                                          \
+        if ((bn) == 64) {                                                         \
+            if (ent) LL_ONE(64, (kernel<64, true>), grid, args);                  \
+            else LL_ONE(64, (kernel<64, false>), grid, args);                     \
+        } else if ((bn) == 128) {                                                 \
+            if (ent) LL_ONE(128, (kernel<128, true>), grid, args);                \
+            else LL_ONE(128, (kernel<128, false>), grid, args);                   \
+        } else {                                                                  \
+            if (ent) LL_ONE(256, (kernel<256, true>), grid, args);                \
+            else LL_ONE(256, (kernel<256, false>), grid, args);                   \
+        }                                                                         \
     } while (0)
 
-#define LL_LAUNCH_BN(kernel, bn, grid, args)                        \
-    do {                                                            \
-        if ((bn) == 64) LL_LAUNCH((kernel<64>), 64, grid, args);    \
-        else if ((bn) == 128) LL_LAUNCH((kernel<128>), 128, grid, args); \
-        else LL_LAUNCH((kernel<256>), 256, grid, args);             \
-    } while (0)
+static LlOperands ll_operands(const grx_lm_token_logps_args* p) {
+    return {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, reinterpret_cast<const uint16_t*>(p->hidden),
+            p->hidden_stride, p->N, p->H, p->V};
+}
 
 extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratch, size_t scratch_bytes, void* stream_) {
     const char* who = "grx_lm_token_logps";
-    int rc = ll_check(who, p);
+    const int rc = ll_check(who, p);
     if (rc != GRX_OK || p->N == 0) return rc;
     GRX_REQUIRE(p->logps != nullptr, GRX_E_INVALID, "%s: null logps", who);
-    const LlForward f = ll_forward(p->N, p->V, p->entropy != nullptr);
+    const bool ent = p->entropy != nullptr;
+    const LlForward f = ll_forward(p->N, p->V, ent);
     GRX_REQUIRE(scratch != nullptr && scratch_bytes >= f.total, GRX_E_WORKSPACE, "%s: scratch of %zu bytes, need %zu", who,
                 scratch_bytes, f.total);
     GRX_REQUIRE(((uintptr_t)scratch & 15u) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
-    GRX_REQUIRE((int64_t)f.m_tiles * f.n_tiles < (1 << 23), GRX_E_UNSUPPORTED, "%s: too many tiles", who);
+    GRX_REQUIRE((int64_t)f.m_tiles * f.n_tiles < (1ll << 31) - LL_CUS * 2, GRX_E_UNSUPPORTED, "%s: too many tiles", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
     LlJoin j;
     LlArgs& a = j.g;
-    a.w = {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, p->V, 0};
-    a.h = {reinterpret_cast<const uint16_t*>(p->hidden), p->hidden_stride, p->N, 0};
-    a.N = p->N;
-    a.H = p->H;
-    a.V = p->V;
+    a.o = ll_operands(p);
     a.m_tiles = f.m_tiles;
     a.n_tiles = f.n_tiles;
     a.k = (float)(1.4426950408889634 / (double)p->temperature);
     a.ids = p->token_ids;
     a.partials = reinterpret_cast<float2*>(s + f.partials);
-    a.weighted = p->entropy ? reinterpret_cast<float*>(s + f.weighted) : nullptr;
+    a.weighted = ent ? reinterpret_cast<float*>(s + f.weighted) : nullptr;
     a.n_pad = f.n_pad;
     a.chosen = reinterpret_cast<float*>(s + f.chosen);
-    LL_LAUNCH_BN(lm_logps_kernel, f.bn, f.m_tiles * f.n_tiles, a);
+    LL_EACH_ENT(f.bn, ent, lm_logps_kernel, ll_resident(f.bn, (int64_t)f.m_tiles * f.n_tiles), a);
+    j.parts = f.parts;
     j.logps = p->logps;
     j.stats = reinterpret_cast<float2*>(p->row_stats);
     j.entropy = p->entropy;
-    hipLaunchKernelGGL(lm_logps_join_kernel, dim3((unsigned)((p->N + 15) / 16)), dim3(256), 0, stream, j);
+    if (p->N <= 1024) hipLaunchKernelGGL(lm_logps_join_kernel<1>, dim3((unsigned)p->N), dim3(256), 0, stream, j);
+    else hipLaunchKernelGGL(lm_logps_join_kernel<16>, dim3((unsigned)((p->N + 15) / 16)), dim3(256), 0, stream, j);
     GRX_CHECK_HIP(hipGetLastError());
     return GRX_OK;
 }
@@ -509,71 +638,50 @@ extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratc
 extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, void* scratch, size_t scratch_bytes,
                                            void* stream_) {
     const char* who = "grx_lm_token_logps_backward";
-    int rc = ll_check(who, p);
+    const int rc = ll_check(who, p);
     if (rc != GRX_OK) return rc;
     GRX_REQUIRE(p->grad_entropy == nullptr || p->entropy != nullptr, GRX_E_INVALID,
                 "%s: a gradient of the entropies needs the entropies", who);
     GRX_REQUIRE((((uintptr_t)p->grad_hidden | (uintptr_t)p->grad_weight) & 15u) == 0, GRX_E_INVALID, "%s: misaligned gradient", who);
-    const bool want_h = p->grad_hidden != nullptr, want_w = p->grad_weight != nullptr;
+    const bool want_h = p->grad_hidden != nullptr, want_w = p->grad_weight != nullptr, ent = p->grad_entropy != nullptr;
     if (p->N == 0 || (!want_h && !want_w)) return GRX_OK;
     const LlBackward b = ll_backward(p->N, p->H, p->V, want_h, want_w);
     GRX_REQUIRE(scratch != nullptr && scratch_bytes >= b.total, GRX_E_WORKSPACE, "%s: scratch of %zu bytes, need %zu", who,
                 scratch_bytes, b.total);
     GRX_REQUIRE(((uintptr_t)scratch & 15u) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
-    GRX_REQUIRE(b.chunk / MT_BM * b.n_tiles < (1 << 23) && (int64_t)b.splits * b.h_tiles * b.n_tiles < (1 << 23) &&
-                    b.n_pad <= GRX_MAX_TOKEN_ROWS,
-                GRX_E_UNSUPPORTED, "%s: too many tiles", who);
+    GRX_REQUIRE((int64_t)b.splits * b.h_tiles * b.n_tiles < (1 << 23), GRX_E_UNSUPPORTED, "%s: too many tiles", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
     LlRow* rows = reinterpret_cast<LlRow*>(s + b.rows);
-    uint16_t* copy = want_w ? reinterpret_cast<uint16_t*>(s + b.copy) : nullptr;
-    uint16_t* g = reinterpret_cast<uint16_t*>(s + b.g);
+    char* copy = want_w ? s + b.copy : nullptr;
+    char* g = s + b.g;
     float* slabs = reinterpret_cast<float*>(s + b.slabs);
-    const uint16_t* weight = reinterpret_cast<const uint16_t*>(p->weight);
-    const uint16_t* hidden = reinterpret_cast<const uint16_t*>(p->hidden);
+    const LlOperands o = ll_operands(p);
 
-    LlPrep pr = {p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
-                 (float)(1.0 / (double)p->temperature), p->N, p->V, p->H, rows, hidden, p->hidden_stride, copy};
-    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)b.n_pad), dim3(256), 0, stream, pr);
+    LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
+                 (float)(1.0 / (double)p->temperature), rows, copy};
+    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_pad / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
+                       stream, pr);
     GRX_CHECK_HIP(hipGetLastError());
     for (int c = 0; c < b.n_chunks; ++c) {
-        const int v0 = (int)(c * b.chunk);
+        const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
-        LlGrad d = {{weight, p->weight_stride, p->V, 0}, {hidden, p->hidden_stride, p->N, 0}, p->N, p->H, p->V,
-                    (int)(cols / MT_BM), b.n_tiles, v0, (float)(1.4426950408889634 / (double)p->temperature), rows, g, b.chunk,
-                    (int)b.n_pad};
-        LL_LAUNCH_BN(lm_logps_dlogits_kernel, b.bn, d.m_tiles * d.n_tiles, d);
+        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (float)(1.4426950408889634 / (double)p->temperature), rows, g};
+        LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * d.n_tiles), d);
         if (want_h) {
-            LlDh x;
-            x.w = {weight + (int64_t)v0 * p->weight_stride, p->weight_stride, p->H, p->V - v0};
-            x.g = {g, b.chunk, (int)b.n_pad, 0};
-            x.N = p->N;
-            x.H = p->H;
-            x.m_tiles = b.h_tiles;
-            x.n_tiles = b.n_tiles;
-            x.splits = b.splits;
-            x.steps = (int)(cols / MT_BK);
-            x.steps_per = (x.steps + b.splits - 1) / b.splits;
-            x.add = c > 0;
-            x.slabs = slabs;
-            LL_LAUNCH_BN(lm_logps_dhidden_kernel, b.bn, b.splits * b.h_tiles * b.n_tiles, x);
+            const int steps = (int)(cols / MT_BK);
+            LlDh x = {o, g, b.h_tiles, b.n_tiles, b.splits, steps, (steps + b.splits - 1) / b.splits, v0, v64, c > 0, slabs};
+            LL_EACH(b.bn, lm_logps_dhidden_kernel, b.splits * b.h_tiles * b.n_tiles, x);
         }
         if (want_w) {
-            LlDw x;
-            x.h = {copy, p->H, p->H, (int)b.n_pad};
-            x.g = {g, b.chunk, (int)cols, (int)b.n_pad};
-            x.H = p->H;
-            x.V = p->V;
-            x.m_tiles = b.h_tiles;
-            x.n_tiles = (int)(cols / 256);
-            x.steps = (int)(b.n_pad / MT_BK);
-            x.v_begin = v0;
-            x.out = reinterpret_cast<uint16_t*>(p->grad_weight);
-            LL_LAUNCH(lm_logps_dweight_kernel, 256, x.m_tiles * x.n_tiles, x);
+            LlDw x = {copy, g, p->H, p->V, b.bn, b.h_tiles, (int)(cols / 256), (int)((p->N + MT_BK - 1) / MT_BK), v0, v64,
+                      reinterpret_cast<uint16_t*>(p->grad_weight)};
+            LL_ONE(256, lm_logps_dweight_kernel, ll_resident(256, (int64_t)x.m_tiles * x.n_tiles), x);
         }
     }
     if (want_h) {
         const int64_t n = (int64_t)p->N * p->H;
+        GRX_REQUIRE(n / 1024 < (1 << 24), GRX_E_UNSUPPORTED, "%s: too many elements", who);
         hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, slabs, b.splits,
                            n, p->H, rows, reinterpret_cast<uint16_t*>(p->grad_hidden));
         GRX_CHECK_HIP(hipGetLastError());

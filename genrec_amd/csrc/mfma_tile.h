@@ -1,13 +1,20 @@
 // A 256 x BN tile of C[n][m] = sum_k A(m, k) B(n, k) on the matrix cores (v_mfma_f32_32x32x16_bf16, fp32
-// accumulators), by one workgroup of eight waves.  Either operand lies in memory with k running along its rows
-// (rows of m or n) or across them (rows of k); both come through LDS by the copy path that bypasses the registers,
-// two tiles of 64 k in turn, so that the next one travels while the present one is multiplied.
+// accumulators), by one workgroup of eight waves.  Both operands come through LDS by the copy path that bypasses the
+// registers, 64 k at a time.  An operand lies in memory in one of four ways, each with a stage (what is copied where)
+// and a reader (how a wave gets its fragments back):
+//   MtAlong          rows of m (n), k along them
+//   MtAcross         rows of k, m along them
+//   MtBlocksAlong    blocks of 32 m (n) x 16 k in fragment order
+//   MtBlocksAcross   such blocks made for the other axis: 32 k x 16 n
+// A fragment block is the 1 KB that one wave holds of a 32 x 16 operand: lane l has row l & 31, k = 8 (l >> 5) + 0 .. 7.
 //
 // C/D layout of the instruction: element e of lane l is m = (e & 3) + 8 (e >> 2) + 4 (l >> 5), n = l & 31: a lane
 // holds one row n and runs of four m.
 #pragma once
 
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "common.h"
 
@@ -17,189 +24,371 @@
 
 typedef short mt_s16x4 __attribute__((ext_vector_type(4)));
 typedef short mt_s16x8 __attribute__((ext_vector_type(8)));
+typedef float mt_f32x4 __attribute__((ext_vector_type(4)));
 typedef float mt_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 mt_b16x4 __attribute__((ext_vector_type(4)));
-typedef float mt_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mt_u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void mt_lds_void;
 typedef __attribute__((address_space(3))) mt_s16x4 mt_lds_s16x4;
+typedef __attribute__((address_space(3))) const mt_s16x8 mt_lds_s16x8;
 typedef __attribute__((address_space(1))) const void mt_global_void;
 
-// One operand: `rows` rows of `ld` elements.  k along: a row per m (n), starting at column k0; rows past the end
-// read the last one, and k0 + 64 nk elements of each are there.  k across: a row per k, starting at row k0, columns
-// past the end (a multiple of 8) read the last eight, rows past the end the last row: the other operand is 0 there.
-// What else is read twice is multiplied into elements of C that nobody keeps.
-struct MtOperand {
-    const uint16_t* p;
-    int64_t ld;
-    int extent;  // valid m (n)
-    int k_rows;  // k across: rows of k
-};
+// Waves as WM x WN, MA x NB blocks of 32 x 32 a wave; AR, BR: buffers of A and of B in LDS.
+template <int BN>
+struct MtShape;
+template <> struct MtShape<256> { static constexpr int WM = 2, WN = 4, MA = 4, NB = 2, AR = 3, BR = 2; };
+template <> struct MtShape<128> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 2, AR = 3, BR = 3; };
+template <> struct MtShape<64> { static constexpr int WM = 8, WN = 1, MA = 1, NB = 2, AR = 2, BR = 2; };
 
 template <int BN>
-struct MtShape;  // waves as WM x WN, MA x NB blocks of 32 x 32 a wave
-template <> struct MtShape<256> { static constexpr int WM = 2, WN = 4, MA = 4, NB = 2; };
-template <> struct MtShape<128> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 2; };
-template <> struct MtShape<64> { static constexpr int WM = 8, WN = 1, MA = 1, NB = 2; };
+constexpr int mt_lds_bytes() { return (MtShape<BN>::AR * MT_BM + MtShape<BN>::BR * BN) * MT_BK * 2; }
 
-template <int BN>
-constexpr int mt_lds_bytes() { return 2 * (MT_BM + BN) * MT_BK * 2; }
+__device__ __forceinline__ int mt_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+__device__ __forceinline__ void mt_copy(const char* from, uint32_t to) {  // 16 bytes a lane; `to` uniform
+    __builtin_amdgcn_global_load_lds((mt_global_void*)from, (mt_lds_void*)(uintptr_t)to, 16, 0, 0);
+}
 
-// LDS images, in chunks of 16 bytes, permuted so that no read meets a bank twice:
-//  k along:  row r holds 64 k (8 chunks), chunk c at c ^ ((r >> 1) & 7): the 16 lanes that read the same chunk of
-//            consecutive rows find 16 different chunks of a 256-byte bank row (two rows).
-//  k across: row k holds W elements, chunk c at c ^ (4 (k & 3)): 32 lanes of a transposing read take four chunks of
-//            each of four rows.
-// The copy writes lane l of an instruction at base + 16 l, so the permutation is applied to the source address.
-__device__ __forceinline__ int mt_swz_along(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
-__device__ __forceinline__ int mt_swz_across(int k, int chunk) { return chunk ^ ((k & 3) << 2); }
+// ---- stages.  N: copies per wave and step (1 KB each, eight waves); issue(i, to): the i-th of them into the buffer at
+// `to`; advance(): on to the next step.  The addresses are a uniform base plus lane offsets that stay.  A copy writes
+// lane l at 16 l, so the order inside a buffer is chosen by what each lane fetches: all orders below are such that no
+// fragment read meets an LDS bank twice.
 
-// W: rows (k along) or columns (k across) of the operand's tile
-template <int W, bool ACROSS>
-struct MtStage {
-    static constexpr int N = W * MT_BK * 2 / 1024 / 8;  // instructions per wave: 1 KB each, eight waves
-    const uint16_t* src[N];
-    int64_t ld;
-    int k[N], k_last;
-    __device__ __forceinline__ MtStage(const MtOperand& o, int at, int k0) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Row r of a buffer: 64 k in 8 chunks of 16 bytes, chunk c at c ^ ((r >> 1) & 7).  Rows past the end read the last one:
+// they make rows of C that nobody keeps.  Rows are less than 2^22 elements apart.
+template <int W>
+struct MtAlong {
+    static constexpr int N = W * MT_BK * 2 / 8192;
+    const char* base;
+    uint32_t off[N];
+    __device__ __forceinline__ MtAlong() {}
+    __device__ __forceinline__ MtAlong(const uint16_t* p, int64_t ld, int rows, int at, int k0) {
+        const int lane = threadIdx.x & 63, wave = mt_wave();
+        base = reinterpret_cast<const char*>(p + (int64_t)at * ld + k0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (ACROSS) {
-                constexpr int PER = 64 / (W / 8);  // rows of k per instruction
-                const int row = (wave * N + i) * PER + lane / (W / 8);
-                int col = at + mt_swz_across(row, lane % (W / 8)) * 8;
-                col = col < o.extent ? col : o.extent - 8;
-                src[i] = o.p + col;
-                k[i] = k0 + row;
-            } else {
-                const int r = (wave * N + i) * 8 + (lane >> 3);
-                int row = at + r;
-                row = row < o.extent ? row : o.extent - 1;
-                src[i] = o.p + (int64_t)row * o.ld + k0 + mt_swz_along(r, lane & 7) * 8;
-            }
+            int row = (wave * N + i) * 8 + (lane >> 3);
+            const int chunk = (lane & 7) ^ ((row >> 1) & 7);
+            row = at + row < rows ? row : rows - 1 - at;
+            off[i] = (uint32_t)row * (uint32_t)ld * 2u + chunk * 16;
         }
-        ld = o.ld;
-        k_last = o.k_rows - 1;
     }
-    __device__ __forceinline__ void issue(unsigned char* dst) {
-        const int wave = threadIdx.x >> 6;
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
+    __device__ __forceinline__ void advance() { base += MT_BK * 2; }
+    __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
+};
+
+// Row k of a buffer: 256 m in 32 chunks, chunk c at c ^ (4 (k & 3)).  Columns past the end (a multiple of 8) read the
+// last eight; rows past the end read the last one, where the other operand is 0.
+struct MtAcross {
+    static constexpr int N = 4;
+    const char* base;
+    uint32_t off[N];
+    int64_t ld;
+    int left;  // rows of k from the step's first on
+    __device__ __forceinline__ MtAcross() {}
+    __device__ __forceinline__ MtAcross(const uint16_t* p, int64_t ld_, int cols, int k_rows, int at, int k0) {
+        const int lane = threadIdx.x & 63, wave = mt_wave();
+        ld = ld_;
+        left = k_rows - k0;
+        base = reinterpret_cast<const char*>(p + (int64_t)k0 * ld + at);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const uint16_t* from = src[i];
-            if (ACROSS) {
-                from += (int64_t)(k[i] < k_last ? k[i] : k_last) * ld;
-                k[i] += MT_BK;
-            } else {
-                src[i] += MT_BK;
-            }
-            __builtin_amdgcn_global_load_lds((mt_global_void*)from, (mt_lds_void*)(dst + (wave * N + i) * 1024), 16, 0, 0);
+            const int row = (wave * N + i) * 2 + (lane >> 5);
+            int col = ((lane & 31) ^ ((row & 3) << 2)) * 8;
+            col = at + col < cols ? col : cols - 8 - at;
+            off[i] = (uint32_t)row * (uint32_t)ld * 2u + (uint32_t)(col * 2);
         }
+    }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue_any(int i, uint32_t to) const {
+        const int row = (mt_wave() * N + i) * 2 + ((threadIdx.x & 63) >> 5);
+        const int64_t back = row < left ? 0 : (int64_t)(row - left + 1) * ld * 2;
+        mt_copy(base + off[i] - back, to + (mt_wave() * N + i) * 1024);
+    }
+    __device__ __forceinline__ void advance() {
+        base += ld * (MT_BK * 2);
+        left -= MT_BK;
+    }
+    __device__ __forceinline__ int whole_steps(int nk) const { return nk < left / MT_BK ? nk : left / MT_BK; }
+};
+
+// W / 32 x 4 blocks a step, in memory one behind the other (groups past `groups` read the last one).
+template <int W>
+struct MtBlocksAlong {
+    static constexpr int N = W * MT_BK * 2 / 8192;
+    const char* base;
+    uint32_t off[N];
+    int64_t step;
+    __device__ __forceinline__ MtBlocksAlong() {}
+    // p: the step's first block; groups: groups of 32 rows that are there from it on
+    __device__ __forceinline__ MtBlocksAlong(const char* p, int64_t step_bytes, int groups) {
+        base = p;
+        step = step_bytes;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int block = mt_wave() * N + i;
+            const int group = block / 4 < groups ? block / 4 : groups - 1;
+            off[i] = (group * 4 + block % 4) * 1024 + (threadIdx.x & 63) * 16;
+        }
+    }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
+    __device__ __forceinline__ void advance() { base += step; }
+    __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
+};
+
+// G as d weight reads it: blocks of 32 n x 16 v, in memory [tile of BN n][64 v][BN / 32][4], a step being 64 n of 256 v.
+// In a buffer, [64 v][32 n][16 v] blocks whose unit of 16 bytes (n, 8 v h) stands at (2 n + h) ^ (8 in odd blocks): the
+// 32 lanes of a transposing read take 16 different units of a bank row.
+struct MtBlocksAcross {
+    static constexpr int N = 4;
+    const char* base;
+    uint32_t off[N];
+    int64_t tile_bytes;  // from one tile of BN n to the next
+    int per, at;         // steps in such a tile, the present one
+    __device__ __forceinline__ MtBlocksAcross() {}
+    __device__ __forceinline__ MtBlocksAcross(const char* p, int64_t tile_bytes_, int bn) {
+        base = p;
+        tile_bytes = tile_bytes_;
+        per = bn / 64;
+        at = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int block = mt_wave() * N + i, inner = block & 7;  // inner: 2 of 32 n, 4 of 16 v
+            const int unit = (threadIdx.x & 63) ^ ((inner & 1) << 3);
+            off[i] = (block >> 3) * (bn * 128) + inner * 1024 + ((unit & 1) * 32 + (unit >> 1)) * 16;
+        }
+    }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
+    __device__ __forceinline__ void advance() {
+        const bool turn = ++at == per;
+        base += turn ? tile_bytes - (per - 1) * 8192 : 8192;
+        at = turn ? 0 : at;
+    }
+    __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
+};
+
+// ---- readers: read(tile, sub, j) is fragment j (rows first + 32 j ...) of the 16 k at `sub` --------------------
+struct MtReadAlong {
+    uint32_t lane_off;
+    __device__ __forceinline__ MtReadAlong(int first) {
+        const int lane = threadIdx.x & 63, row = first + (lane & 31);
+        lane_off = row * 128 + ((lane >> 5) ^ ((row >> 1) & 7)) * 16;
+    }
+    static constexpr int READS = 1;
+    __device__ __forceinline__ mt_s16x8 read(uint32_t tile, int sub, int j) const {
+        return *(mt_lds_s16x8*)(uintptr_t)(((tile + lane_off) ^ (sub * 32)) + j * 4096);
     }
 };
 
-// The fragment of the 32 x 16 block at row `at` (inside the tile) and sub-step `sub`: lane l gets row l & 31,
-// k = 8 (l >> 5) + 0 .. 7.
-template <int W, bool ACROSS>
-__device__ __forceinline__ mt_s16x8 mt_fragment(const unsigned char* tile, int at, int sub) {
-    const int lane = threadIdx.x & 63;
-    if constexpr (!ACROSS) {
-        const int row = at + (lane & 31);
-        return *reinterpret_cast<const mt_s16x8*>(tile + row * 128 + mt_swz_along(row, 2 * sub + (lane >> 5)) * 16);
-    } else {
-        // the transposing read works on 16 lanes: lane i fetches four m of row k + i / 4 and receives element m = i of
-        // the four rows
-        const int i = lane & 15, group = lane >> 4;
-        const int k = sub * 16 + (group >> 1) * 8 + (i >> 2);
-        const int m = at + (group & 1) * 16 + (i & 3) * 4;
-        const unsigned char* p = tile + k * (W * 2) + mt_swz_across(k, m >> 3) * 16 + (m & 7) * 2;
-        const mt_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)p);
-        const mt_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)(p + 4 * (W * 2)));  // k + 4: same permutation
+// The transposing read works on 16 lanes: lane i fetches four m of row k + i / 4 and receives m = i of the four rows.
+struct MtReadAcross {
+    uint32_t lane_off;
+    __device__ __forceinline__ MtReadAcross(int first) {
+        const int i = threadIdx.x & 15, group = (threadIdx.x & 63) >> 4;
+        const int k = (group >> 1) * 8 + (i >> 2), m = first + (group & 1) * 16 + (i & 3) * 4;
+        lane_off = k * 512 + ((m >> 3) ^ ((k & 3) << 2)) * 16 + (m & 7) * 2;
+    }
+    static constexpr int READS = 2;
+    __device__ __forceinline__ mt_s16x8 read(uint32_t tile, int sub, int j) const {
+        const uint32_t q = ((tile + lane_off) ^ (j * 64)) + sub * 8192;
+        const mt_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)(uintptr_t)q);
+        const mt_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)(uintptr_t)(q + 2048));  // k + 4
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+};
+
+struct MtReadBlocksAlong {
+    uint32_t lane_off;
+    __device__ __forceinline__ MtReadBlocksAlong(int first) { lane_off = (first >> 5) * 4096 + (threadIdx.x & 63) * 16; }
+    static constexpr int READS = 1;
+    __device__ __forceinline__ mt_s16x8 read(uint32_t tile, int sub, int j) const {
+        return *(mt_lds_s16x8*)(uintptr_t)(tile + lane_off + j * 4096 + sub * 1024);
+    }
+};
+
+struct MtReadBlocksAcross {
+    uint32_t lane_off;
+    __device__ __forceinline__ MtReadBlocksAcross(int first) {  // a multiple of 64
+        const int i = threadIdx.x & 15, group = (threadIdx.x & 63) >> 4;
+        const int unit = ((i >> 2) * 2 + ((i & 3) >> 1)) ^ ((group & 1) << 3);
+        lane_off = (first >> 6) * 8192 + (group & 1) * 1024 + ((group >> 1) * 16 + unit) * 16 + (i & 1) * 8;
+    }
+    static constexpr int READS = 2;
+    __device__ __forceinline__ mt_s16x8 read(uint32_t tile, int sub, int j) const {
+        const uint32_t q = tile + lane_off, at = (sub >> 1) * 4096 + (sub & 1) * 512 + j * 2048;
+        const mt_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)(uintptr_t)(q + at));
+        const mt_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((mt_lds_s16x4*)(uintptr_t)((q ^ 128) + at));  // n + 4
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// ---- the pipeline ------------------------------------------------------------------------------------------
+// Waits until at most VM of this wave's copies are under way and its LDS reads are done, then meets the other waves.
+template <int VM>
+__device__ __forceinline__ void mt_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(VM) : "memory");
 }
 
-// acc += over nk steps of 64 k.  Ends with a barrier: the LDS is free again.
-template <int BN, bool A_ACROSS, bool B_ACROSS>
-__device__ __forceinline__ void mt_multiply(mt_f32x16 (&acc)[MtShape<BN>::MA][MtShape<BN>::NB], unsigned char* lds,
-                                            const MtOperand& a, int m0, const MtOperand& b, int n0, int k0, int nk) {
+// begin() starts the first copies of a tile (the LDS must be free), run() multiplies and leaves the LDS free: the next
+// tile's begin() may come before this one's results are used, so that its copies travel meanwhile.
+//
+// One meeting of the waves per step, in front of its last quarter: by then every wave holds that quarter's fragments
+// in registers, so the step's buffers are free for the copies of a later step, and the next step's copies, under way
+// for AR - 1 (BR - 1) steps, have landed -- its first fragments are read between the products of the last quarter.
+// Every LDS read goes out a quarter before its product, early in it, and the copies of a step are spread over two
+// quarters, one behind a product: nothing in the loop waits for what was issued right before.
+template <int BN, class StageA, class ReadA, class StageB, class ReadB>
+struct MtPipe {
     typedef MtShape<BN> S;
-    constexpr int A_BYTES = MT_BM * MT_BK * 2, BUF = A_BYTES + BN * MT_BK * 2;
-    const int wave = threadIdx.x >> 6;
-    const int wm = wave / S::WN, wn = wave % S::WN;
-    MtStage<MT_BM, A_ACROSS> sa(a, m0, k0);
-    MtStage<BN, B_ACROSS> sb(b, n0, k0);
+    typedef mt_f32x16 Acc[S::MA][S::NB];
+    static constexpr int A_BYTES = MT_BM * MT_BK * 2, B_BYTES = BN * MT_BK * 2;
+    static constexpr int DEEP = S::AR > S::BR ? S::AR : S::BR;
+    static_assert(S::AR >= S::BR, "the copies of A go out last");
+    StageA sa;
+    StageB sb;
+    int nk;
+    uint32_t la, lb;
+
+    __device__ __forceinline__ explicit MtPipe(unsigned char* lds) {
+        la = (uint32_t)(uintptr_t)(mt_lds_void*)lds;
+        lb = la + S::AR * A_BYTES;
+    }
+    __device__ __forceinline__ void begin(const StageA& a, const StageB& b, int steps) {
+        sa = a;
+        sb = b;
+        nk = steps;
 #pragma unroll
-    for (int m = 0; m < S::MA; ++m)
+        for (int t = 0; t < DEEP; ++t) {
+            if (t < S::BR && t < nk) {
 #pragma unroll
-        for (int n = 0; n < S::NB; ++n)
+                for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, lb + t * B_BYTES);
+                sb.advance();
+            }
+            if (t < S::AR && t < nk) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.f;
-    if (nk <= 0) return;
-    sa.issue(lds);
-    sb.issue(lds + A_BYTES);
-    __syncthreads();  // waits for the copies as well
-    for (int kt = 0; kt < nk; ++kt) {
-        unsigned char* cur = lds + (kt & 1) * BUF;
-        if (kt + 1 < nk) {
-            unsigned char* nxt = lds + ((kt + 1) & 1) * BUF;
-            sa.issue(nxt);
-            sb.issue(nxt + A_BYTES);
+                for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, la + t * A_BYTES);
+                sa.advance();
+            }
         }
-        // Four sub-steps of 16 k with two register sets of fragments: the reads of sub-step s + 1 go out between the
-        // products of sub-step s, so the matrix pipe waits for LDS once per step of 64.
-        auto read_set = [&](int sub, mt_s16x8* fa, mt_s16x8* fb) {
+    }
+    __device__ __forceinline__ void run(Acc& acc) {
 #pragma unroll
-            for (int m = 0; m < S::MA; ++m) fa[m] = mt_fragment<MT_BM, A_ACROSS>(cur, wm * S::MA * 32 + m * 32, sub);
+        for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-            for (int n = 0; n < S::NB; ++n) fb[n] = mt_fragment<BN, B_ACROSS>(cur + A_BYTES, wn * S::NB * 32 + n * 32, sub);
+            for (int n = 0; n < S::NB; ++n)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.f;
+        if (nk <= 0) return;
+        const int wave = mt_wave();
+        const ReadA ra(wave / S::WN * S::MA * 32);
+        const ReadB rb(wave % S::WN * S::NB * 32);
+        constexpr int AHEAD = (S::AR - 2) * StageA::N + (S::BR - 2) * StageB::N;  // copies that may stay under way
+        mt_meet<0>();
+        uint32_t ca = la, cb = lb;  // the present step's buffers
+        mt_s16x8 fa[2][S::MA], fb[2][S::NB];
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j) fb[0][j] = rb.read(cb, 0, j);
+#pragma unroll
+        for (int j = 0; j < S::MA; ++j) fa[0][j] = ra.read(ca, 0, j);
+
+        // the products of fragment set `set`, with the reads of (ra_at, rb_at, sub) into the other set and `n` copies
+        // (copy(i)) between them
+        auto quarter = [&](auto set_, uint32_t ra_at, uint32_t rb_at, int sub, auto n_, auto&& copy) {
+            constexpr int set = decltype(set_)::value, COPIES = decltype(n_)::value;
+            constexpr int FRAGS = S::MA + S::NB, PRODUCTS = S::MA * S::NB;
+            constexpr int PER = (2 * FRAGS + PRODUCTS - 1) / PRODUCTS;  // all reads in the first half of the products
+#pragma unroll
+            for (int p = 0; p < PRODUCTS; ++p) {
+                __builtin_amdgcn_sched_barrier(0);
+                const int m = p / S::NB, n = p % S::NB;
+                acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[set][m], fb[set][n], acc[m][n], 0, 0, 0);
+#pragma unroll
+                for (int f = p * PER; f < (p + 1) * PER; ++f) {
+                    if (f < S::NB) fb[set ^ 1][f] = rb.read(rb_at, sub, f);
+                    else if (f < FRAGS) fa[set ^ 1][f - S::NB] = ra.read(ra_at, sub, f - S::NB);
+                }
+#pragma unroll
+                for (int i = p * COPIES / PRODUCTS; i < (p + 1) * COPIES / PRODUCTS; ++i) copy(i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         };
-        auto multiply = [&](const mt_s16x8* fa, const mt_s16x8* fb) {
+        typedef std::integral_constant<int, 0> Zero;
+        typedef std::integral_constant<int, 1> One;
+        auto none = [](int) {};
+        int ia = 0, ib = 0, kt = 0;
+        uint32_t free_a = 0;
+        auto step = [&](auto whole_, bool a_due) {  // a_due: A's copies that follow the meeting of the step before
+            constexpr bool whole = decltype(whole_)::value;
+            if constexpr (whole) {
+                quarter(Zero(), ca, cb, 1, std::integral_constant<int, StageA::N>(), [&](int i) { sa.issue(i, free_a); });
+                sa.advance();
+            } else {
+                quarter(Zero(), ca, cb, 1, Zero(), none);
+                if (a_due) {
 #pragma unroll
-            for (int m = 0; m < S::MA; ++m)
+                    for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, free_a);
+                    sa.advance();
+                }
+            }
+            quarter(One(), ca, cb, 2, Zero(), none);
+            quarter(Zero(), ca, cb, 3, Zero(), none);
+            if (whole) mt_meet<AHEAD>();
+            else mt_meet<0>();
+            const uint32_t free_b = cb;
+            free_a = ca;
+            ia = ia + 1 == S::AR ? 0 : ia + 1;
+            ib = ib + 1 == S::BR ? 0 : ib + 1;
+            ca = la + ia * A_BYTES;
+            cb = lb + ib * B_BYTES;
+            if constexpr (whole) {
+                quarter(One(), ca, cb, 0, std::integral_constant<int, StageB::N>(), [&](int i) { sb.issue(i, free_b); });
+                sb.advance();
+            } else {
+                if (kt + S::BR < nk) {
 #pragma unroll
-                for (int n = 0; n < S::NB; ++n)
-                    acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[m], fb[n], acc[m][n], 0, 0, 0);
-        };
-        mt_s16x8 fa0[S::MA], fb0[S::NB], fa1[S::MA], fb1[S::NB];
-        constexpr int READS = S::MA * (A_ACROSS ? 2 : 1) + S::NB * (B_ACROSS ? 2 : 1), PRODUCTS = S::MA * S::NB;
-        constexpr int PER = (READS + PRODUCTS - 1) / PRODUCTS;
-        auto interleave = [&]() {
-#pragma unroll
-            for (int i = 0; i < PRODUCTS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+                    for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, free_b);
+                    sb.advance();
+                }
+                // behind the last step: whatever the next buffer holds, not used
+                quarter(One(), ca, cb, 0, Zero(), none);
             }
         };
-        read_set(0, fa0, fb0);
-        __builtin_amdgcn_sched_barrier(0);
-        read_set(1, fa1, fb1);
-        multiply(fa0, fb0);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        read_set(2, fa0, fb0);
-        multiply(fa1, fb1);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        read_set(3, fa1, fb1);
-        multiply(fa0, fb0);
-        interleave();
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(fa1, fb1);
-        __syncthreads();  // the next tiles have landed, and everybody is done with these
+        // Copies in a whole step kt: A of step kt - 1 + AR (in its first quarter), B of step kt + BR (in its last).
+        const int ws = sa.whole_steps(nk - S::AR) + S::AR, wb = sb.whole_steps(nk - S::BR) + S::BR;  // as seen from here
+        int safe = ws - S::AR + 1 < wb - S::BR ? ws - S::AR + 1 : wb - S::BR;
+        step(std::false_type(), false);
+        for (kt = 1; kt < safe; ++kt) step(std::true_type(), true);
+        for (; kt < nk; ++kt) step(std::false_type(), kt - 1 + S::AR < nk);
+        mt_meet<0>();
     }
+};
+
+// Workgroups are dealt to the eight XCDs round robin, and about 32 run on each at a time.  All XCDs work on the same
+// few m tiles at a time -- the large operand, which one of them fetches from memory and the others from the cache
+// behind the L2s -- and each keeps to its own n tiles (n tile = XCD modulo 8) where there are that many; else
+// an m tile stays on one XCD with all its n tiles.
+__device__ __forceinline__ void mt_tile(int block, int m_tiles, int n_tiles, int& tm, int& tn) {
+    if (n_tiles >= 8) {
+        tm = block / n_tiles;
+        tn = block - tm * n_tiles;
+        return;
+    }
+    const int group = block / (8 * n_tiles), left = m_tiles - group * 8;
+    const int rest = block - group * 8 * n_tiles, wide = left < 8 ? left : 8;
+    tn = rest / wide;
+    tm = group * 8 + rest - tn * wide;
 }
 
-// Workgroups are dealt to the eight XCDs round robin; every XCD takes one contiguous stretch of the tiles, ordered
-// in groups of eight n tiles that walk the m tiles together: the 32 workgroups an XCD runs at a time share about
-// four m tiles and eight n tiles in its L2.
-__device__ __forceinline__ void mt_tile(int block, int m_tiles, int n_tiles, int& tm, int& tn) {
-    const int total = m_tiles * n_tiles;
-    const int xcd = block & 7, slot = block >> 3;
-    const int per = total >> 3, extra = total & 7;
-    const int id = xcd * per + (xcd < extra ? xcd : extra) + slot;
-    const int group = id / (8 * m_tiles);
-    const int in_group = n_tiles - group * 8 < 8 ? n_tiles - group * 8 : 8;
-    const int rest = id - group * 8 * m_tiles;
-    tm = rest / in_group;
-    tn = group * 8 + rest - tm * in_group;
+// Eight m of a lane's row in memory order: quads 2 q and 2 q + 1 of a 32 x 32 block (elements 8 q ..), rounded to bf16,
+// as the half of the wave that holds m 16 q + 8 (l >> 5) + 0 .. 7.  The halves trade their middle runs of four.
+__device__ __forceinline__ mt_u32x4 mt_pack8(mt_f32x4 x, mt_f32x4 y) {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 a = __builtin_bit_cast(u2, __builtin_convertvector(x, mt_b16x4));
+    const u2 b = __builtin_bit_cast(u2, __builtin_convertvector(y, mt_b16x4));
+    const auto p = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
+    const auto q = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+    return mt_u32x4{p[0], q[0], p[1], q[1]};
 }

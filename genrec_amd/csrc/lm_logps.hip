@@ -17,6 +17,12 @@
 
 #define LL_FLOOR (-200.f)           // 2^-200 is 0 in fp32: keeps 0 * -inf out of the entropy sums
 #define LL_CUS 256
+#ifndef LL_DW_BDEEP
+#define LL_DW_BDEEP true
+#endif
+#ifndef LL_DH_BDEEP
+#define LL_DH_BDEEP false
+#endif
 #ifndef LL_CHUNK_BYTES
 #define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk
 #endif
@@ -31,7 +37,7 @@ struct LlOperands {
 
 struct LlArgs {
     LlOperands o;
-    int m_tiles, n_tiles;
+    int m_begin, m_tiles, n_tiles;  // this launch's share of the m tiles
     float k;                    // log2(e) / temperature
     const int64_t* ids;         // [N]
     float2* partials;           // [parts][n_pad] (max, sum), parts = m_tiles x waves along m
@@ -41,17 +47,17 @@ struct LlArgs {
 };
 
 template <int BN>
-using LlLogits = MtPipe<BN, MtAlong<MT_BM>, MtReadAlong, MtAlong<BN>, MtReadAlong>;
+using LlLogits = MtPipe<BN, MtAlong<MT_BM, BN>, MtReadAlong, MtAlong<BN, BN>, MtReadAlong>;
 
 template <int BN>
 __device__ __forceinline__ void ll_begin(LlLogits<BN>& pipe, const LlOperands& o, int v0, int r0) {
-    pipe.begin(MtAlong<MT_BM>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN>(o.hidden, o.hidden_ld, o.N, r0, 0), o.H / MT_BK);
+    pipe.begin(MtAlong<MT_BM, BN>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN, BN>(o.hidden, o.hidden_ld, o.N, r0, 0), o.H / MT_BK);
 }
 
 // As many workgroups as run at a time; each takes every gridDim-th tile and starts the next one's copies before it
 // turns to its own results.  Those stay inside the wave: a row's sums over the wave's columns are one partial.
 template <int BN, bool ENT>
-__global__ __launch_bounds__(MT_THREADS) void lm_logps_kernel(LlArgs a) {
+__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
@@ -60,9 +66,9 @@ __global__ __launch_bounds__(MT_THREADS) void lm_logps_kernel(LlArgs a) {
     LlLogits<BN> pipe(lds);
     int tm, tn;
     mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    ll_begin(pipe, a.o, tm * MT_BM, tn * BN);
+    ll_begin(pipe, a.o, (a.m_begin + tm) * MT_BM, tn * BN);
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int v0 = tm * MT_BM, r0 = tn * BN, part = tm * S::WM + wm;
+        const int v0 = (a.m_begin + tm) * MT_BM, r0 = tn * BN, part = (a.m_begin + tm) * S::WM + wm;
         int64_t id[S::NB];
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
@@ -73,7 +79,7 @@ __global__ __launch_bounds__(MT_THREADS) void lm_logps_kernel(LlArgs a) {
         pipe.run(acc);
         if (tile + (int)gridDim.x < tiles) {
             mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
-            ll_begin(pipe, a.o, tm * MT_BM, tn * BN);
+            ll_begin(pipe, a.o, (a.m_begin + tm) * MT_BM, tn * BN);
         }
         const int vw = v0 + wm * S::MA * 32 + 4 * half;  // vocabulary entry of m = 0, e = 0
 #pragma unroll
@@ -256,7 +262,7 @@ struct LlGrad {
 };
 
 template <int BN, bool ENT>
-__global__ __launch_bounds__(MT_THREADS) void lm_logps_dlogits_kernel(LlGrad a) {
+__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(LlGrad a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
@@ -337,7 +343,7 @@ struct LlDh {
 };
 
 template <int BN>
-__global__ __launch_bounds__(MT_THREADS) void lm_logps_dhidden_kernel(LlDh a) {
+__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(LlDh a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
     // one XCD takes neighbouring tiles: all h tiles of a few n tiles, which share G
@@ -347,10 +353,10 @@ __global__ __launch_bounds__(MT_THREADS) void lm_logps_dhidden_kernel(LlDh a) {
     const int tn = rest % a.n_tiles, split = rest / a.n_tiles;
     const int h0 = tm * MT_BM, r0 = tn * BN;
     const int s0 = split * a.steps_per, s1 = s0 + a.steps_per < a.steps ? s0 + a.steps_per : a.steps;
-    MtPipe<BN, MtAcross, MtReadAcross, MtBlocksAlong<BN>, MtReadBlocksAlong> pipe(lds);
+    MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong, LL_DH_BDEEP && BN == 256> pipe(lds);
     typename decltype(pipe)::Acc acc;
-    pipe.begin(MtAcross(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
-               MtBlocksAlong<BN>(a.g + ((int64_t)tn * a.v64 + s0) * (BN * 128), BN * 128, BN / 32), s1 - s0);
+    pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
+               MtBlocksAlong<BN, BN>(a.g + ((int64_t)tn * a.v64 + s0) * (BN * 128), BN * 128, BN / 32), s1 - s0);
     pipe.run(acc);
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
@@ -393,7 +399,7 @@ struct LlDw {
     uint16_t* out;             // [V][H]
 };
 
-typedef MtPipe<256, MtBlocksAlong<MT_BM>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross> LlDwPipe;
+typedef MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, LL_DW_BDEEP> LlDwPipe;
 
 // Eight v tiles at a time, one per XCD, all h tiles of each: G is read by one XCD.
 __device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int tile, int& h0, int& c0) {
@@ -401,11 +407,11 @@ __device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int t
     const int rest = tile - group * 8 * a.m_tiles;
     h0 = rest / wide * MT_BM;
     c0 = (group * 8 + rest % wide) * 256;
-    pipe.begin(MtBlocksAlong<MT_BM>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, a.H / 32 - h0 / 32),
+    pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, a.H / 32 - h0 / 32),
                MtBlocksAcross(a.g + (int64_t)(c0 / 64) * (a.bn * 128), (int64_t)a.v64 * (a.bn * 128), a.bn), a.steps);
 }
 
-__global__ __launch_bounds__(MT_THREADS) void lm_logps_dweight_kernel(LlDw a) {
+__global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel(LlDw a) {
     typedef MtShape<256> S;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
@@ -442,7 +448,12 @@ __global__ __launch_bounds__(MT_THREADS) void lm_logps_dweight_kernel(LlDw a) {
 static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 // Rows per tile: as few as hold all rows.
-static int ll_bn(int N) { return N <= 64 ? 64 : N <= 128 ? 128 : 256; }
+static int ll_bn(int N) {
+#ifdef LL_FORCE_BN
+    return LL_FORCE_BN;
+#endif
+    return N <= 64 ? 64 : N <= 128 ? 128 : 256;
+}
 
 struct LlForward {
     int bn, m_tiles, n_tiles, parts;
@@ -558,7 +569,7 @@ template <int BN, typename K, typename A>
 static int ll_launch(K kernel, int64_t grid, const A& args, hipStream_t stream, std::atomic<uint64_t>& done) {
     const int rc = ll_allow_lds(kernel, mt_lds_bytes<BN>(), done);
     if (rc != GRX_OK) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(MT_THREADS), mt_lds_bytes<BN>(), stream, args);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(MtShape<BN>::THREADS), mt_lds_bytes<BN>(), stream, args);
     GRX_CHECK_HIP(hipGetLastError());
     return GRX_OK;
 }
@@ -616,7 +627,6 @@ extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratc
     LlJoin j;
     LlArgs& a = j.g;
     a.o = ll_operands(p);
-    a.m_tiles = f.m_tiles;
     a.n_tiles = f.n_tiles;
     a.k = (float)(1.4426950408889634 / (double)p->temperature);
     a.ids = p->token_ids;
@@ -624,7 +634,9 @@ extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratc
     a.weighted = ent ? reinterpret_cast<float*>(s + f.weighted) : nullptr;
     a.n_pad = f.n_pad;
     a.chosen = reinterpret_cast<float*>(s + f.chosen);
-    LL_EACH_ENT(f.bn, ent, lm_logps_kernel, ll_resident(f.bn, (int64_t)f.m_tiles * f.n_tiles), a);
+    a.m_begin = 0;
+    a.m_tiles = f.m_tiles;
+    LL_EACH_ENT(f.bn, ent, lm_logps_kernel, ll_resident(f.bn, (int64_t)a.m_tiles * f.n_tiles), a);
     j.parts = f.parts;
     j.logps = p->logps;
     j.stats = reinterpret_cast<float2*>(p->row_stats);

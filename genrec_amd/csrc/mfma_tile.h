@@ -1,5 +1,5 @@
 // A 256 x BN tile of C[n][m] = sum_k A(m, k) B(n, k) on the matrix cores (v_mfma_f32_32x32x16_bf16, fp32
-// accumulators), by one workgroup of eight waves.  Both operands come through LDS by the copy path that bypasses the
+// accumulators), by one workgroup.  Both operands come through LDS by the copy path that bypasses the
 // registers, 64 k at a time.  An operand lies in memory in one of four ways, each with a stage (what is copied where)
 // and a reader (how a wave gets its fragments back):
 //   MtAlong          rows of m (n), k along them
@@ -18,7 +18,6 @@
 
 #include "common.h"
 
-#define MT_THREADS 512
 #define MT_BM 256
 #define MT_BK 64
 
@@ -31,33 +30,43 @@ typedef uint32_t mt_u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void mt_lds_void;
 typedef __attribute__((address_space(3))) mt_s16x4 mt_lds_s16x4;
 typedef __attribute__((address_space(3))) const mt_s16x8 mt_lds_s16x8;
-typedef __attribute__((address_space(1))) const void mt_global_void;
 
-// Waves as WM x WN, MA x NB blocks of 32 x 32 a wave; AR, BR: buffers of A and of B in LDS.
+// Waves as WM x WN, MA x NB blocks of 32 x 32 a wave.  DEEP, FLAT: buffers in LDS of the operand that comes from
+// further away, and of the other one.
 template <int BN>
 struct MtShape;
-template <> struct MtShape<256> { static constexpr int WM = 2, WN = 4, MA = 4, NB = 2, AR = 3, BR = 2; };
-template <> struct MtShape<128> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 2, AR = 3, BR = 3; };
-template <> struct MtShape<64> { static constexpr int WM = 8, WN = 1, MA = 1, NB = 2, AR = 2, BR = 2; };
+template <> struct MtShape<256> { static constexpr int WM = 2, WN = 4, MA = 4, NB = 2, DEEP = 3, FLAT = 2, THREADS = 512; };
+template <> struct MtShape<128> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 2, DEEP = 3, FLAT = 3, THREADS = 512; };
+template <> struct MtShape<64> { static constexpr int WM = 8, WN = 1, MA = 1, NB = 2, DEEP = 2, FLAT = 2, THREADS = 512; };
 
 template <int BN>
-constexpr int mt_lds_bytes() { return (MtShape<BN>::AR * MT_BM + MtShape<BN>::BR * BN) * MT_BK * 2; }
-
-__device__ __forceinline__ int mt_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
-__device__ __forceinline__ void mt_copy(const char* from, uint32_t to) {  // 16 bytes a lane; `to` uniform
-    __builtin_amdgcn_global_load_lds((mt_global_void*)from, (mt_lds_void*)(uintptr_t)to, 16, 0, 0);
+constexpr int mt_lds_bytes() {  // A is the deep one, or the two are alike
+    return (MtShape<BN>::DEEP * MT_BM + MtShape<BN>::FLAT * BN) * MT_BK * 2;
 }
 
-// ---- stages.  N: copies per wave and step (1 KB each, eight waves); issue(i, to): the i-th of them into the buffer at
+__device__ __forceinline__ int mt_wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// The copy path from memory to LDS, 16 bytes a lane: from base + off (base uniform) or from a lane's own address to
+// `to` (uniform) + 16 x lane.  As instructions of our own because the compiler, which cannot tell the buffers apart,
+// puts a wait for all copies under way in front of every transposing LDS read; here they have no register result, and
+// what has to be waited for is written out (mt_meet).  The compiler's own counts of loads under way come out too low
+// beside them, which only makes its waits longer; M0 holds nothing of its own on this target.
+__device__ __forceinline__ void mt_copy(const char* base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base));
+}
+__device__ __forceinline__ void mt_copy_from(const char* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from));
+}
+
+// ---- stages.  N: copies per wave and step (1 KB each); issue(i, to): the i-th of them into the buffer at
 // `to`; advance(): on to the next step.  The addresses are a uniform base plus lane offsets that stay.  A copy writes
 // lane l at 16 l, so the order inside a buffer is chosen by what each lane fetches: all orders below are such that no
 // fragment read meets an LDS bank twice.
 
 // Row r of a buffer: 64 k in 8 chunks of 16 bytes, chunk c at c ^ ((r >> 1) & 7).  Rows past the end read the last one:
 // they make rows of C that nobody keeps.  Rows are less than 2^22 elements apart.
-template <int W>
+template <int W, int BN>
 struct MtAlong {
-    static constexpr int N = W * MT_BK * 2 / 8192;
+    static constexpr int N = W * MT_BK * 2 / 16 / MtShape<BN>::THREADS;
     const char* base;
     uint32_t off[N];
     __device__ __forceinline__ MtAlong() {}
@@ -72,7 +81,7 @@ struct MtAlong {
             off[i] = (uint32_t)row * (uint32_t)ld * 2u + chunk * 16;
         }
     }
-    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
     __device__ __forceinline__ void advance() { base += MT_BK * 2; }
     __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
@@ -80,8 +89,9 @@ struct MtAlong {
 
 // Row k of a buffer: 256 m in 32 chunks, chunk c at c ^ (4 (k & 3)).  Columns past the end (a multiple of 8) read the
 // last eight; rows past the end read the last one, where the other operand is 0.
+template <int BN>
 struct MtAcross {
-    static constexpr int N = 4;
+    static constexpr int N = 2048 / MtShape<BN>::THREADS;
     const char* base;
     uint32_t off[N];
     int64_t ld;
@@ -100,11 +110,11 @@ struct MtAcross {
             off[i] = (uint32_t)row * (uint32_t)ld * 2u + (uint32_t)(col * 2);
         }
     }
-    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const {
         const int row = (mt_wave() * N + i) * 2 + ((threadIdx.x & 63) >> 5);
         const int64_t back = row < left ? 0 : (int64_t)(row - left + 1) * ld * 2;
-        mt_copy(base + off[i] - back, to + (mt_wave() * N + i) * 1024);
+        mt_copy_from(base + off[i] - back, to + (mt_wave() * N + i) * 1024);
     }
     __device__ __forceinline__ void advance() {
         base += ld * (MT_BK * 2);
@@ -114,9 +124,9 @@ struct MtAcross {
 };
 
 // W / 32 x 4 blocks a step, in memory one behind the other (groups past `groups` read the last one).
-template <int W>
+template <int W, int BN>
 struct MtBlocksAlong {
-    static constexpr int N = W * MT_BK * 2 / 8192;
+    static constexpr int N = W * MT_BK * 2 / 16 / MtShape<BN>::THREADS;
     const char* base;
     uint32_t off[N];
     int64_t step;
@@ -132,7 +142,7 @@ struct MtBlocksAlong {
             off[i] = (group * 4 + block % 4) * 1024 + (threadIdx.x & 63) * 16;
         }
     }
-    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
     __device__ __forceinline__ void advance() { base += step; }
     __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
@@ -142,7 +152,7 @@ struct MtBlocksAlong {
 // In a buffer, [64 v][32 n][16 v] blocks whose unit of 16 bytes (n, 8 v h) stands at (2 n + h) ^ (8 in odd blocks): the
 // 32 lanes of a transposing read take 16 different units of a bank row.
 struct MtBlocksAcross {
-    static constexpr int N = 4;
+    static constexpr int N = 2048 / MtShape<256>::THREADS;
     const char* base;
     uint32_t off[N];
     int64_t tile_bytes;  // from one tile of BN n to the next
@@ -160,7 +170,7 @@ struct MtBlocksAcross {
             off[i] = (block >> 3) * (bn * 128) + inner * 1024 + ((unit & 1) * 32 + (unit >> 1)) * 16;
         }
     }
-    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base + off[i], to + (mt_wave() * N + i) * 1024); }
+    __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
     __device__ __forceinline__ void advance() {
         const bool turn = ++at == per;
@@ -237,16 +247,15 @@ __device__ __forceinline__ void mt_meet() {
 //
 // One meeting of the waves per step, in front of its last quarter: by then every wave holds that quarter's fragments
 // in registers, so the step's buffers are free for the copies of a later step, and the next step's copies, under way
-// for AR - 1 (BR - 1) steps, have landed -- its first fragments are read between the products of the last quarter.
+// for one or two steps, have landed -- its first fragments are read between the products of the last quarter.
 // Every LDS read goes out a quarter before its product, early in it, and the copies of a step are spread over two
 // quarters, one behind a product: nothing in the loop waits for what was issued right before.
-template <int BN, class StageA, class ReadA, class StageB, class ReadB>
+template <int BN, class StageA, class ReadA, class StageB, class ReadB, bool B_DEEP = false>
 struct MtPipe {
     typedef MtShape<BN> S;
+    static constexpr int AR = B_DEEP ? S::FLAT : S::DEEP, BR = B_DEEP ? S::DEEP : S::FLAT;
     typedef mt_f32x16 Acc[S::MA][S::NB];
     static constexpr int A_BYTES = MT_BM * MT_BK * 2, B_BYTES = BN * MT_BK * 2;
-    static constexpr int DEEP = S::AR > S::BR ? S::AR : S::BR;
-    static_assert(S::AR >= S::BR, "the copies of A go out last");
     StageA sa;
     StageB sb;
     int nk;
@@ -254,20 +263,20 @@ struct MtPipe {
 
     __device__ __forceinline__ explicit MtPipe(unsigned char* lds) {
         la = (uint32_t)(uintptr_t)(mt_lds_void*)lds;
-        lb = la + S::AR * A_BYTES;
+        lb = la + AR * A_BYTES;
     }
     __device__ __forceinline__ void begin(const StageA& a, const StageB& b, int steps) {
         sa = a;
         sb = b;
         nk = steps;
 #pragma unroll
-        for (int t = 0; t < DEEP; ++t) {
-            if (t < S::BR && t < nk) {
+        for (int t = 0; t < S::DEEP; ++t) {
+            if (t < BR && t < nk) {
 #pragma unroll
                 for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, lb + t * B_BYTES);
                 sb.advance();
             }
-            if (t < S::AR && t < nk) {
+            if (t < AR && t < nk) {
 #pragma unroll
                 for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, la + t * A_BYTES);
                 sa.advance();
@@ -285,7 +294,7 @@ struct MtPipe {
         const int wave = mt_wave();
         const ReadA ra(wave / S::WN * S::MA * 32);
         const ReadB rb(wave % S::WN * S::NB * 32);
-        constexpr int AHEAD = (S::AR - 2) * StageA::N + (S::BR - 2) * StageB::N;  // copies that may stay under way
+        constexpr int AHEAD = (AR - 2) * StageA::N + (BR - 2) * StageB::N;  // copies that may stay under way
         mt_meet<0>();
         uint32_t ca = la, cb = lb;  // the present step's buffers
         mt_s16x8 fa[2][S::MA], fb[2][S::NB];
@@ -319,49 +328,74 @@ struct MtPipe {
         typedef std::integral_constant<int, 1> One;
         auto none = [](int) {};
         int ia = 0, ib = 0, kt = 0;
-        uint32_t free_a = 0;
-        auto step = [&](auto whole_, bool a_due) {  // a_due: A's copies that follow the meeting of the step before
+        uint32_t free_deep = 0;
+        // Copies in step kt: the deep operand's of step kt - 1 + its depth in the first quarter, the flat one's of step
+        // kt + its depth in the last, so that what is needed first goes out first.
+        auto step = [&](auto whole_, bool deep_due) {
             constexpr bool whole = decltype(whole_)::value;
             if constexpr (whole) {
-                quarter(Zero(), ca, cb, 1, std::integral_constant<int, StageA::N>(), [&](int i) { sa.issue(i, free_a); });
-                sa.advance();
+                if constexpr (B_DEEP) {
+                    quarter(Zero(), ca, cb, 1, std::integral_constant<int, StageB::N>(), [&](int i) { sb.issue(i, free_deep); });
+                    sb.advance();
+                } else {
+                    quarter(Zero(), ca, cb, 1, std::integral_constant<int, StageA::N>(), [&](int i) { sa.issue(i, free_deep); });
+                    sa.advance();
+                }
             } else {
                 quarter(Zero(), ca, cb, 1, Zero(), none);
-                if (a_due) {
+                if (deep_due) {
+                    if constexpr (B_DEEP) {
 #pragma unroll
-                    for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, free_a);
-                    sa.advance();
+                        for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, free_deep);
+                        sb.advance();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, free_deep);
+                        sa.advance();
+                    }
                 }
             }
             quarter(One(), ca, cb, 2, Zero(), none);
             quarter(Zero(), ca, cb, 3, Zero(), none);
             if (whole) mt_meet<AHEAD>();
             else mt_meet<0>();
-            const uint32_t free_b = cb;
-            free_a = ca;
-            ia = ia + 1 == S::AR ? 0 : ia + 1;
-            ib = ib + 1 == S::BR ? 0 : ib + 1;
+            const uint32_t free_flat = B_DEEP ? ca : cb;
+            free_deep = B_DEEP ? cb : ca;
+            ia = ia + 1 == AR ? 0 : ia + 1;
+            ib = ib + 1 == BR ? 0 : ib + 1;
             ca = la + ia * A_BYTES;
             cb = lb + ib * B_BYTES;
             if constexpr (whole) {
-                quarter(One(), ca, cb, 0, std::integral_constant<int, StageB::N>(), [&](int i) { sb.issue(i, free_b); });
-                sb.advance();
-            } else {
-                if (kt + S::BR < nk) {
-#pragma unroll
-                    for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, free_b);
+                if constexpr (B_DEEP) {
+                    quarter(One(), ca, cb, 0, std::integral_constant<int, StageA::N>(), [&](int i) { sa.issue(i, free_flat); });
+                    sa.advance();
+                } else {
+                    quarter(One(), ca, cb, 0, std::integral_constant<int, StageB::N>(), [&](int i) { sb.issue(i, free_flat); });
                     sb.advance();
+                }
+            } else {
+                if (kt + S::FLAT < nk) {
+                    if constexpr (B_DEEP) {
+#pragma unroll
+                        for (int i = 0; i < StageA::N; ++i) sa.issue_any(i, free_flat);
+                        sa.advance();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, free_flat);
+                        sb.advance();
+                    }
                 }
                 // behind the last step: whatever the next buffer holds, not used
                 quarter(One(), ca, cb, 0, Zero(), none);
             }
         };
-        // Copies in a whole step kt: A of step kt - 1 + AR (in its first quarter), B of step kt + BR (in its last).
-        const int ws = sa.whole_steps(nk - S::AR) + S::AR, wb = sb.whole_steps(nk - S::BR) + S::BR;  // as seen from here
-        int safe = ws - S::AR + 1 < wb - S::BR ? ws - S::AR + 1 : wb - S::BR;
+        // whole steps of either operand, as seen behind the copies of begin()
+        const int wa = sa.whole_steps(nk - AR) + AR, wb = sb.whole_steps(nk - BR) + BR;
+        const int wd = (B_DEEP ? wb : wa) - S::DEEP + 1, wf = (B_DEEP ? wa : wb) - S::FLAT;
+        const int safe = wd < wf ? wd : wf;
         step(std::false_type(), false);
         for (kt = 1; kt < safe; ++kt) step(std::true_type(), true);
-        for (; kt < nk; ++kt) step(std::false_type(), kt - 1 + S::AR < nk);
+        for (; kt < nk; ++kt) step(std::false_type(), kt - 1 + S::DEEP < nk);
         mt_meet<0>();
     }
 };

@@ -250,12 +250,13 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
     *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
-// G of a chunk of columns, in fragment blocks of 32 n x 16 v, [tile of BN n][64 v][BN / 32][4]: a wave's results are
-// such blocks already, so a store is 1 KB in one piece, and both products read it in pieces of 8 KB and more.
+// G of a chunk of columns, in fragment blocks of 32 n x 16 v, [64 n][64 v][2][4]: a wave's results are such blocks
+// already, so a store is 1 KB in one piece, and both products read it in pieces of 8 KB and more.
 struct LlGrad {
     LlOperands o;
     int m_tiles, n_tiles;
     int v_begin, v64;          // first column of the chunk, its width in 64s
+    int n_pad;                 // rows of G
     float k;
     const LlRow* rows;
     char* out;
@@ -274,10 +275,10 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
     ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int v0 = a.v_begin + tm * MT_BM, r0 = tn * BN;
-        char* const out = a.out + ((int64_t)tn * a.v64 + tm * 4) * (BN * 128) + lane * 16;
         LlRow row[S::NB];
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) row[n] = a.rows[r0 + (wn * S::NB + n) * 32 + (lane & 31)];
+        const int v64 = tm * 4;
         typename LlLogits<BN>::Acc acc;
         pipe.run(acc);
         if (tile + (int)gridDim.x < tiles) {
@@ -287,6 +288,9 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
         const int vw = v0 + wm * S::MA * 32 + 4 * half;
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
+            const int n32 = r0 / 32 + wn * S::NB + n;
+            if (n32 * 32 >= a.n_pad) continue;
+            char* const out = a.out + ((int64_t)(n32 >> 1) * a.v64 + v64) * 8192 + (n32 & 1) * 4096 + lane * 16;
             const float m0 = row[n].m, alpha = row[n].alpha, beta = row[n].beta;
 #pragma unroll
             for (int m = 0; m < S::MA; ++m)
@@ -326,8 +330,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
                     const mt_f32x4 x = {c[8 * q], c[8 * q + 1], c[8 * q + 2], c[8 * q + 3]};
                     const mt_f32x4 y = {c[8 * q + 4], c[8 * q + 5], c[8 * q + 6], c[8 * q + 7]};
                     const int v16 = (wm * S::MA + m) * 2 + q;
-                    *reinterpret_cast<mt_u32x4*>(out + (v16 >> 2) * (BN * 128) + ((wn * S::NB + n) * 4 + (v16 & 3)) * 1024) =
-                        mt_pack8(x, y);
+                    *reinterpret_cast<mt_u32x4*>(out + (v16 >> 2) * 8192 + (v16 & 3) * 1024) = mt_pack8(x, y);
                 }
         }
     }
@@ -337,7 +340,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
 struct LlDh {
     LlOperands o;
     const char* g;
-    int m_tiles, n_tiles, splits, steps, steps_per, v_begin, v64;
+    int m_tiles, n_tiles, splits, steps, steps_per, v_begin, v64, n_pad;
     int add;                   // 1: add to what the chunk before left
     float* slabs;              // [splits][N][H]
 };
@@ -356,7 +359,8 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong, LL_DH_BDEEP && BN == 256> pipe(lds);
     typename decltype(pipe)::Acc acc;
     pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
-               MtBlocksAlong<BN, BN>(a.g + ((int64_t)tn * a.v64 + s0) * (BN * 128), BN * 128, BN / 32), s1 - s0);
+               MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u, a.n_pad / 32 - r0 / 32),
+               s1 - s0);
     pipe.run(acc);
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(const float*
 struct LlDw {
     const char* copy;
     const char* g;
-    int H, V, bn;
+    int H, V;
     int m_tiles, n_tiles, steps, v_begin, v64;
     uint16_t* out;             // [V][H]
 };
@@ -407,8 +411,8 @@ __device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int t
     const int rest = tile - group * 8 * a.m_tiles;
     h0 = rest / wide * MT_BM;
     c0 = (group * 8 + rest % wide) * 256;
-    pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, a.H / 32 - h0 / 32),
-               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * (a.bn * 128), (int64_t)a.v64 * (a.bn * 128), a.bn), a.steps);
+    pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
+               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), a.steps);
 }
 
 __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel(LlDw a) {
@@ -447,12 +451,21 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
 // ---- host ------------------------------------------------------------------------------------------
 static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// Rows per tile: as few as hold all rows.
-static int ll_bn(int N) {
-#ifdef LL_FORCE_BN
-    return LL_FORCE_BN;
-#endif
-    return N <= 64 ? 64 : N <= 128 ? 128 : 256;
+// Rows per tile of the products with the logits' shape (m_tiles x n tiles of 256 x BN).  A tile of 64 rows costs about
+// 0.37 of one of 256, one of 128 0.64 (measured per round of 256 tiles at H = 2048: 24, 40 and 64 us; two workgroups of
+// 64 rows share a CU); what counts is whole rounds over the CUs.
+static int ll_bn(int N, int64_t m_tiles) {
+    int best = 0;
+    double least = 0.0;
+    for (int bn = 64; bn <= 256; bn *= 2) {
+        const int64_t tiles = m_tiles * ((N + bn - 1) / bn), wgs = bn == 64 ? 2 * LL_CUS : LL_CUS;
+        const double cost = (double)((tiles + wgs - 1) / wgs) * (bn == 64 ? 0.74 : bn == 128 ? 0.64 : 1.0);
+        if (best == 0 || cost <= least) {
+            best = bn;
+            least = cost;
+        }
+    }
+    return best;
 }
 
 struct LlForward {
@@ -465,8 +478,8 @@ static int ll_wm(int bn) { return bn == 64 ? MtShape<64>::WM : bn == 128 ? MtSha
 
 static LlForward ll_forward(int N, int V, bool ent) {
     LlForward f;
-    f.bn = ll_bn(N);
     f.m_tiles = (V + MT_BM - 1) / MT_BM;
+    f.bn = ll_bn(N, f.m_tiles);
     f.n_tiles = (N + f.bn - 1) / f.bn;
     f.parts = f.m_tiles * ll_wm(f.bn);
     f.n_pad = (int64_t)f.n_tiles * f.bn;
@@ -478,8 +491,9 @@ static LlForward ll_forward(int N, int V, bool ent) {
 }
 
 struct LlBackward {
-    int bn, n_tiles, h_tiles;
-    int64_t n_pad;             // rows of G: whole tiles
+    int bn, n_tiles;           // of d logits
+    int dh_bn, dh_tiles, h_tiles;  // of d hidden
+    int64_t n_pad;             // rows of G: whole steps of d weight
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
     int splits;
@@ -503,20 +517,22 @@ static int ll_splits(int64_t tiles, int64_t steps) {
 
 static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     LlBackward b;
-    b.bn = ll_bn(N);
-    b.n_tiles = (N + b.bn - 1) / b.bn;
+    b.dh_bn = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+    b.dh_tiles = (N + b.dh_bn - 1) / b.dh_bn;
     b.h_tiles = (H + MT_BM - 1) / MT_BM;
-    b.n_pad = (int64_t)b.n_tiles * b.bn;
+    b.n_pad = ll_up(N, MT_BK);
     const int64_t v_pad = ll_up(V, MT_BM);
     int64_t most = LL_CHUNK_BYTES / 2 / b.n_pad / MT_BM * MT_BM;
     if (most < MT_BM) most = MT_BM;
     b.n_chunks = (int)((v_pad + most - 1) / most);
     b.chunk = ll_up((v_pad + b.n_chunks - 1) / b.n_chunks, MT_BM);
     b.n_chunks = (int)((v_pad + b.chunk - 1) / b.chunk);
-    b.splits = ll_splits((int64_t)b.h_tiles * b.n_tiles, b.chunk / MT_BK);
+    b.bn = ll_bn(N, b.chunk / MT_BM);
+    b.n_tiles = (N + b.bn - 1) / b.bn;
+    b.splits = ll_splits((int64_t)b.h_tiles * b.dh_tiles, b.chunk / MT_BK);
     b.rows = 0;
-    b.copy = (size_t)ll_up(b.n_pad * sizeof(LlRow), 256);
-    b.g = b.copy + (want_w ? (size_t)ll_up(N, MT_BK) * H * 2 : 0);
+    b.copy = (size_t)ll_up(ll_up(N, 256) * sizeof(LlRow), 256);  // tiles may reach past n_pad
+    b.g = b.copy + (want_w ? (size_t)b.n_pad * H * 2 : 0);
     b.slabs = b.g + (size_t)(b.n_pad * b.chunk * 2);
     b.total = b.slabs + (want_h ? (size_t)b.splits * N * H * sizeof(float) : 0);
     return b;
@@ -661,7 +677,7 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     GRX_REQUIRE(scratch != nullptr && scratch_bytes >= b.total, GRX_E_WORKSPACE, "%s: scratch of %zu bytes, need %zu", who,
                 scratch_bytes, b.total);
     GRX_REQUIRE(((uintptr_t)scratch & 15u) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
-    GRX_REQUIRE((int64_t)b.splits * b.h_tiles * b.n_tiles < (1 << 23), GRX_E_UNSUPPORTED, "%s: too many tiles", who);
+    GRX_REQUIRE((int64_t)b.splits * b.h_tiles * b.dh_tiles < (1 << 23), GRX_E_UNSUPPORTED, "%s: too many tiles", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
     LlRow* rows = reinterpret_cast<LlRow*>(s + b.rows);
@@ -672,21 +688,22 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
 
     LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
                  (float)(1.0 / (double)p->temperature), rows, copy};
-    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_pad / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
+    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(ll_up(p->N, 256) / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
                        stream, pr);
     GRX_CHECK_HIP(hipGetLastError());
     for (int c = 0; c < b.n_chunks; ++c) {
         const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
-        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (float)(1.4426950408889634 / (double)p->temperature), rows, g};
+        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (int)b.n_pad, (float)(1.4426950408889634 / (double)p->temperature), rows, g};
         LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * d.n_tiles), d);
         if (want_h) {
             const int steps = (int)(cols / MT_BK);
-            LlDh x = {o, g, b.h_tiles, b.n_tiles, b.splits, steps, (steps + b.splits - 1) / b.splits, v0, v64, c > 0, slabs};
-            LL_EACH(b.bn, lm_logps_dhidden_kernel, b.splits * b.h_tiles * b.n_tiles, x);
+            LlDh x = {o, g, b.h_tiles, b.dh_tiles, b.splits, steps, (steps + b.splits - 1) / b.splits, v0, v64, (int)b.n_pad, c > 0,
+                      slabs};
+            LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, b.splits * b.h_tiles * b.dh_tiles, x);
         }
         if (want_w) {
-            LlDw x = {copy, g, p->H, p->V, b.bn, b.h_tiles, (int)(cols / 256), (int)((p->N + MT_BK - 1) / MT_BK), v0, v64,
+            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
             LL_ONE(256, lm_logps_dweight_kernel, ll_resident(256, (int64_t)x.m_tiles * x.n_tiles), x);
         }

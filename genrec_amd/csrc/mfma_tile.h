@@ -123,7 +123,8 @@ struct MtAcross {
     __device__ __forceinline__ int whole_steps(int nk) const { return nk < left / MT_BK ? nk : left / MT_BK; }
 };
 
-// W / 32 x 4 blocks a step, in memory one behind the other (groups past `groups` read the last one).
+// W / 32 x 4 blocks a step: the four of a group of 32 rows in one piece, the groups of a pair one behind the other,
+// pairs `pair_bytes` apart (less than 2^31 in all).  Groups past `groups` read the last one.
 template <int W, int BN>
 struct MtBlocksAlong {
     static constexpr int N = W * MT_BK * 2 / 16 / MtShape<BN>::THREADS;
@@ -132,14 +133,14 @@ struct MtBlocksAlong {
     int64_t step;
     __device__ __forceinline__ MtBlocksAlong() {}
     // p: the step's first block; groups: groups of 32 rows that are there from it on
-    __device__ __forceinline__ MtBlocksAlong(const char* p, int64_t step_bytes, int groups) {
+    __device__ __forceinline__ MtBlocksAlong(const char* p, int64_t step_bytes, uint32_t pair_bytes, int groups) {
         base = p;
         step = step_bytes;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int block = mt_wave() * N + i;
             const int group = block / 4 < groups ? block / 4 : groups - 1;
-            off[i] = (group * 4 + block % 4) * 1024 + (threadIdx.x & 63) * 16;
+            off[i] = (uint32_t)(group >> 1) * pair_bytes + ((group & 1) * 4 + block % 4) * 1024 + (threadIdx.x & 63) * 16;
         }
     }
     __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
@@ -148,35 +149,28 @@ struct MtBlocksAlong {
     __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
 };
 
-// G as d weight reads it: blocks of 32 n x 16 v, in memory [tile of BN n][64 v][BN / 32][4], a step being 64 n of 256 v.
+// G as d weight reads it: blocks of 32 n x 16 v, in memory [64 n][64 v][2][4], a step being 64 n of 256 v.
 // In a buffer, [64 v][32 n][16 v] blocks whose unit of 16 bytes (n, 8 v h) stands at (2 n + h) ^ (8 in odd blocks): the
 // 32 lanes of a transposing read take 16 different units of a bank row.
 struct MtBlocksAcross {
     static constexpr int N = 2048 / MtShape<256>::THREADS;
     const char* base;
     uint32_t off[N];
-    int64_t tile_bytes;  // from one tile of BN n to the next
-    int per, at;         // steps in such a tile, the present one
+    int64_t step;
     __device__ __forceinline__ MtBlocksAcross() {}
-    __device__ __forceinline__ MtBlocksAcross(const char* p, int64_t tile_bytes_, int bn) {
+    __device__ __forceinline__ MtBlocksAcross(const char* p, int64_t step_bytes) {
         base = p;
-        tile_bytes = tile_bytes_;
-        per = bn / 64;
-        at = 0;
+        step = step_bytes;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int block = mt_wave() * N + i, inner = block & 7;  // inner: 2 of 32 n, 4 of 16 v
-            const int unit = (threadIdx.x & 63) ^ ((inner & 1) << 3);
-            off[i] = (block >> 3) * (bn * 128) + inner * 1024 + ((unit & 1) * 32 + (unit >> 1)) * 16;
+            const int block = mt_wave() * N + i;
+            const int unit = (threadIdx.x & 63) ^ ((block & 1) << 3);
+            off[i] = block * 1024 + ((unit & 1) * 32 + (unit >> 1)) * 16;
         }
     }
     __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
-    __device__ __forceinline__ void advance() {
-        const bool turn = ++at == per;
-        base += turn ? tile_bytes - (per - 1) * 8192 : 8192;
-        at = turn ? 0 : at;
-    }
+    __device__ __forceinline__ void advance() { base += step; }
     __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
 };
 

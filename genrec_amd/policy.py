@@ -15,6 +15,7 @@ Everything runs on the current stream; nothing is read back.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional
 
 import torch
@@ -33,12 +34,20 @@ def _same_device(dev, **tensors) -> None:
             raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
 def _scratch(n: int, dev):
     return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
 
 
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
+def _run(call, index: int, *args) -> None:
+    """``call(*args, current stream)`` with device ``index`` current."""
+    with _lib.on_device(index):
+        status = call(*args, _lib.current_stream_ptr(index))
+    if status:
+        _lib.check(status)
 
 
 def _rows_2d(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -47,12 +56,18 @@ def _rows_2d(t: torch.Tensor, what: str) -> torch.Tensor:
         return t.unsqueeze(1)
     if t.dim() != 2:
         raise ValueError(f"{what} must be [rows] or [rows, positions], got {tuple(t.shape)}")
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _f32_rows(t: Optional[torch.Tensor], what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    return _rows_2d(t if t.dtype is torch.float32 else t.detach().to(torch.float32), what)
 
 
 def _temperature(value) -> float:
     value = float(value)
-    if not 0.0 < value < float("inf"):
+    if not 0.0 < value < math.inf:
         raise ValueError(f"temperature must be positive and finite, got {value}")
     return value
 
@@ -60,10 +75,11 @@ def _temperature(value) -> float:
 def _token_ids(ids: torch.Tensor, dev) -> torch.Tensor:
     if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
         raise TypeError(f"token_ids must be integers, got {ids.dtype}")
-    _same_device(dev, token_ids=ids)
+    if ids.device != dev:
+        raise ValueError(f"token_ids is on {ids.device}, expected {dev}")
     if ids.numel() > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows per call, got {ids.numel()}")
-    return _rows_2d(ids.detach().to(torch.int64), "token_ids")
+    return _rows_2d(ids if ids.dtype is torch.int64 else ids.to(torch.int64), "token_ids")
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
@@ -75,57 +91,45 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grad_rows(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return None if g is None else g.to(torch.float32).contiguous()
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
+
+
+def _token_logps_args(logits, ids, temperature, logps, stats, entropy, g=None, h=None, grad=None):
+    three = logits.dim() == 3
+    return _lib.GrxTokenLogpsArgs(
+        logits.data_ptr(), logits.stride(0), logits.stride(1) if three else 0, ids.data_ptr(), ids.stride(0), ids.shape[0],
+        ids.shape[1], logits.shape[-1], _lib.torch_dtype_code(logits.dtype), temperature, 0, logps, stats, entropy, g, h, grad)
 
 
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, temperature, entropy):
-        B, T = ids.shape
-        dev = logits.device
-        V = logits.shape[-1]
-        a = _lib.GrxTokenLogpsArgs()
-        a.logits = logits.data_ptr()
-        a.row_stride, a.pos_stride = logits.stride(0), (logits.stride(1) if logits.dim() == 3 else 0)
-        a.token_ids, a.ids_stride = ids.data_ptr(), ids.stride(0)
-        a.B, a.T, a.V, a.dtype, a.temperature = B, T, V, _lib.torch_dtype_code(logits.dtype), temperature
-        out = torch.empty((2, B, T) if entropy else (1, B, T), dtype=torch.float32, device=dev)
-        stats = torch.empty((B, T, 2), dtype=torch.float32, device=dev)
-        a.logps, a.row_stats = out.data_ptr(), stats.data_ptr()
-        logps, ent = out[0], None
-        if entropy:
-            ent = out[1]
-            a.entropy = ent.data_ptr()
-        index = dev.index
+        shape, dev = ids.shape, logits.device
+        logps = torch.empty(shape, dtype=torch.float32, device=dev)
+        ent = torch.empty(shape, dtype=torch.float32, device=dev) if entropy else None
+        stats = torch.empty((*shape, 2), dtype=torch.float32, device=dev)
+        a = _token_logps_args(logits, ids, temperature, logps.data_ptr(), stats.data_ptr(), _ptr(ent))
         lib = _lib.lib()
-        n = lib.grx_token_logps_scratch_bytes(B * T, V, a.dtype)
+        n = lib.grx_token_logps_scratch_bytes(a.B * a.T, a.V, a.dtype)
         scratch = _scratch(n, dev)
-        with _lib.on_device(index):
-            _lib.check(lib.grx_token_logps(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
-        ctx.save_for_backward(logits, ids, stats, *((ent,) if entropy else ()))
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
+        _run(lib.grx_token_logps, dev.index, C.byref(a), _ptr(scratch), n)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(logits, ids, stats, ent)
+            ctx.temperature = temperature
+            ctx.set_materialize_grads(False)
         return (logps, ent) if entropy else logps
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logps, g_entropy=None):
-        logits, ids, stats, *rest = ctx.saved_tensors
-        B, T = ids.shape
-        dev = logits.device
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        logits, ids, stats, ent = ctx.saved_tensors
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         g_logps, g_entropy = _grad_rows(g_logps), _grad_rows(g_entropy)
-        a = _lib.GrxTokenLogpsArgs()
-        a.logits = logits.data_ptr()
-        a.row_stride, a.pos_stride = logits.stride(0), (logits.stride(1) if logits.dim() == 3 else 0)
-        a.token_ids, a.ids_stride = ids.data_ptr(), ids.stride(0)
-        a.B, a.T, a.V, a.dtype, a.temperature = B, T, logits.shape[-1], _lib.torch_dtype_code(logits.dtype), ctx.temperature
-        a.row_stats = stats.data_ptr()
-        a.entropy = _ptr(rest[0]) if rest else None
-        a.grad_logps, a.grad_entropy, a.grad_logits = _ptr(g_logps), _ptr(g_entropy), grad.data_ptr()
-        index = dev.index
-        with _lib.on_device(index):
-            _lib.check(_lib.lib().grx_token_logps_backward(C.byref(a), _lib.current_stream_ptr(index)))
+        a = _token_logps_args(logits, ids, ctx.temperature, None, stats.data_ptr(), _ptr(ent), _ptr(g_logps), _ptr(g_entropy),
+                              grad.data_ptr())
+        _run(_lib.lib().grx_token_logps_backward, logits.device.index, C.byref(a))
         return grad, None, None, None
 
 
@@ -157,60 +161,48 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
     return tuple(t.reshape(shape) for t in out) if return_entropy else out.reshape(shape)
 
 
+def _lm_token_logps_args(hidden, weight, ids, temperature, logps, stats, entropy, g=None, h=None, grad_h=None, grad_w=None):
+    (N, H), V = hidden.shape, weight.shape[0]
+    return _lib.GrxLmTokenLogpsArgs(
+        hidden.data_ptr(), hidden.stride(0) if N > 1 else H, weight.data_ptr(), weight.stride(0) if V > 1 else H, ids.data_ptr(),
+        N, H, V, temperature, logps, stats, entropy, g, h, grad_h, grad_w)
+
+
 class _LmTokenLogps(torch.autograd.Function):
     @staticmethod
-    def _args(hidden, weight, ids, temperature):
-        a = _lib.GrxLmTokenLogpsArgs()
-        a.hidden, a.hidden_stride = hidden.data_ptr(), hidden.stride(0) if hidden.shape[0] > 1 else hidden.shape[1]
-        a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0) if weight.shape[0] > 1 else weight.shape[1]
-        a.token_ids, a.temperature = ids.data_ptr(), temperature
-        (a.N, a.H), a.V = hidden.shape, weight.shape[0]
-        return a
-
-    @staticmethod
     def forward(ctx, hidden, weight, ids, temperature, entropy):
-        N = hidden.shape[0]
-        dev = hidden.device
-        a = _LmTokenLogps._args(hidden, weight, ids, temperature)
-        out = torch.empty((2, N) if entropy else (1, N), dtype=torch.float32, device=dev)
+        N, dev = hidden.shape[0], hidden.device
+        logps = torch.empty(N, dtype=torch.float32, device=dev)
+        ent = torch.empty(N, dtype=torch.float32, device=dev) if entropy else None
         stats = torch.empty((N, 2), dtype=torch.float32, device=dev)
-        a.logps, a.row_stats = out.data_ptr(), stats.data_ptr()
-        logps, ent = out[0], None
-        if entropy:
-            ent = out[1]
-            a.entropy = ent.data_ptr()
-        index = dev.index
+        a = _lm_token_logps_args(hidden, weight, ids, temperature, logps.data_ptr(), stats.data_ptr(), _ptr(ent))
         lib = _lib.lib()
         n = lib.grx_lm_token_logps_scratch_bytes(N, a.H, a.V, int(entropy))
         scratch = _scratch(n, dev)
-        with _lib.on_device(index):
-            _lib.check(lib.grx_lm_token_logps(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
-        ctx.save_for_backward(hidden, weight, ids, stats, *((ent,) if entropy else ()))
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
+        _run(lib.grx_lm_token_logps, dev.index, C.byref(a), _ptr(scratch), n)
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            ctx.save_for_backward(hidden, weight, ids, stats, ent)
+            ctx.temperature = temperature
+            ctx.set_materialize_grads(False)
         return (logps, ent) if entropy else logps
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_logps, g_entropy=None):
-        hidden, weight, ids, stats, *rest = ctx.saved_tensors
-        dev = hidden.device
-        a = _LmTokenLogps._args(hidden, weight, ids, ctx.temperature)
+        hidden, weight, ids, stats, ent = ctx.saved_tensors
+        dev, N = hidden.device, hidden.shape[0]
         want_h, want_w = ctx.needs_input_grad[:2]
         grad_h = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
         grad_w = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
-        if a.N == 0 and want_w:
+        if N == 0 and want_w:
             grad_w.zero_()
         g_logps, g_entropy = _grad_rows(g_logps), _grad_rows(g_entropy)
-        a.row_stats, a.entropy = stats.data_ptr(), (_ptr(rest[0]) if rest else None)
-        a.grad_logps, a.grad_entropy = _ptr(g_logps), _ptr(g_entropy)
-        a.grad_hidden, a.grad_weight = _ptr(grad_h), _ptr(grad_w)
-        index = dev.index
+        a = _lm_token_logps_args(hidden, weight, ids, ctx.temperature, None, stats.data_ptr(), _ptr(ent), _ptr(g_logps),
+                                 _ptr(g_entropy), _ptr(grad_h), _ptr(grad_w))
         lib = _lib.lib()
-        n = lib.grx_lm_token_logps_backward_scratch_bytes(a.N, a.H, a.V, int(want_h), int(want_w))
+        n = lib.grx_lm_token_logps_backward_scratch_bytes(N, a.H, a.V, int(want_h), int(want_w))
         scratch = _scratch(n, dev)
-        with _lib.on_device(index):
-            _lib.check(lib.grx_lm_token_logps_backward(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
+        _run(lib.grx_lm_token_logps_backward, dev.index, C.byref(a), _ptr(scratch), n)
         return grad_h, grad_w, None, None, None
 
 
@@ -261,37 +253,28 @@ class PolicyLoss:
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logps, a, keep):
+    def forward(ctx, logps, a, stats):
         dev = logps.device
-        R, T = logps.shape
-        out = torch.empty(5, dtype=torch.float32, device=dev)
-        loss, stats = out[0], out[1:]
-        unit = torch.empty((R, T), dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        unit = torch.empty(logps.shape, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
         a.loss, a.stats, a.unit_grad = loss.data_ptr(), stats.data_ptr(), _ptr(unit)
-        index = dev.index
         lib = _lib.lib()
-        n = lib.grx_policy_loss_scratch_bytes(R, T)
+        n = lib.grx_policy_loss_scratch_bytes(a.R, a.T)
         scratch = _scratch(n, dev)
-        with _lib.on_device(index):
-            _lib.check(lib.grx_policy_loss(C.byref(a), _ptr(scratch), n, _lib.current_stream_ptr(index)))
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
+        _run(lib.grx_policy_loss, dev.index, C.byref(a), _ptr(scratch), n)
         if unit is not None:
             ctx.save_for_backward(unit, stats)
-        return loss, stats
+        return loss
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, g_loss, _g_stats):
-        if g_loss is None:
-            return None, None, None
+    def backward(ctx, g_loss):
         unit, stats = ctx.saved_tensors
         grad = torch.empty_like(unit)
-        g_loss = g_loss.to(torch.float32)
-        index = unit.device.index
-        with _lib.on_device(index):
-            _lib.check(_lib.lib().grx_policy_loss_backward(unit.data_ptr(), stats.data_ptr(), g_loss.data_ptr(),
-                                                           unit.numel(), grad.data_ptr(), _lib.current_stream_ptr(index)))
+        if g_loss.dtype is not torch.float32:
+            g_loss = g_loss.to(torch.float32)
+        _run(_lib.lib().grx_policy_loss_backward, unit.device.index, unit.data_ptr(), stats.data_ptr(), g_loss.data_ptr(),
+             unit.numel(), grad.data_ptr())
         return grad, None, None
 
 
@@ -326,18 +309,20 @@ def policy_loss(
     ``num_items`` (the valid tokens of the whole step, e.g. over gradient accumulation).  ``epsilon_high`` defaults
     to ``epsilon_low``; ``delta`` must lie above 1 + ``epsilon_high``.  Masked positions are not read, whatever they
     hold, and get gradient 0; a batch without valid tokens has loss 0.  Only ``logps`` gets a gradient."""
-    dev = logps.device
-    if logps.dim() != 2:
-        raise ValueError(f"logps must be [rows, positions], got {tuple(logps.shape)}")
-    R, T = logps.shape
-    if max(R, T) >= 1 << 31:
+    dev, shape = logps.device, logps.shape
+    if len(shape) != 2:
+        raise ValueError(f"logps must be [rows, positions], got {tuple(shape)}")
+    R, T = shape
+    if R >= 1 << 31 or T >= 1 << 31:
         raise ValueError("rows and positions must stay below 2^31")
     for name, t in (("mask", mask), ("old_logps", old_logps), ("ref_logps", ref_logps)):
-        if t is not None and t.shape != logps.shape:
-            raise ValueError(f"{name} must have the shape of logps {tuple(logps.shape)}, got {tuple(t.shape)}")
-    if tuple(advantages.shape) not in ((R,), (R, T)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{name} must have the shape of logps {tuple(shape)}, got {tuple(t.shape)}")
+    if advantages.shape != shape and advantages.shape != shape[:1]:
         raise ValueError(f"advantages must be [{R}] or [{R}, {T}], got {tuple(advantages.shape)}")
-    _same_device(dev, mask=mask, old_logps=old_logps, ref_logps=ref_logps, advantages=advantages)
+    for name, t in (("mask", mask), ("old_logps", old_logps), ("ref_logps", ref_logps), ("advantages", advantages)):
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
     for name, t in (("logps", logps), ("old_logps", old_logps), ("ref_logps", ref_logps), ("advantages", advantages)):
         if t is not None and not t.is_floating_point():
             raise TypeError(f"{name} must be floating point, got {t.dtype}")
@@ -346,41 +331,35 @@ def policy_loss(
     if importance_sampling_level not in ("token", "sequence"):
         raise ValueError(f"importance_sampling_level must be 'token' or 'sequence', got {importance_sampling_level!r}")
     epsilon_high = epsilon_low if epsilon_high is None else epsilon_high
-    if not (0.0 <= epsilon_low < 1.0 and 0.0 <= epsilon_high < float("inf")):
+    if not (0.0 <= epsilon_low < 1.0 and 0.0 <= epsilon_high < math.inf):
         raise ValueError(f"epsilon_low must lie in [0, 1) and epsilon_high must not be negative, got {epsilon_low}, {epsilon_high}")
-    if delta is not None and not 1.0 + epsilon_high < delta < float("inf"):
+    if delta is not None and not 1.0 + epsilon_high < delta < math.inf:
         raise ValueError(f"delta must lie above 1 + epsilon_high, got {delta}")
-    if not -float("inf") < beta < float("inf"):
+    if not -math.inf < beta < math.inf:
         raise ValueError(f"beta must be finite, got {beta}")
     if beta != 0.0 and ref_logps is None:
         raise ValueError("a KL term (beta) needs ref_logps")
     normalizer = 0.0
-    if loss_type in ("dr_grpo", "dapo"):
+    if loss_type == "dr_grpo" or loss_type == "dapo":
         given = max_completion_length if loss_type == "dr_grpo" else num_items
-        if given is None or not 0.0 < float(given) < float("inf"):
+        if given is None or not 0.0 < float(given) < math.inf:
             raise ValueError(f"loss_type {loss_type!r} needs a positive "
                              f"{'max_completion_length' if loss_type == 'dr_grpo' else 'num_items'}, got {given}")
         normalizer = float(given) * (max(R, 1) if loss_type == "dr_grpo" else 1)
     _lib.require_cuda(logps, "logps")
-    f32 = torch.float32
-    logps = logps if logps.dtype == f32 else logps.to(f32)
+    # without detach() where nothing is converted: only addresses are taken of these
+    if logps.dtype is not torch.float32:
+        logps = logps.to(torch.float32)
     logps = _rows_2d(logps, "logps")
-    old, ref = (None if t is None else _rows_2d(t.detach().to(f32), "log-probabilities") for t in (old_logps, ref_logps))
-    adv = advantages.detach().to(f32)
+    old, ref = _f32_rows(old_logps, "old_logps"), _f32_rows(ref_logps, "ref_logps")
+    adv = advantages if advantages.dtype is torch.float32 else advantages.detach().to(torch.float32)
     if mask.dtype not in _MASK_TYPES:
         mask = mask > 0
-    mask = _rows_2d(mask.detach(), "mask")
-    a = _lib.GrxPolicyLossArgs()
-    a.logps, a.logps_stride = logps.data_ptr(), logps.stride(0)
-    if old is not None:
-        a.old_logps, a.old_stride = old.data_ptr(), old.stride(0)
-    if ref is not None:
-        a.ref_logps, a.ref_stride = ref.data_ptr(), ref.stride(0)
-    a.advantages = adv.data_ptr()
-    a.adv_row_stride, a.adv_pos_stride = adv.stride(0), (adv.stride(1) if adv.dim() == 2 else 0)
-    a.mask, a.mask_stride, a.mask_type = mask.data_ptr(), mask.stride(0), _MASK_TYPES[mask.dtype]
-    a.R, a.T = R, T
-    a.sequence_level, a.row_mean = int(importance_sampling_level == "sequence"), int(loss_type == "grpo")
-    a.beta, a.epsilon_low, a.epsilon_high = beta, epsilon_low, epsilon_high
-    a.delta, a.normalizer = delta or 0.0, normalizer
-    return PolicyLoss(*_PolicyLoss.apply(logps, a, (old, ref, adv, mask)))
+    mask = _rows_2d(mask, "mask")
+    stats = torch.empty(4, dtype=torch.float32, device=dev)
+    a = _lib.GrxPolicyLossArgs(
+        logps.data_ptr(), logps.stride(0), _ptr(old), old.stride(0) if old is not None else 0, _ptr(ref),
+        ref.stride(0) if ref is not None else 0, adv.data_ptr(), adv.stride(0), adv.stride(1) if adv.dim() == 2 else 0,
+        mask.data_ptr(), mask.stride(0), _MASK_TYPES[mask.dtype], R, T, importance_sampling_level == "sequence",
+        loss_type == "grpo", beta, epsilon_low, epsilon_high, delta or 0.0, normalizer)
+    return PolicyLoss(_PolicyLoss.apply(logps, a, stats), stats)

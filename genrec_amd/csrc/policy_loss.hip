@@ -17,7 +17,7 @@
 #define PL_THREADS 256
 #define PL_BIG 1024
 #define PL_SINGLE_TOKENS 4096   // up to here one workgroup does the whole call
-#define PL_MAX_WGS 1024
+#define PL_MAX_WGS 2048
 #define PL_SUMS 5               // loss, kl, clipped below, clipped above, valid tokens
 
 struct PlArgs {
@@ -40,7 +40,7 @@ __device__ __forceinline__ bool pl_valid(const grx_policy_loss_args& p, int64_t 
 }
 
 // exp(q) - 1 - q without the cancellation near 0: its Taylor series (the first term left out is below 2^-26 of the
-// sum for |q| < 1), the difference itself elsewhere.
+// sum for |q| < 1), the difference itself elsewhere.  With q added it is exp(q) - 1.
 __device__ __forceinline__ float pl_kl(float q) {
     if (fabsf(q) < 1.f) {
         float s = 1.f / 39916800.f;
@@ -74,6 +74,32 @@ __device__ __forceinline__ double pl_row_sum(double v, double* lds) {
     return v;
 }
 
+struct PlTerm {
+    float loss, slope, kl, kl_slope;
+    bool cut_low, cut_high;
+};
+
+// A thread's share of the sums; loss: of its present row, without the row's weight.
+struct PlShare {
+    double total, loss, kl;
+    int low, high, valid;
+};
+
+// One token: d = log ratio in 64 bits, w = exp(d); q = ref - logp where there is a reference.
+__device__ __forceinline__ PlTerm pl_term(const PlArgs& a, double d, float w, float adv, bool ref, float q) {
+    PlTerm r;
+    r.kl = ref ? pl_kl(q) : 0.f;
+    r.kl_slope = ref ? -a.p.beta * (r.kl + q) : 0.f;
+    const bool below = d < a.log_low, above = d > a.log_high, capped = d > a.log_delta;
+    const float first = (capped ? a.delta : w) * adv;
+    const float second = (below ? a.low : above ? a.high : w) * adv;
+    r.loss = fmaf(a.p.beta, r.kl, -(second < first ? second : first));  // a NaN of either stays
+    r.cut_low = below && adv < 0.f;
+    r.cut_high = above && adv > 0.f;
+    r.slope = (r.cut_low || r.cut_high || capped) ? 0.f : -w * adv;
+    return r;
+}
+
 // What the call returns, from the sums over all tokens.  global: the factor that the stored gradient still lacks.
 __device__ __forceinline__ void pl_finish(const PlArgs& a, const double* s) {
     const double tokens = s[4] > 1.0 ? s[4] : 1.0;
@@ -85,86 +111,18 @@ __device__ __forceinline__ void pl_finish(const PlArgs& a, const double* s) {
     a.p.stats[3] = (float)global;
 }
 
-// LANES lanes share a row; a workgroup of THREADS threads holds THREADS / LANES rows at a time.
-template <int LANES, int THREADS>
-__global__ __launch_bounds__(THREADS) void policy_loss_kernel(PlArgs a) {
-    __shared__ double lds[16 * PL_SUMS];
-    const grx_policy_loss_args& p = a.p;
-    constexpr int ROWS = THREADS / LANES;
-    const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES;
-    double sum[PL_SUMS] = {0.0, 0.0, 0.0, 0.0, 0.0};
-    // every thread of the workgroup makes the same number of turns (barriers inside): rows past the end are empty
-    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < p.R; base += (int64_t)gridDim.x * ROWS) {
-        const int64_t r = base + slot;
-        const bool live = r < p.R;
-        const float* lp = p.logps + r * p.logps_stride;
-        const float* old = p.old_logps ? p.old_logps + r * p.old_stride : nullptr;
-        const float* ref = p.ref_logps ? p.ref_logps + r * p.ref_stride : nullptr;
-        float* grad = p.unit_grad ? p.unit_grad + r * p.T : nullptr;
-        double row_w = 1.0, row_d = 0.0, inv_n = 1.0;
-        if (p.row_mean || p.sequence_level) {
-            double n = 0.0, d = 0.0;
-            if (live)
-                for (int t = lane; t < p.T; t += LANES)
-                    if (pl_valid(p, r, t)) {
-                        n += 1.0;
-                        if (p.sequence_level && old) d += (double)lp[t] - (double)old[t];
-                    }
-            n = pl_row_sum<LANES>(n, lds);
-            inv_n = 1.0 / (n > 1.0 ? n : 1.0);
-            if (p.sequence_level) row_d = pl_row_sum<LANES>(d, lds) * inv_n;
-            if (p.row_mean) row_w = inv_n;
-        }
-        float seq_w = 1.f;
-        double seq_slope = 0.0;
-        if (p.sequence_level) seq_w = expf((float)row_d);
-        for (int pass = 0; pass < (p.sequence_level && grad ? 2 : 1); ++pass) {
-            // second pass (one ratio per sequence): every token of the row carries the row's slope
-            if (pass == 1) seq_slope = pl_row_sum<LANES>(seq_slope, lds) * inv_n;
-            if (live)
-                for (int t = lane; t < p.T; t += LANES) {
-                    if (!pl_valid(p, r, t)) {
-                        if (grad && pass == 0) grad[t] = 0.f;
-                        continue;
-                    }
-                    const float x = lp[t];
-                    float kl = 0.f, kl_slope = 0.f;
-                    if (ref) {
-                        const float q = (float)((double)ref[t] - (double)x);
-                        kl = pl_kl(q);
-                        kl_slope = -p.beta * expm1f(q);
-                    }
-                    if (pass == 1) {
-                        grad[t] = (float)(row_w * (seq_slope + (double)kl_slope));
-                        continue;
-                    }
-                    double d = row_d;
-                    float w = seq_w;
-                    if (!p.sequence_level) {
-                        d = old ? (double)x - (double)old[t] : 0.0;
-                        w = expf((float)d);
-                    }
-                    const float adv = p.advantages[r * p.adv_row_stride + (int64_t)t * p.adv_pos_stride];
-                    const bool below = d < a.log_low, above = d > a.log_high, capped = d > a.log_delta;
-                    const float first = (capped ? a.delta : w) * adv;
-                    const float second = (below ? a.low : above ? a.high : w) * adv;
-                    const float l = fmaf(p.beta, kl, -(second < first ? second : first));  // a NaN of either stays
-                    const bool cut_low = below && adv < 0.f, cut_high = above && adv > 0.f;
-                    const float slope = (cut_low || cut_high || capped) ? 0.f : -w * adv;
-                    sum[0] += row_w * (double)l;
-                    sum[1] += (double)kl;
-                    sum[2] += cut_low ? 1.0 : 0.0;
-                    sum[3] += cut_high ? 1.0 : 0.0;
-                    sum[4] += 1.0;
-                    if (!grad) continue;
-                    if (p.sequence_level)
-                        seq_slope += (double)slope;
-                    else
-                        grad[t] = (float)(row_w * ((double)slope + (double)kl_slope));
-                }
-        }
-    }
-    // totals of the workgroup, waves in order
+__device__ __forceinline__ void pl_count(PlShare& s, const PlTerm& k) {
+    s.loss += (double)k.loss;
+    s.kl += (double)k.kl;
+    s.low += k.cut_low ? 1 : 0;
+    s.high += k.cut_high ? 1 : 0;
+    s.valid += 1;
+}
+
+// Totals of the workgroup, waves in order; of the only workgroup: the results.
+template <int THREADS>
+__device__ __forceinline__ void pl_totals(const PlArgs& a, const PlShare& s, double* lds) {
+    double sum[PL_SUMS] = {s.total, s.kl, (double)s.low, (double)s.high, (double)s.valid};
 #pragma unroll
     for (int i = 0; i < PL_SUMS; ++i) {
 #pragma unroll
@@ -184,6 +142,148 @@ __global__ __launch_bounds__(THREADS) void policy_loss_kernel(PlArgs a) {
             for (int i = 0; i < PL_SUMS; ++i) a.partials[(int64_t)blockIdx.x * PL_SUMS + i] = sum[i];
         }
     }
+}
+
+// Rows of up to LANES * E tokens, LANES lanes a row, a lane's tokens in registers: every input is read once, and all
+// loads of a kind are under way together (masks first, then what they leave).
+template <int LANES, int E, int THREADS>
+__global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
+    __shared__ double lds[16 * PL_SUMS];
+    const grx_policy_loss_args& p = a.p;
+    constexpr int ROWS = THREADS / LANES;
+    const int lane = threadIdx.x % LANES;
+    PlShare share = {0.0, 0.0, 0.0, 0, 0, 0};
+    for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; r < p.R; r += (int64_t)gridDim.x * ROWS) {
+        bool valid[E];
+        float x[E], old[E], ref[E], adv[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int t = lane + e * LANES;
+            valid[e] = t < p.T && pl_valid(p, r, t);
+        }
+        const float row_adv = p.adv_pos_stride == 0 ? p.advantages[r * p.adv_row_stride] : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int t = lane + e * LANES;
+            x[e] = old[e] = ref[e] = 0.f;
+            adv[e] = row_adv;
+            if (valid[e]) {
+                x[e] = p.logps[r * p.logps_stride + t];
+                old[e] = p.old_logps ? p.old_logps[r * p.old_stride + t] : x[e];
+                if (p.ref_logps) ref[e] = p.ref_logps[r * p.ref_stride + t];
+                if (p.adv_pos_stride != 0) adv[e] = p.advantages[r * p.adv_row_stride + (int64_t)t * p.adv_pos_stride];
+            }
+        }
+        double row_w = 1.0, inv_n = 1.0, row_d = 0.0;
+        float seq_w = 1.f;
+        if (p.row_mean || p.sequence_level) {
+            double n = 0.0, d = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                n += valid[e] ? 1.0 : 0.0;
+                if (valid[e]) d += (double)x[e] - (double)old[e];
+            }
+            n = pl_row_sum<LANES>(n, lds);
+            inv_n = 1.0 / (n > 1.0 ? n : 1.0);
+            if (p.row_mean) row_w = inv_n;
+            if (p.sequence_level) {
+                row_d = pl_row_sum<LANES>(d, lds) * inv_n;
+                seq_w = expf((float)row_d);
+            }
+        }
+        double slope = 0.0;
+        float* grad = p.unit_grad ? p.unit_grad + r * p.T : nullptr;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (valid[e]) {
+                double d = row_d;
+                float w = seq_w;
+                if (!p.sequence_level) {
+                    d = (double)x[e] - (double)old[e];
+                    w = expf((float)d);
+                }
+                const PlTerm k = pl_term(a, d, w, adv[e], p.ref_logps != nullptr, (float)((double)ref[e] - (double)x[e]));
+                pl_count(share, k);
+                if (p.sequence_level) slope += (double)k.slope;
+                x[e] = k.slope;
+                old[e] = k.kl_slope;
+            }
+        }
+        share.total += row_w * share.loss;
+        share.loss = 0.0;
+        if (grad == nullptr) continue;
+        if (p.sequence_level) slope = pl_row_sum<LANES>(slope, lds) * inv_n;  // every token carries the row's slope
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int t = lane + e * LANES;
+            if (t < p.T)
+                grad[t] = valid[e] ? (float)(row_w * ((p.sequence_level ? slope : (double)x[e]) + (double)old[e])) : 0.f;
+        }
+    }
+    pl_totals<THREADS>(a, share, lds);
+}
+
+// Rows of any length, one workgroup a row, in passes over it.
+template <int LANES>
+__global__ __launch_bounds__(LANES) void policy_loss_kernel(PlArgs a) {
+    __shared__ double lds[16 * PL_SUMS];
+    const grx_policy_loss_args& p = a.p;
+    const int lane = threadIdx.x;
+    PlShare share = {0.0, 0.0, 0.0, 0, 0, 0};
+    for (int64_t r = blockIdx.x; r < p.R; r += gridDim.x) {
+        const float* lp = p.logps + r * p.logps_stride;
+        const float* old = p.old_logps ? p.old_logps + r * p.old_stride : nullptr;
+        const float* ref = p.ref_logps ? p.ref_logps + r * p.ref_stride : nullptr;
+        float* grad = p.unit_grad ? p.unit_grad + r * p.T : nullptr;
+        double row_w = 1.0, row_d = 0.0, inv_n = 1.0;
+        if (p.row_mean || p.sequence_level) {
+            double n = 0.0, d = 0.0;
+            for (int t = lane; t < p.T; t += LANES)
+                if (pl_valid(p, r, t)) {
+                    n += 1.0;
+                    if (p.sequence_level && old) d += (double)lp[t] - (double)old[t];
+                }
+            n = pl_row_sum<LANES>(n, lds);
+            inv_n = 1.0 / (n > 1.0 ? n : 1.0);
+            if (p.sequence_level) row_d = pl_row_sum<LANES>(d, lds) * inv_n;
+            if (p.row_mean) row_w = inv_n;
+        }
+        float seq_w = 1.f;
+        double seq_slope = 0.0;
+        if (p.sequence_level) seq_w = expf((float)row_d);
+        for (int pass = 0; pass < (p.sequence_level && grad ? 2 : 1); ++pass) {
+            // second pass (one ratio per sequence): every token of the row carries the row's slope
+            if (pass == 1) seq_slope = pl_row_sum<LANES>(seq_slope, lds) * inv_n;
+            for (int t = lane; t < p.T; t += LANES) {
+                if (!pl_valid(p, r, t)) {
+                    if (grad && pass == 0) grad[t] = 0.f;
+                    continue;
+                }
+                const float x = lp[t];
+                const float q = ref ? (float)((double)ref[t] - (double)x) : 0.f;
+                if (pass == 1) {
+                    grad[t] = (float)(row_w * (seq_slope + (ref ? (double)(-p.beta * (pl_kl(q) + q)) : 0.0)));
+                    continue;
+                }
+                double d = row_d;
+                float w = seq_w;
+                if (!p.sequence_level) {
+                    d = old ? (double)x - (double)old[t] : 0.0;
+                    w = expf((float)d);
+                }
+                const PlTerm k = pl_term(a, d, w, p.advantages[r * p.adv_row_stride + (int64_t)t * p.adv_pos_stride], ref, q);
+                pl_count(share, k);
+                if (!grad) continue;
+                if (p.sequence_level)
+                    seq_slope += (double)k.slope;
+                else
+                    grad[t] = (float)(row_w * ((double)k.slope + (double)k.kl_slope));
+            }
+        }
+        share.total += row_w * share.loss;
+        share.loss = 0.0;
+    }
+    pl_totals<LANES>(a, share, lds);
 }
 
 __global__ __launch_bounds__(PL_THREADS) void policy_loss_join_kernel(PlArgs a) {
@@ -228,7 +328,9 @@ __global__ __launch_bounds__(PL_THREADS) void policy_loss_grad_kernel(const floa
 }
 
 // ---- host ------------------------------------------------------------------------------------------
-static int pl_lanes(int T) { return T <= 8 ? 8 : T <= 2048 ? 64 : PL_BIG; }
+// Lanes per row; a lane's share of a row of up to 1024 tokens stays in registers (4096 rows of 1001 tokens, one ratio a
+// row: 64 lanes with 16 tokens each 45 us, for 174 registers leave two waves on a SIMD).
+static int pl_lanes(int T) { return T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : T <= 256 ? 64 : T <= 1024 ? PL_THREADS : PL_BIG; }
 
 static int pl_groups(int R, int T) {
     if ((int64_t)R * T <= PL_SINGLE_TOKENS) return 1;
@@ -282,15 +384,18 @@ extern "C" int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, 
                     "%s: scratch of %zu bytes, need %zu", who, scratch_bytes, need);
         a.partials = reinterpret_cast<double*>(scratch);
     }
-    if (lanes == PL_BIG) {
-        hipLaunchKernelGGL((policy_loss_kernel<PL_BIG, PL_BIG>), dim3(groups), dim3(PL_BIG), 0, stream, a);
-    } else if (groups == 1) {
-        if (lanes == 8) hipLaunchKernelGGL((policy_loss_kernel<8, PL_BIG>), dim3(1), dim3(PL_BIG), 0, stream, a);
-        else hipLaunchKernelGGL((policy_loss_kernel<64, PL_BIG>), dim3(1), dim3(PL_BIG), 0, stream, a);
-    } else {
-        if (lanes == 8) hipLaunchKernelGGL((policy_loss_kernel<8, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a);
-        else hipLaunchKernelGGL((policy_loss_kernel<64, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a);
-    }
+#define PL_LAUNCH(LANES, E)                                                                                          \
+    do {                                                                                                             \
+        if (groups == 1) hipLaunchKernelGGL((policy_loss_row_kernel<LANES, E, PL_BIG>), dim3(1), dim3(PL_BIG), 0, stream, a); \
+        else hipLaunchKernelGGL((policy_loss_row_kernel<LANES, E, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a); \
+    } while (0)
+    if (lanes == PL_BIG) hipLaunchKernelGGL((policy_loss_kernel<PL_BIG>), dim3(groups), dim3(PL_BIG), 0, stream, a);
+    else if (lanes == 8) PL_LAUNCH(8, 1);
+    else if (lanes == 16) PL_LAUNCH(16, 1);
+    else if (lanes == 32) PL_LAUNCH(32, 1);
+    else if (p.T <= 64) PL_LAUNCH(64, 1);
+    else if (p.T <= 256) PL_LAUNCH(64, 4);
+    else hipLaunchKernelGGL((policy_loss_row_kernel<PL_THREADS, 4, PL_THREADS>), dim3(groups), dim3(PL_THREADS), 0, stream, a);
     GRX_CHECK_HIP(hipGetLastError());
     if (groups > 1) {
         hipLaunchKernelGGL(policy_loss_join_kernel, dim3(1), dim3(PL_THREADS), 0, stream, a);

@@ -2,9 +2,11 @@
 // logits: what token_logps.hip computes from them.  Forward, the products of a 256 x BN tile are consumed where they
 // are: a row keeps (max, sum of exponentials, weighted sum) per 256 columns and its own token's logit.  Backward,
 // the product is formed again and turned into the logits' gradient G = dL/dlogits in bf16 -- the type autograd would
-// hold it in; half a step (2^-9) of each element, independent over the vocabulary -- in chunks of columns, and
+// hold it in -- in chunks of columns, and
 //   d hidden = G x weight (sum over v),    d weight = G^T x hidden (sum over rows)
-// follow with fp32 accumulators.  Four products of 2 N V H; bound by the matrix cores at many rows, by the weight
+// follow with fp32 accumulators.  What rounding takes from a row's largest element, the one at its token, is kept in
+// fp32 and added to both sums (as a multiple of the token's weight row, of the row's hidden state): without it it is
+// an error of up to 2^-8 of a whole row of either gradient.  Four products of 2 N V H; bound by the matrix cores at many rows, by the weight
 // (V H elements read per product, written once) at few.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -205,7 +207,10 @@ struct LlPrep {
     const float* h;
     float inv_t;
     LlRow* rows;               // one per row of the n tiles
-    char* copy;                // hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4]; null: not needed
+    int* tok;                  // [N] rows[].tok
+    float* rest;               // [N] cleared: what rounding G takes from the element at the token
+    char* copy;                // hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4]; null: no d weight
+    int* slot;                 // [V] cleared to -1, with copy
 };
 
 // Workgroup (64 rows, 32 h).  The copy holds 0 in the rows that do not count.
@@ -238,9 +243,16 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
                 o.tok = id < a.o.V ? (int)id : 0;
             }
             a.rows[r] = o;
+            if (r < a.o.N) {
+                a.tok[r] = o.tok;
+                a.rest[r] = 0.f;
+            }
         }
     }
-    if (a.copy == nullptr || r0 >= a.o.N) return;
+    if (a.copy == nullptr) return;
+    const int threads = gridDim.x * gridDim.y * 256;
+    for (int v = (blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.o.V; v += threads) a.slot[v] = -1;
+    if (r0 >= a.o.N) return;
     __syncthreads();
     const int lane = threadIdx.x & 63, n0 = (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -248,6 +260,120 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = live[n0 + j] ? a.o.hidden[(int64_t)(r0 + n0 + j) * a.o.hidden_ld + h] : (uint16_t)0;
     *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
+}
+
+// Rows that share a token: the first of them stands for all.  One workgroup per row looks through the tokens.
+struct LlGroup {
+    LlOperands o;
+    const int* tok;
+    const float* rest;
+    int* first;                // [N] first row with the same token, -1: no token
+    int* count;                // [N] rows with the same token
+    int* slot;                 // [V] a token's first row
+    float* sums;               // [N][H] in a first row: sum over the rows of its token of rest x hidden
+};
+
+__global__ __launch_bounds__(256) void lm_logps_group_kernel(LlGroup a) {
+    __shared__ int s_first[4], s_count[4];
+    const int r = blockIdx.x, t = a.tok[r];
+    int first = a.o.N, count = 0;
+    if (t >= 0)
+        for (int i = threadIdx.x; i < a.o.N; i += 256)
+            if (a.tok[i] == t) {
+                first = i < first ? i : first;
+                ++count;
+            }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const int f = __shfl_xor(first, o, 64);
+        first = f < first ? f : first;
+        count += __shfl_xor(count, o, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        s_first[threadIdx.x >> 6] = first;
+        s_count[threadIdx.x >> 6] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 4; ++w) {
+        first = s_first[w] < first ? s_first[w] : first;
+        count += s_count[w];
+    }
+    a.first[r] = t >= 0 ? first : -1;
+    a.count[r] = count;
+    if (t >= 0 && first == r) a.slot[t] = r;
+}
+
+// The sums of the tokens of one chunk.  Workgroup (rows blockIdx.x, + gridDim.x, ...; 256 h): the rows with the token
+// are listed 1024 at a time, in their order; eight groups of 32 lanes take every eighth of the list, a lane eight h.
+__global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_begin, int v_end) {
+    __shared__ float part[8][32][9];
+    __shared__ int list[1024], listed[4];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, wave = threadIdx.x >> 6;
+    const int h = blockIdx.y * 256 + lane * 8;
+    for (int r = blockIdx.x; r < a.o.N; r += gridDim.x) {
+        const int t = a.tok[r];
+        if (a.first[r] != r || t < v_begin || t >= v_end) continue;
+        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        int left = a.count[r];
+        for (int base = r; left > 0; base += 1024) {
+            int n = 1;
+            if (left == 1 && base == r) {  // the usual case: nobody else
+                __syncthreads();
+                if (threadIdx.x == 0) list[0] = r;
+            } else {
+                // thread i looks at rows base + 4 i .. + 3: lanes, then waves in order
+                int mine = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = base + (int)threadIdx.x * 4 + j;
+                    mine |= (i < a.o.N && a.tok[i] == t) ? 1 << j : 0;
+                }
+                const int have = __popc(mine);
+                int before = have;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int x = __shfl_up(before, o, 64);
+                    if ((threadIdx.x & 63) >= o) before += x;
+                }
+                __syncthreads();  // the list before has been read
+                if ((threadIdx.x & 63) == 63) listed[wave] = before;
+                __syncthreads();
+                int at = before - have;
+                n = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    if (w < wave) at += listed[w];
+                    n += listed[w];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (mine >> j & 1) list[at++] = base + (int)threadIdx.x * 4 + j;
+            }
+            __syncthreads();
+            if (h < a.o.H)
+#pragma unroll 4
+                for (int i = group; i < n; i += 8) {
+                    const int row = list[i];
+                    const float w = a.rest[row];
+                    float x[8];
+                    Elem<GRX_BF16>::unpack(*reinterpret_cast<const u32x4*>(a.o.hidden + (int64_t)row * a.o.hidden_ld + h), x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum[j] = fmaf(w, x[j], sum[j]);
+                }
+            left -= n;
+        }
+        __syncthreads();  // the parts of the row before have been read
+#pragma unroll
+        for (int j = 0; j < 8; ++j) part[group][lane][j] = sum[j];
+        __syncthreads();
+        if (group != 0 || h >= a.o.H) continue;
+        for (int g = 1; g < 8; ++g)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum[j] += part[g][lane][j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a.sums[(int64_t)r * a.o.H + h + j] = sum[j];
+    }
 }
 
 // G of a chunk of columns, in fragment blocks of 32 n x 16 v, [64 n][64 v][2][4]: a wave's results are such blocks
@@ -259,6 +385,7 @@ struct LlGrad {
     int n_pad;                 // rows of G
     float k;
     const LlRow* rows;
+    float* rest;
     char* out;
 };
 
@@ -306,7 +433,10 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
                 for (int m = 0; m < S::MA; ++m)
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
-                        if (m * 16 + e == at) acc[m][n][e] += row[n].at;
+                        if (m * 16 + e == at) {
+                            acc[m][n][e] += row[n].at;
+                            a.rest[n32 * 32 + (lane & 31)] = acc[m][n][e] - (float)(__bf16)acc[m][n][e];
+                        }
             }
             const bool dead = row[n].tok < 0;
             if (__any(dead)) {
@@ -383,14 +513,18 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     }
 }
 
-// Sum of the slabs in their order, rounded once.
-__global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(const float* slabs, int splits, int64_t n, int H,
-                                                                    const LlRow* rows, uint16_t* out) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// Sum of the slabs in their order and of what rounding took from G at the row's token, rounded once.
+__global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o, const float* slabs, int splits, const int* tok,
+                                                                    const float* rest, uint16_t* out) {
+    const int64_t n = (int64_t)o.N * o.H, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
+    const int r = (int)(i / o.H), h = (int)(i - (int64_t)r * o.H), t = tok[r];
     mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (rows[i / H].tok >= 0)
+    if (t >= 0) {
+        const mt_b16x4 w = *reinterpret_cast<const mt_b16x4*>(o.weight + (int64_t)t * o.weight_ld + h);
         for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const mt_f32x4*>(slabs + s * n + i);
+        v += rest[r] * __builtin_convertvector(w, mt_f32x4);
+    }
     *reinterpret_cast<mt_b16x4*>(out + i) = __builtin_convertvector(v, mt_b16x4);
 }
 
@@ -400,6 +534,8 @@ struct LlDw {
     const char* g;
     int H, V;
     int m_tiles, n_tiles, steps, v_begin, v64;
+    const int* slot;           // [V], sums [N][H]: what rounding took from G at the rows' tokens
+    const float* sums;
     uint16_t* out;             // [V][H]
 };
 
@@ -426,6 +562,12 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
     ll_dw_begin(pipe, a, blockIdx.x, h_next, c_next);
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int h0 = h_next, c0 = c_next;
+        int slot[S::NB];
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) {
+            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
+            slot[n] = v < a.V ? a.slot[v] : -1;
+        }
         LlDwPipe::Acc acc;
         pipe.run(acc);
         if (tile + (int)gridDim.x < tiles) ll_dw_begin(pipe, a, tile + gridDim.x, h_next, c_next);
@@ -433,6 +575,19 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
         for (int n = 0; n < S::NB; ++n) {
             const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
             uint16_t* const out = a.out + (int64_t)v * a.H;
+            if (slot[n] >= 0) {
+                const float* const sums = a.sums + (int64_t)slot[n] * a.H;
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
+                        if (h >= a.H) continue;
+                        const mt_f32x4 add = *reinterpret_cast<const mt_f32x4*>(sums + h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) acc[m][n][4 * q + j] += add[j];
+                    }
+            }
 #pragma unroll
             for (int m = 0; m < S::MA; ++m)
 #pragma unroll
@@ -497,7 +652,7 @@ struct LlBackward {
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
     int splits;
-    size_t rows, copy, g, slabs, total;
+    size_t rows, tok, rest, first, count, slot, sums, copy, g, slabs, total;
 };
 
 // Splits of d hidden's sum: as many as fill the CUs evenly, each at least eight steps long.
@@ -530,8 +685,20 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.bn = ll_bn(N, b.chunk / MT_BM);
     b.n_tiles = (N + b.bn - 1) / b.bn;
     b.splits = ll_splits((int64_t)b.h_tiles * b.dh_tiles, b.chunk / MT_BK);
-    b.rows = 0;
-    b.copy = (size_t)ll_up(ll_up(N, 256) * sizeof(LlRow), 256);  // tiles may reach past n_pad
+    size_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const size_t begin = at;
+        at += (size_t)ll_up(bytes, 256);
+        return begin;
+    };
+    b.rows = take(ll_up(N, 256) * sizeof(LlRow));  // tiles may reach past n_pad
+    b.tok = take((int64_t)N * 4);
+    b.rest = take((int64_t)N * 4);
+    b.first = take(want_w ? (int64_t)N * 4 : 0);
+    b.count = take(want_w ? (int64_t)N * 4 : 0);
+    b.slot = take(want_w ? (int64_t)V * 4 : 0);
+    b.sums = take(want_w ? (int64_t)N * H * 4 : 0);
+    b.copy = at;
     b.g = b.copy + (want_w ? (size_t)b.n_pad * H * 2 : 0);
     b.slabs = b.g + (size_t)(b.n_pad * b.chunk * 2);
     b.total = b.slabs + (want_h ? (size_t)b.splits * N * H * sizeof(float) : 0);
@@ -681,20 +848,30 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
     LlRow* rows = reinterpret_cast<LlRow*>(s + b.rows);
+    int* tok = reinterpret_cast<int*>(s + b.tok);
+    float* rest = reinterpret_cast<float*>(s + b.rest);
+    int* slot = reinterpret_cast<int*>(s + b.slot);
+    float* sums = reinterpret_cast<float*>(s + b.sums);
     char* copy = want_w ? s + b.copy : nullptr;
     char* g = s + b.g;
     float* slabs = reinterpret_cast<float*>(s + b.slabs);
     const LlOperands o = ll_operands(p);
 
     LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
-                 (float)(1.0 / (double)p->temperature), rows, copy};
+                 (float)(1.0 / (double)p->temperature), rows, tok, rest, copy, slot};
     hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(ll_up(p->N, 256) / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
                        stream, pr);
     GRX_CHECK_HIP(hipGetLastError());
+    const LlGroup gr = {o, tok, rest, reinterpret_cast<int*>(s + b.first), reinterpret_cast<int*>(s + b.count), slot, sums};
+    if (want_w) {
+        hipLaunchKernelGGL(lm_logps_group_kernel, dim3((unsigned)p->N), dim3(256), 0, stream, gr);
+        GRX_CHECK_HIP(hipGetLastError());
+    }
     for (int c = 0; c < b.n_chunks; ++c) {
         const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
-        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (int)b.n_pad, (float)(1.4426950408889634 / (double)p->temperature), rows, g};
+        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (int)b.n_pad, (float)(1.4426950408889634 / (double)p->temperature),
+                    rows, rest, g};
         LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * d.n_tiles), d);
         if (want_h) {
             const int steps = (int)(cols / MT_BK);
@@ -703,7 +880,10 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
             LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, b.splits * b.h_tiles * b.dh_tiles, x);
         }
         if (want_w) {
-            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64,
+            hipLaunchKernelGGL(lm_logps_rest_kernel, dim3((unsigned)(p->N < 1024 ? p->N : 1024), (unsigned)((p->H + 255) / 256)),
+                               dim3(256), 0, stream, gr, v0, (int)(v0 + cols));
+            GRX_CHECK_HIP(hipGetLastError());
+            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64, slot, sums,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
             LL_ONE(256, lm_logps_dweight_kernel, ll_resident(256, (int64_t)x.m_tiles * x.n_tiles), x);
         }
@@ -711,8 +891,8 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     if (want_h) {
         const int64_t n = (int64_t)p->N * p->H;
         GRX_REQUIRE(n / 1024 < (1 << 24), GRX_E_UNSUPPORTED, "%s: too many elements", who);
-        hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, slabs, b.splits,
-                           n, p->H, rows, reinterpret_cast<uint16_t*>(p->grad_hidden));
+        hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, o, slabs,
+                           b.splits, tok, rest, reinterpret_cast<uint16_t*>(p->grad_hidden));
         GRX_CHECK_HIP(hipGetLastError());
     }
     return GRX_OK;

@@ -121,6 +121,21 @@ def test_strided_operands_and_one_gradient_only():
         assert torch.equal(grads[0], dh if need[0] else dw)
 
 
+@pytest.mark.parametrize("N,tokens", [(1, 1), (7, 1), (300, 3), (2600, 2), (2600, 700)])
+def test_shared_tokens_and_the_size_of_the_error(N, tokens):
+    """Rows that share tokens (an end token is in every row), and how far the gradients are off as a whole: besides
+    their own rounding (half a step, uniform: at most 2^-8 and about 2^-8 / sqrt(3) of an element) only what bf16 takes
+    from the elements of G beside the tokens', which at a probability p of the token is below p of it."""
+    hidden, weight, ids, g, h = _inputs((N,), 256, 3000, seed=N + tokens, pad=0.1)
+    ids = torch.where(ids >= 0, ids % tokens * 17 % 3000, ids)
+    ids[0] = 0
+    lp, _, dh, dw = _check(hidden, weight, ids, g)
+    _, _, G, flat, wd, err, p, _ = _definition(hidden, weight, ids, 1.0, g, None)
+    for got, want in ((dh.double().reshape(N, -1), G @ wd), (dw.double(), G.T @ flat)):
+        own = (want.to(torch.bfloat16).double() - want).norm() / want.norm()
+        assert (got - want).norm() / want.norm() <= 1.25 * own + 1e-6
+
+
 def test_padding_may_hold_anything():
     hidden, weight, ids, g, h = _inputs((4, 20), 128, 900, seed=5, pad=0.4)
     g = torch.where(torch.rand(g.shape, device=g.device) < 0.2, torch.zeros_like(g), g)

@@ -56,6 +56,17 @@ __device__ __forceinline__ void ll_begin(LlLogits<BN>& pipe, const LlOperands& o
     pipe.begin(MtAlong<MT_BM, BN>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN, BN>(o.hidden, o.hidden_ld, o.N, r0, 0), o.H / MT_BK);
 }
 
+// Element `at` of a lane's row n: selected, where branches would make a jump table of stores.
+template <int MA, int NB>
+__device__ __forceinline__ float ll_pick(const mt_f32x16 (&acc)[MA][NB], int n, int at) {
+    float v = acc[0][n][0];
+#pragma unroll
+    for (int m = 0; m < MA; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v = m * 16 + e == at ? acc[m][n][e] : v;
+    return v;
+}
+
 // As many workgroups as run at a time; each takes every gridDim-th tile and starts the next one's copies before it
 // turns to its own results.  Those stay inside the wave: a row's sums over the wave's columns are one partial.
 template <int BN, bool ENT>
@@ -78,7 +89,10 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
             id[n] = r < a.o.N ? a.ids[r] : -1;
         }
         typename LlLogits<BN>::Acc acc;
-        pipe.run(acc);
+        pipe.clear(acc);
+        pipe.template run<S::NB>(acc, tile != (int)blockIdx.x);  // the stores of the tile before's sums
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(id[n]));  // waited for here, not behind the next copies
         if (tile + (int)gridDim.x < tiles) {
             mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
             ll_begin(pipe, a.o, (a.m_begin + tm) * MT_BM, tn * BN);
@@ -118,14 +132,10 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
                 a.partials[(int64_t)part * a.n_pad + r] = make_float2(mx, s);
                 if (ENT) a.weighted[(int64_t)part * a.n_pad + r] = u;
             }
-            const int64_t off = id[n] - vw;  // runs of four entries, every eight
-            if (off >= 0 && off < S::MA * 32 && (off & 4) == 0) {
-                const int at = (int)(off >> 5) * 16 + (int)((off & 31) >> 3) * 4 + (int)(off & 3);
-#pragma unroll
-                for (int m = 0; m < S::MA; ++m)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (m * 16 + e == at) a.chosen[r] = acc[m][n][e];
+            const int off = (int)(id[n] - vw);  // runs of four entries, every eight
+            if (id[n] >= vw && id[n] < vw + S::MA * 32 && (off & 4) == 0) {
+                const int at = (off >> 5) * 16 + ((off & 31) >> 3) * 4 + (off & 3);
+                a.chosen[r] = ll_pick<S::MA, S::NB>(acc, n, at);
             }
         }
     }
@@ -400,6 +410,8 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
     int tm, tn;
     mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
     ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
+    constexpr int STORES = S::MA * S::NB * 2;
+    bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int v0 = a.v_begin + tm * MT_BM, r0 = tn * BN;
         LlRow row[S::NB];
@@ -407,7 +419,12 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
         for (int n = 0; n < S::NB; ++n) row[n] = a.rows[r0 + (wn * S::NB + n) * 32 + (lane & 31)];
         const int v64 = tm * 4;
         typename LlLogits<BN>::Acc acc;
-        pipe.run(acc);
+        pipe.clear(acc);
+        pipe.template run<STORES>(acc, stored);
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n)  // waited for here, not behind the next copies
+            asm volatile("" : "+v"(row[n].m), "+v"(row[n].alpha), "+v"(row[n].beta), "+v"(row[n].at), "+v"(row[n].tok));
+        stored = r0 + (wn + 1) * S::NB * 32 <= a.n_pad;
         if (tile + (int)gridDim.x < tiles) {
             mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
             ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
@@ -432,11 +449,9 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
 #pragma unroll
                 for (int m = 0; m < S::MA; ++m)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        if (m * 16 + e == at) {
-                            acc[m][n][e] += row[n].at;
-                            a.rest[n32 * 32 + (lane & 31)] = acc[m][n][e] - (float)(__bf16)acc[m][n][e];
-                        }
+                    for (int e = 0; e < 16; ++e) acc[m][n][e] += m * 16 + e == at ? row[n].at : 0.f;
+                const float whole = ll_pick<S::MA, S::NB>(acc, n, at);
+                a.rest[n32 * 32 + (lane & 31)] = whole - (float)(__bf16)whole;
             }
             const bool dead = row[n].tok < 0;
             if (__any(dead)) {
@@ -471,7 +486,7 @@ struct LlDh {
     LlOperands o;
     const char* g;
     int m_tiles, n_tiles, splits, steps, steps_per, v_begin, v64, n_pad;
-    int add;                   // 1: add to what the chunk before left
+    int add;                   // 1: go on from what the chunk before left
     float* slabs;              // [splits][N][H]
 };
 
@@ -491,10 +506,23 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
                MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u, a.n_pad / 32 - r0 / 32),
                s1 - s0);
-    pipe.run(acc);
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
     float* slab = a.slabs + (int64_t)split * a.o.N * a.o.H;
+    pipe.clear(acc);
+    if (a.add) {
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) {
+            const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+            if (r >= a.o.N) continue;
+#pragma unroll
+            for (int m = 0; m < S::MA; ++m) {
+                const int h = h0 + (wm * S::MA + m) * 32;
+                if (h < a.o.H) pipe.load(acc, m, n, slab + (int64_t)r * a.o.H + h);
+            }
+        }
+    }
+    pipe.run(acc);
 #pragma unroll
     for (int n = 0; n < S::NB; ++n) {
         const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
@@ -506,9 +534,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
                 const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
                 if (h >= a.o.H) continue;
                 mt_f32x4* o = reinterpret_cast<mt_f32x4*>(slab + (int64_t)r * a.o.H + h);
-                mt_f32x4 v = {acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
-                if (a.add) v += *o;
-                *o = v;
+                *o = mt_f32x4{acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
             }
     }
 }
@@ -542,11 +568,15 @@ struct LlDw {
 typedef MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, LL_DW_BDEEP> LlDwPipe;
 
 // Eight v tiles at a time, one per XCD, all h tiles of each: G is read by one XCD.
-__device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int tile, int& h0, int& c0) {
-    const int group = tile / (8 * a.m_tiles), left = a.n_tiles - group * 8, wide = left < 8 ? left : 8;
+__device__ __forceinline__ void ll_dw_at(const LlDw& a, int tile, int& h0, int& c0) {
+    const int group = tile / (8 * a.m_tiles), left = a.n_tiles - group * 8, wide = left < 1 ? 1 : left < 8 ? left : 8;
     const int rest = tile - group * 8 * a.m_tiles;
     h0 = rest / wide * MT_BM;
     c0 = (group * 8 + rest % wide) * 256;
+}
+
+__device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int tile, int& h0, int& c0) {
+    ll_dw_at(a, tile, h0, c0);
     pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
                MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), a.steps);
 }
@@ -558,36 +588,46 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
     const int tiles = a.m_tiles * a.n_tiles;
     LlDwPipe pipe(lds);
-    int h_next, c_next;
+    int h_next, c_next, slot_next[S::NB];
+    const auto find = [&](int tile) {  // a tile ahead, so that nobody waits for it
+        int h0, c0;
+        ll_dw_at(a, tile, h0, c0);
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) {
+            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
+            slot_next[n] = tile < tiles && v < a.V ? a.slot[v] : -1;
+        }
+    };
     ll_dw_begin(pipe, a, blockIdx.x, h_next, c_next);
+    find(blockIdx.x);
+    constexpr int STORES = S::MA * S::NB * 2;
+    bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int h0 = h_next, c0 = c_next;
         int slot[S::NB];
 #pragma unroll
-        for (int n = 0; n < S::NB; ++n) {
-            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
-            slot[n] = v < a.V ? a.slot[v] : -1;
-        }
+        for (int n = 0; n < S::NB; ++n) slot[n] = slot_next[n];
         LlDwPipe::Acc acc;
-        pipe.run(acc);
+        pipe.clear(acc);
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n)
+            if (__any(slot[n] >= 0)) {  // the sum goes on from what rounding took from G
+                const float* const sums = a.sums + (int64_t)slot[n] * a.H;
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m) {
+                    const int h = h0 + (wm * S::MA + m) * 32;
+                    if (slot[n] >= 0 && h < a.H) pipe.load(acc, m, n, sums + h);
+                    asm volatile("" : "+v"(acc[m][n]));  // waited for here, and not by the waves without a token
+                }
+            }
+        find(tile + gridDim.x);
+        pipe.run<STORES>(acc, stored);
+        stored = a.v_begin + c0 + (wn + 1) * S::NB * 32 <= a.V && h0 + (wm + 1) * S::MA * 32 <= a.H;
         if (tile + (int)gridDim.x < tiles) ll_dw_begin(pipe, a, tile + gridDim.x, h_next, c_next);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
             uint16_t* const out = a.out + (int64_t)v * a.H;
-            if (slot[n] >= 0) {
-                const float* const sums = a.sums + (int64_t)slot[n] * a.H;
-#pragma unroll
-                for (int m = 0; m < S::MA; ++m)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
-                        if (h >= a.H) continue;
-                        const mt_f32x4 add = *reinterpret_cast<const mt_f32x4*>(sums + h);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[m][n][4 * q + j] += add[j];
-                    }
-            }
 #pragma unroll
             for (int m = 0; m < S::MA; ++m)
 #pragma unroll

@@ -51,10 +51,10 @@ __device__ __forceinline__ int mt_wave() { return __builtin_amdgcn_readfirstlane
 // what has to be waited for is written out (mt_meet).  The compiler's own counts of loads under way come out too low
 // beside them, which only makes its waits longer; M0 holds nothing of its own on this target.
 __device__ __forceinline__ void mt_copy(const char* base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory");
 }
 __device__ __forceinline__ void mt_copy_from(const char* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
 }
 
 // ---- stages.  N: copies per wave and step (1 KB each); issue(i, to): the i-th of them into the buffer at
@@ -236,7 +236,8 @@ __device__ __forceinline__ void mt_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(VM) : "memory");
 }
 
-// begin() starts the first copies of a tile (the LDS must be free), run() multiplies and leaves the LDS free: the next
+// begin() starts the first copies of a tile (the LDS must be free), run() adds the products to acc and leaves the LDS
+// free: the next
 // tile's begin() may come before this one's results are used, so that its copies travel meanwhile.
 //
 // One meeting of the waves per step, in front of its last quarter: by then every wave holds that quarter's fragments
@@ -277,19 +278,35 @@ struct MtPipe {
             }
         }
     }
-    __device__ __forceinline__ void run(Acc& acc) {
+    static __device__ __forceinline__ void clear(Acc& acc) {
 #pragma unroll
         for (int m = 0; m < S::MA; ++m)
 #pragma unroll
             for (int n = 0; n < S::NB; ++n)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.f;
+    }
+    // The 32 elements of block m of a lane's row n from memory (p: the row at the block), as they lie in acc.
+    static __device__ __forceinline__ void load(Acc& acc, int m, int n, const float* p) {
+        const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const mt_f32x4 v = *reinterpret_cast<const mt_f32x4*>(p + 8 * q + 4 * half);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[m][n][4 * q + j] = v[j];
+        }
+    }
+    // stores: at least LATER vector memory instructions of this wave came behind begin()'s copies (stores of the tile
+    // before); they need not have ended.  Memory instructions of a wave end in their order on this target.
+    template <int LATER = 0>
+    __device__ __forceinline__ void run(Acc& acc, bool stores = false) {
         if (nk <= 0) return;
         const int wave = mt_wave();
         const ReadA ra(wave / S::WN * S::MA * 32);
         const ReadB rb(wave % S::WN * S::NB * 32);
         constexpr int AHEAD = (AR - 2) * StageA::N + (BR - 2) * StageB::N;  // copies that may stay under way
-        mt_meet<0>();
+        if (LATER > 0 && stores) mt_meet<LATER>();
+        else mt_meet<0>();
         uint32_t ca = la, cb = lb;  // the present step's buffers
         mt_s16x8 fa[2][S::MA], fb[2][S::NB];
 #pragma unroll

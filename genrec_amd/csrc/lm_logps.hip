@@ -19,15 +19,7 @@
 
 #define LL_FLOOR (-200.f)           // 2^-200 is 0 in fp32: keeps 0 * -inf out of the entropy sums
 #define LL_CUS 256
-#ifndef LL_DW_BDEEP
-#define LL_DW_BDEEP true
-#endif
-#ifndef LL_DH_BDEEP
-#define LL_DH_BDEEP false
-#endif
-#ifndef LL_CHUNK_BYTES
 #define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk
-#endif
 
 struct LlOperands {
     const uint16_t* weight;     // [V, H]
@@ -501,7 +493,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     const int tn = rest % a.n_tiles, split = rest / a.n_tiles;
     const int h0 = tm * MT_BM, r0 = tn * BN;
     const int s0 = split * a.steps_per, s1 = s0 + a.steps_per < a.steps ? s0 + a.steps_per : a.steps;
-    MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong, LL_DH_BDEEP && BN == 256> pipe(lds);
+    MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong> pipe(lds);
     typename decltype(pipe)::Acc acc;
     pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
                MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u, a.n_pad / 32 - r0 / 32),
@@ -565,7 +557,13 @@ struct LlDw {
     uint16_t* out;             // [V][H]
 };
 
-typedef MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, LL_DW_BDEEP> LlDwPipe;
+// LINES: two buffers of either operand, and the LDS left holds the results on their way to whole lines of 128 bytes;
+// otherwise three buffers of G and stores of the 16 bytes that a lane holds.  Up to LL_LINES_STEPS steps the stores weigh
+// more: at H = 2048 and V = 152,640 (625 MB to write) 64 rows take 155 us against 208, 512 rows 419 against 464, 1024 rows
+// 675 against 677, 2048 rows 1221 against 1177, 4096 rows 2280 against 2176.
+#define LL_LINES_STEPS 16
+template <bool LINES>
+using LlDwPipe = MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, !LINES, LINES ? 2 : 3>;
 
 // Eight v tiles at a time, one per XCD, all h tiles of each: G is read by one XCD.
 __device__ __forceinline__ void ll_dw_at(const LlDw& a, int tile, int& h0, int& c0) {
@@ -575,19 +573,23 @@ __device__ __forceinline__ void ll_dw_at(const LlDw& a, int tile, int& h0, int& 
     c0 = (group * 8 + rest % wide) * 256;
 }
 
-__device__ __forceinline__ void ll_dw_begin(LlDwPipe& pipe, const LlDw& a, int tile, int& h0, int& c0) {
+template <bool LINES>
+__device__ __forceinline__ void ll_dw_begin(LlDwPipe<LINES>& pipe, const LlDw& a, int tile, int& h0, int& c0) {
     ll_dw_at(a, tile, h0, c0);
     pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
                MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), a.steps);
 }
 
+template <bool LINES>
 __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel(LlDw a) {
     typedef MtShape<256> S;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
-    const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    const int wm = wave / S::WN, wn = wave % S::WN;
     const int tiles = a.m_tiles * a.n_tiles;
-    LlDwPipe pipe(lds);
+    LlDwPipe<LINES> pipe(lds);
+    // LINES: behind the 128 KB of the pipe, 4 KB of each wave
+    const uint32_t staging = (uint32_t)(uintptr_t)(mt_lds_void*)lds + 4 * MT_BM * MT_BK * 2 + wave * 4096;
     int h_next, c_next, slot_next[S::NB];
     const auto find = [&](int tile) {  // a tile ahead, so that nobody waits for it
         int h0, c0;
@@ -598,7 +600,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
             slot_next[n] = tile < tiles && v < a.V ? a.slot[v] : -1;
         }
     };
-    ll_dw_begin(pipe, a, blockIdx.x, h_next, c_next);
+    ll_dw_begin<LINES>(pipe, a, blockIdx.x, h_next, c_next);
     find(blockIdx.x);
     constexpr int STORES = S::MA * S::NB * 2;
     bool stored = false;  // all STORES of the tile before were made
@@ -607,7 +609,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
         int slot[S::NB];
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) slot[n] = slot_next[n];
-        LlDwPipe::Acc acc;
+        typename LlDwPipe<LINES>::Acc acc;
         pipe.clear(acc);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n)
@@ -621,24 +623,20 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
                 }
             }
         find(tile + gridDim.x);
-        pipe.run<STORES>(acc, stored);
+        pipe.template run<STORES>(acc, stored);
         stored = a.v_begin + c0 + (wn + 1) * S::NB * 32 <= a.V && h0 + (wm + 1) * S::MA * 32 <= a.H;
-        if (tile + (int)gridDim.x < tiles) ll_dw_begin(pipe, a, tile + gridDim.x, h_next, c_next);
+        if (tile + (int)gridDim.x < tiles) ll_dw_begin<LINES>(pipe, a, tile + gridDim.x, h_next, c_next);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
-            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
+            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32;
             uint16_t* const out = a.out + (int64_t)v * a.H;
 #pragma unroll
-            for (int m = 0; m < S::MA; ++m)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const mt_f32x16& c = acc[m][n];
-                    const mt_f32x4 x = {c[8 * q], c[8 * q + 1], c[8 * q + 2], c[8 * q + 3]};
-                    const mt_f32x4 y = {c[8 * q + 4], c[8 * q + 5], c[8 * q + 6], c[8 * q + 7]};
-                    const mt_u32x4 packed = mt_pack8(x, y);
-                    const int h = h0 + (wm * S::MA + m) * 32 + 16 * q + 8 * half;
-                    if (v < a.V && h < a.H) *reinterpret_cast<mt_u32x4*>(out + h) = packed;
-                }
+            for (int m = 0; m < S::MA; m += 2) {
+                const int h = h0 + (wm * S::MA + m) * 32;
+                if (h >= a.H) continue;
+                if constexpr (LINES) mt_store_rows(acc[m][n], acc[m + 1][n], staging, out + h, a.H, a.V - v);
+                else if (v + (lane & 31) < a.V) mt_store_lanes(acc[m][n], acc[m + 1][n], out + (int64_t)(lane & 31) * a.H + h);
+            }
         }
     }
 }
@@ -646,15 +644,15 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
 // ---- host ------------------------------------------------------------------------------------------
 static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
-// Rows per tile of the products with the logits' shape (m_tiles x n tiles of 256 x BN).  A tile of 64 rows costs about
-// 0.37 of one of 256, one of 128 0.64 (measured per round of 256 tiles at H = 2048: 24, 40 and 64 us; two workgroups of
-// 64 rows share a CU); what counts is whole rounds over the CUs.
+// Rows per tile of the products with the logits' shape (m_tiles x n tiles of 256 x BN): what counts is whole rounds over
+// the CUs.  At H = 2048 a round takes 52 to 56 us with tiles of 256 rows, 33 to 37 with 128, 41 with 64 (two to a CU):
+// 320 rows at V = 152,640 take 240 us in 7 rounds of 128 and 267 in 5 of 256, 400 rows 309 in 10 and 270 in 5.
 static int ll_bn(int N, int64_t m_tiles) {
     int best = 0;
     double least = 0.0;
     for (int bn = 64; bn <= 256; bn *= 2) {
         const int64_t tiles = m_tiles * ((N + bn - 1) / bn), wgs = bn == 64 ? 2 * LL_CUS : LL_CUS;
-        const double cost = (double)((tiles + wgs - 1) / wgs) * (bn == 64 ? 0.74 : bn == 128 ? 0.64 : 1.0);
+        const double cost = (double)((tiles + wgs - 1) / wgs) * (bn == 64 ? 0.8 : bn == 128 ? 0.64 : 1.0);
         if (best == 0 || cost <= least) {
             best = bn;
             least = cost;
@@ -925,7 +923,9 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
             GRX_CHECK_HIP(hipGetLastError());
             LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64, slot, sums,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
-            LL_ONE(256, lm_logps_dweight_kernel, ll_resident(256, (int64_t)x.m_tiles * x.n_tiles), x);
+            const int64_t wgs = ll_resident(256, (int64_t)x.m_tiles * x.n_tiles);
+            if (x.steps <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
+            else LL_ONE(256, lm_logps_dweight_kernel<false>, wgs, x);
         }
     }
     if (want_h) {

@@ -245,10 +245,10 @@ __device__ __forceinline__ void mt_meet() {
 // for one or two steps, have landed -- its first fragments are read between the products of the last quarter.
 // Every LDS read goes out a quarter before its product, early in it, and the copies of a step are spread over two
 // quarters, one behind a product: nothing in the loop waits for what was issued right before.
-template <int BN, class StageA, class ReadA, class StageB, class ReadB, bool B_DEEP = false>
+template <int BN, class StageA, class ReadA, class StageB, class ReadB, bool B_DEEP = false, int DEEP = MtShape<BN>::DEEP>
 struct MtPipe {
     typedef MtShape<BN> S;
-    static constexpr int AR = B_DEEP ? S::FLAT : S::DEEP, BR = B_DEEP ? S::DEEP : S::FLAT;
+    static constexpr int AR = B_DEEP ? S::FLAT : DEEP, BR = B_DEEP ? DEEP : S::FLAT;
     typedef mt_f32x16 Acc[S::MA][S::NB];
     static constexpr int A_BYTES = MT_BM * MT_BK * 2, B_BYTES = BN * MT_BK * 2;
     StageA sa;
@@ -265,7 +265,7 @@ struct MtPipe {
         sb = b;
         nk = steps;
 #pragma unroll
-        for (int t = 0; t < S::DEEP; ++t) {
+        for (int t = 0; t < DEEP; ++t) {
             if (t < BR && t < nk) {
 #pragma unroll
                 for (int i = 0; i < StageB::N; ++i) sb.issue_any(i, lb + t * B_BYTES);
@@ -402,11 +402,11 @@ struct MtPipe {
         };
         // whole steps of either operand, as seen behind the copies of begin()
         const int wa = sa.whole_steps(nk - AR) + AR, wb = sb.whole_steps(nk - BR) + BR;
-        const int wd = (B_DEEP ? wb : wa) - S::DEEP + 1, wf = (B_DEEP ? wa : wb) - S::FLAT;
+        const int wd = (B_DEEP ? wb : wa) - DEEP + 1, wf = (B_DEEP ? wa : wb) - S::FLAT;
         const int safe = wd < wf ? wd : wf;
         step(std::false_type(), false);
         for (kt = 1; kt < safe; ++kt) step(std::true_type(), true);
-        for (; kt < nk; ++kt) step(std::false_type(), kt - 1 + S::DEEP < nk);
+        for (; kt < nk; ++kt) step(std::false_type(), kt - 1 + DEEP < nk);
         mt_meet<0>();
     }
 };
@@ -436,4 +436,37 @@ __device__ __forceinline__ mt_u32x4 mt_pack8(mt_f32x4 x, mt_f32x4 y) {
     const auto p = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
     const auto q = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
     return mt_u32x4{p[0], q[0], p[1], q[1]};
+}
+
+// Two blocks of results (m rows of 32 and the next 32, 32 n) rounded to bf16 and stored as 32 rows n of 64 m.
+// Through 4 KB of LDS that belong to this wave (at `lds`, a byte address), in whole lines of 128 bytes.  out: the first
+// row's first element; row r is written if r < rows.
+__device__ __forceinline__ void mt_store_rows(const mt_f32x16& c0, const mt_f32x16& c1, uint32_t lds, uint16_t* out, int64_t ld, int rows) {
+    typedef __attribute__((address_space(3))) mt_u32x4 lds_u32x4;
+    const int lane = threadIdx.x & 63, row = lane & 31;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const mt_f32x16& c = k < 2 ? c0 : c1;
+        const int q = 8 * (k & 1), chunk = k * 2 + (lane >> 5);
+        const mt_f32x4 x = {c[q], c[q + 1], c[q + 2], c[q + 3]}, y = {c[q + 4], c[q + 5], c[q + 6], c[q + 7]};
+        *(lds_u32x4*)(uintptr_t)(lds + row * 128 + ((chunk ^ (row & 7)) << 4)) = mt_pack8(x, y);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 3), chunk = lane & 7;
+        const mt_u32x4 v = *(lds_u32x4*)(uintptr_t)(lds + r * 128 + ((chunk ^ (r & 7)) << 4));
+        if (r < rows) __builtin_nontemporal_store(v, reinterpret_cast<mt_u32x4*>(out + r * ld + chunk * 8));
+    }
+}
+
+// The same from the registers, 16 bytes a lane.  out: the first element of this lane's row.
+__device__ __forceinline__ void mt_store_lanes(const mt_f32x16& c0, const mt_f32x16& c1, uint16_t* out) {
+    const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const mt_f32x16& c = k < 2 ? c0 : c1;
+        const int q = 8 * (k & 1);
+        const mt_f32x4 x = {c[q], c[q + 1], c[q + 2], c[q + 3]}, y = {c[q + 4], c[q + 5], c[q + 6], c[q + 7]};
+        *reinterpret_cast<mt_u32x4*>(out + 16 * k + 8 * half) = mt_pack8(x, y);
+    }
 }

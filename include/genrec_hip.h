@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define GRX_ABI_VERSION 16
+#define GRX_ABI_VERSION 15
 
 #if defined(GRX_BUILDING)
 #define GRX_API __attribute__((visibility("default")))

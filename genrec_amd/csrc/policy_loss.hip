@@ -40,8 +40,8 @@ __device__ __forceinline__ bool pl_valid(const grx_policy_loss_args& p, int64_t 
 }
 
 // exp(q) - 1 - q without the cancellation near 0: its Taylor series (the first term left out is below 2^-26 of the
-// sum for |q| < 1), the difference itself elsewhere.  With q added it is exp(q) - 1.
-__device__ __forceinline__ float pl_kl(float q) {
+// sum for |q| < 1), the difference itself elsewhere.  rise: exp(q) - 1, which stays finite where q = -inf.
+__device__ __forceinline__ float pl_kl(float q, float& rise) {
     if (fabsf(q) < 1.f) {
         float s = 1.f / 39916800.f;
         s = fmaf(s, q, 1.f / 3628800.f);
@@ -53,9 +53,12 @@ __device__ __forceinline__ float pl_kl(float q) {
         s = fmaf(s, q, 1.f / 24.f);
         s = fmaf(s, q, 1.f / 6.f);
         s = fmaf(s, q, 0.5f);
-        return s * q * q;
+        const float kl = s * q * q;
+        rise = kl + q;
+        return kl;
     }
-    return expf(q) - 1.f - q;
+    rise = expf(q) - 1.f;
+    return rise - q;
 }
 
 // Sum over the LANES lanes that share a row; every lane gets it.  LANES > 64: a whole workgroup.
@@ -88,12 +91,14 @@ struct PlShare {
 // One token: d = log ratio in 64 bits, w = exp(d); q = ref - logp where there is a reference.
 __device__ __forceinline__ PlTerm pl_term(const PlArgs& a, double d, float w, float adv, bool ref, float q) {
     PlTerm r;
-    r.kl = ref ? pl_kl(q) : 0.f;
-    r.kl_slope = ref ? -a.p.beta * (r.kl + q) : 0.f;
+    float rise = 0.f;
+    r.kl = ref ? pl_kl(q, rise) : 0.f;
+    r.kl_slope = a.p.beta != 0.f ? -a.p.beta * rise : 0.f;  // without beta an infinite KL is reported and not added
     const bool below = d < a.log_low, above = d > a.log_high, capped = d > a.log_delta;
     const float first = (capped ? a.delta : w) * adv;
     const float second = (below ? a.low : above ? a.high : w) * adv;
-    r.loss = fmaf(a.p.beta, r.kl, -(second < first ? second : first));  // a NaN of either stays
+    const float least = second < first ? second : first;  // a NaN of either stays
+    r.loss = a.p.beta != 0.f ? fmaf(a.p.beta, r.kl, -least) : -least;
     r.cut_low = below && adv < 0.f;
     r.cut_high = above && adv > 0.f;
     r.slope = (r.cut_low || r.cut_high || capped) ? 0.f : -w * adv;
@@ -262,7 +267,9 @@ __global__ __launch_bounds__(LANES) void policy_loss_kernel(PlArgs a) {
                 const float x = lp[t];
                 const float q = ref ? (float)((double)ref[t] - (double)x) : 0.f;
                 if (pass == 1) {
-                    grad[t] = (float)(row_w * (seq_slope + (ref ? (double)(-p.beta * (pl_kl(q) + q)) : 0.0)));
+                    float rise = 0.f;
+                    if (p.beta != 0.f) pl_kl(q, rise);
+                    grad[t] = (float)(row_w * (seq_slope + (double)(-p.beta * rise)));
                     continue;
                 }
                 double d = row_d;
@@ -354,6 +361,7 @@ extern "C" int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, 
     a.p = *args;
     const grx_policy_loss_args& p = a.p;
     GRX_REQUIRE(p.R >= 0 && p.T >= 0, GRX_E_INVALID, "%s: bad shape", who);
+    GRX_REQUIRE(p.T <= (1 << 30), GRX_E_UNSUPPORTED, "%s: more than 2^30 positions", who);  // positions are stepped over as int
     GRX_REQUIRE(p.loss != nullptr && p.stats != nullptr, GRX_E_INVALID, "%s: null output", who);
     const bool any = (int64_t)p.R * p.T > 0;
     GRX_REQUIRE(!any || (p.logps != nullptr && p.advantages != nullptr && p.mask != nullptr), GRX_E_INVALID,
@@ -374,6 +382,7 @@ extern "C" int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, 
     a.low = (float)(1.0 - p.epsilon_low);
     a.high = (float)(1.0 + p.epsilon_high);
     a.constant = p.row_mean ? 1.0 / (double)(p.R > 0 ? p.R : 1) : p.normalizer > 0.0 ? 1.0 / p.normalizer : 0.0;
+    if (!any) a.p.R = 0;  // rows without positions: nothing is read, their advantages neither
     hipStream_t stream = (hipStream_t)stream_;
     const int lanes = pl_lanes(p.T);
     const int groups = any ? pl_groups(p.R, p.T) : 1;

@@ -308,7 +308,7 @@ py::tuple policy_loss(const Tensor& logps_, const Tensor& advantages, const Tens
     const at::Device device = logps_.device();
     TORCH_CHECK_VALUE(logps_.dim() == 2, "logps must be [rows, positions], got ", logps_.sizes());
     const int64_t R = logps_.size(0), T = logps_.size(1);
-    TORCH_CHECK_VALUE(R < 1ll << 31 && T < 1ll << 31, "rows and positions must stay below 2^31");
+    TORCH_CHECK_VALUE(R < 1ll << 31 && T <= 1ll << 30, "at most 2^31 - 1 rows and 2^30 positions, got ", logps_.sizes());
     const auto shaped = [&](const Tensor& t, const char* name) {
         TORCH_CHECK_VALUE(t.sizes() == logps_.sizes(), name, " must have the shape of logps ", logps_.sizes(), ", got ", t.sizes());
     };

@@ -787,6 +787,7 @@ GRX_API int grx_lm_token_logps_backward(const grx_lm_token_logps_args* args, voi
  * A < 0) and upper bound (w above, A > 0), and a factor; unit_grad (fp32 [R, T] contiguous, 16-byte
  * aligned, or null): grx_policy_loss_backward multiplies it by stats[3] and by the device scalar
  * `upstream` (dL/dloss) into grad_logps [R * T].
+ * T <= 2^30.
  * scratch: grx_policy_loss_scratch_bytes(R, T) bytes (0 for small calls), 8-byte aligned, contents
  * need no initialisation; calls that may overlap must not share it.
  */

@@ -360,6 +360,44 @@ def test_bounds_and_extreme_ratios():
     assert float(res.loss) == pytest.approx(-1.2, abs=1e-6) and float(x.grad) == 0.0
 
 
+def test_rows_without_positions_read_nothing():
+    """An expanded view without elements has no memory behind it."""
+    dev = torch.device("cuda", 0)
+    x = torch.zeros((6, 0), device=dev, requires_grad=True)
+    adv = torch.ones((6, 1), device=dev).expand(6, 4)[:, :0]
+    assert adv.data_ptr() == 0 or adv.stride(1) == 0
+    for kind in ("grpo", "bnpo"):
+        res = policy_loss(x, adv, torch.ones((6, 0), device=dev), loss_type=kind)
+        (g,) = torch.autograd.grad(res.loss, x)
+        assert float(res.loss) == 0.0 and float(res.kl) == 0.0 and g.shape == (6, 0)
+
+
+@pytest.mark.parametrize("T", [5, 200, 1500])
+@pytest.mark.parametrize("level", ["token", "sequence"])
+def test_reference_that_rules_a_token_out(T, level):
+    """exp(q) - 1 - q with q = -inf: the KL is infinite, its slope is 1; without beta it does not reach the loss."""
+    logps, adv, mask, old, ref = _loss_inputs(4, T, seed=21)
+    mask = torch.ones_like(mask)
+    clean, _ = _check_loss(logps, adv, mask, old, ref, level=level)
+    _, want = _check_loss(logps, adv, mask, old, ref, level=level, beta=0.1)
+    ref[2, 3] = -math.inf
+    x = logps.clone().requires_grad_()
+    res = policy_loss(x, adv, mask, old, ref, importance_sampling_level=level)
+    (g,) = torch.autograd.grad(res.loss, x)
+    assert torch.equal(res.loss, clean.loss) and torch.isinf(res.kl) and torch.isfinite(g).all()
+    x = logps.clone().requires_grad_()
+    res = policy_loss(x, adv, mask, old, ref, importance_sampling_level=level, beta=0.1)
+    (g,) = torch.autograd.grad(res.loss, x)
+    d = _loss_definition(logps, adv, mask, old, ref, level=level, beta=0.1)
+    assert torch.isinf(res.loss) and float(res.loss) > 0
+    keep = torch.ones_like(mask, dtype=torch.bool)
+    keep[2, 3] = False
+    assert torch.equal(g[keep], want[keep])
+    # the formula's: 24 u of |w A| + beta, per the bound of the checks above (sequence: the row's sum)
+    size = (d["grad"].abs().max() + 1.0) * 64 * U
+    assert abs(float(g[2, 3]) - float(d["grad"][2, 3])) <= float(size)
+
+
 def test_results_do_not_change_from_call_to_call():
     logits, ids = _case((40, 7), 5003, torch.bfloat16, seed=12)
     logps, adv, mask, old, ref = _loss_inputs(700, 90, seed=13)

@@ -105,6 +105,7 @@ def test_token_logps_c_entries_refuse_what_only_one_direction_needs():
 
 @pytest.mark.parametrize("over,code,match", [
     (dict(R=-1), -1, b"bad shape"),
+    (dict(T=(1 << 30) + 1), -3, b"positions"),
     (dict(loss=None), -1, b"null output"),
     (dict(mask=None), -1, b"null input"),
     (dict(mask_type=4), -1, b"mask type"),

@@ -213,6 +213,7 @@ struct LlPrep {
     float* rest;               // [N] cleared: what rounding G takes from the element at the token
     char* copy;                // hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4]; null: no d weight
     int* slot;                 // [V] cleared to -1, with copy
+    int* count;                // [V] cleared to 0, with copy
 };
 
 // Workgroup (64 rows, 32 h).  The copy holds 0 in the rows that do not count.
@@ -252,8 +253,11 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
         }
     }
     if (a.copy == nullptr) return;
-    const int threads = gridDim.x * gridDim.y * 256;
-    for (int v = (blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.o.V; v += threads) a.slot[v] = -1;
+    for (int64_t v = ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.o.V;
+         v += (int64_t)gridDim.x * gridDim.y * 256) {
+        a.slot[v] = -1;
+        a.count[v] = 0;
+    }
     if (r0 >= a.o.N) return;
     __syncthreads();
     const int lane = threadIdx.x & 63, n0 = (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
@@ -264,46 +268,21 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
     *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
-// Rows that share a token: the first of them stands for all.  One workgroup per row looks through the tokens.
+// Rows that share a token: the first of them stands for all.
 struct LlGroup {
     LlOperands o;
     const int* tok;
     const float* rest;
-    int* first;                // [N] first row with the same token, -1: no token
-    int* count;                // [N] rows with the same token
-    int* slot;                 // [V] a token's first row
+    int* slot;                 // [V] N - 1 - the token's first row, -1: no row
+    int* count;                // [V] rows with the token
     float* sums;               // [N][H] in a first row: sum over the rows of its token of rest x hidden
 };
 
 __global__ __launch_bounds__(256) void lm_logps_group_kernel(LlGroup a) {
-    __shared__ int s_first[4], s_count[4];
-    const int r = blockIdx.x, t = a.tok[r];
-    int first = a.o.N, count = 0;
-    if (t >= 0)
-        for (int i = threadIdx.x; i < a.o.N; i += 256)
-            if (a.tok[i] == t) {
-                first = i < first ? i : first;
-                ++count;
-            }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const int f = __shfl_xor(first, o, 64);
-        first = f < first ? f : first;
-        count += __shfl_xor(count, o, 64);
-    }
-    if ((threadIdx.x & 63) == 0) {
-        s_first[threadIdx.x >> 6] = first;
-        s_count[threadIdx.x >> 6] = count;
-    }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int w = 1; w < 4; ++w) {
-        first = s_first[w] < first ? s_first[w] : first;
-        count += s_count[w];
-    }
-    a.first[r] = t >= 0 ? first : -1;
-    a.count[r] = count;
-    if (t >= 0 && first == r) a.slot[t] = r;
+    const int r = blockIdx.x * 256 + threadIdx.x, t = r < a.o.N ? a.tok[r] : -1;
+    if (t < 0) return;
+    atomicMax(a.slot + t, a.o.N - 1 - r);  // whole numbers: any order gives the same
+    atomicAdd(a.count + t, 1);
 }
 
 // The sums of the tokens of one chunk.  Workgroup (rows blockIdx.x, + gridDim.x, ...; 256 h): the rows with the token
@@ -315,9 +294,9 @@ __global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_beg
     const int h = blockIdx.y * 256 + lane * 8;
     for (int r = blockIdx.x; r < a.o.N; r += gridDim.x) {
         const int t = a.tok[r];
-        if (a.first[r] != r || t < v_begin || t >= v_end) continue;
+        if (t < v_begin || t >= v_end || a.slot[t] != a.o.N - 1 - r) continue;
         float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        int left = a.count[r];
+        int left = a.count[t];
         for (int base = r; left > 0; base += 1024) {
             int n = 1;
             if (left == 1 && base == r) {  // the usual case: nobody else
@@ -552,8 +531,9 @@ struct LlDw {
     const char* g;
     int H, V;
     int m_tiles, n_tiles, steps, v_begin, v64;
-    const int* slot;           // [V], sums [N][H]: what rounding took from G at the rows' tokens
-    const float* sums;
+    const int* slot;           // [V] as in LlGroup
+    const float* sums;         // [N][H]: what rounding took from G at the rows' tokens, `last` being row N - 1
+    int last;
     uint16_t* out;             // [V][H]
 };
 
@@ -614,7 +594,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
 #pragma unroll
         for (int n = 0; n < S::NB; ++n)
             if (__any(slot[n] >= 0)) {  // the sum goes on from what rounding took from G
-                const float* const sums = a.sums + (int64_t)slot[n] * a.H;
+                const float* const sums = a.sums + (int64_t)(a.last - slot[n]) * a.H;
 #pragma unroll
                 for (int m = 0; m < S::MA; ++m) {
                     const int h = h0 + (wm * S::MA + m) * 32;
@@ -690,7 +670,7 @@ struct LlBackward {
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
     int splits;
-    size_t rows, tok, rest, first, count, slot, sums, copy, g, slabs, total;
+    size_t rows, tok, rest, count, slot, sums, copy, g, slabs, total;
 };
 
 // Splits of d hidden's sum: as many as fill the CUs evenly, each at least eight steps long.
@@ -732,8 +712,7 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.rows = take(ll_up(N, 256) * sizeof(LlRow));  // tiles may reach past n_pad
     b.tok = take((int64_t)N * 4);
     b.rest = take((int64_t)N * 4);
-    b.first = take(want_w ? (int64_t)N * 4 : 0);
-    b.count = take(want_w ? (int64_t)N * 4 : 0);
+    b.count = take(want_w ? (int64_t)V * 4 : 0);
     b.slot = take(want_w ? (int64_t)V * 4 : 0);
     b.sums = take(want_w ? (int64_t)N * H * 4 : 0);
     b.copy = at;
@@ -883,12 +862,14 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
                 scratch_bytes, b.total);
     GRX_REQUIRE(((uintptr_t)scratch & 15u) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
     GRX_REQUIRE((int64_t)b.splits * b.h_tiles * b.dh_tiles < (1 << 23), GRX_E_UNSUPPORTED, "%s: too many tiles", who);
+    GRX_REQUIRE((int64_t)p->N * p->H / 1024 < (1 << 24), GRX_E_UNSUPPORTED, "%s: more than 2^34 hidden elements", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
     LlRow* rows = reinterpret_cast<LlRow*>(s + b.rows);
     int* tok = reinterpret_cast<int*>(s + b.tok);
     float* rest = reinterpret_cast<float*>(s + b.rest);
     int* slot = reinterpret_cast<int*>(s + b.slot);
+    int* count = reinterpret_cast<int*>(s + b.count);
     float* sums = reinterpret_cast<float*>(s + b.sums);
     char* copy = want_w ? s + b.copy : nullptr;
     char* g = s + b.g;
@@ -896,13 +877,13 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     const LlOperands o = ll_operands(p);
 
     LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
-                 (float)(1.0 / (double)p->temperature), rows, tok, rest, copy, slot};
+                 (float)(1.0 / (double)p->temperature), rows, tok, rest, copy, slot, count};
     hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(ll_up(p->N, 256) / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
                        stream, pr);
     GRX_CHECK_HIP(hipGetLastError());
-    const LlGroup gr = {o, tok, rest, reinterpret_cast<int*>(s + b.first), reinterpret_cast<int*>(s + b.count), slot, sums};
+    const LlGroup gr = {o, tok, rest, slot, count, sums};
     if (want_w) {
-        hipLaunchKernelGGL(lm_logps_group_kernel, dim3((unsigned)p->N), dim3(256), 0, stream, gr);
+        hipLaunchKernelGGL(lm_logps_group_kernel, dim3((unsigned)((p->N + 255) / 256)), dim3(256), 0, stream, gr);
         GRX_CHECK_HIP(hipGetLastError());
     }
     for (int c = 0; c < b.n_chunks; ++c) {
@@ -921,7 +902,7 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
             hipLaunchKernelGGL(lm_logps_rest_kernel, dim3((unsigned)(p->N < 1024 ? p->N : 1024), (unsigned)((p->H + 255) / 256)),
                                dim3(256), 0, stream, gr, v0, (int)(v0 + cols));
             GRX_CHECK_HIP(hipGetLastError());
-            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64, slot, sums,
+            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64, slot, sums, p->N - 1,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
             const int64_t wgs = ll_resident(256, (int64_t)x.m_tiles * x.n_tiles);
             if (x.steps <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
@@ -930,7 +911,6 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     }
     if (want_h) {
         const int64_t n = (int64_t)p->N * p->H;
-        GRX_REQUIRE(n / 1024 < (1 << 24), GRX_E_UNSUPPORTED, "%s: too many elements", who);
         hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, o, slabs,
                            b.splits, tok, rest, reinterpret_cast<uint16_t*>(p->grad_hidden));
         GRX_CHECK_HIP(hipGetLastError());

@@ -274,10 +274,10 @@ py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const
 
 // ---- the loss ------------------------------------------------------------------------------------------------
 struct PolicyLoss : Function<PolicyLoss> {
-    static Tensor forward(AutogradContext* ctx, const Tensor& logps, const Tensor& stats, grx_policy_loss_args* a) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& logps, const Tensor& stats, grx_policy_loss_args* a, bool want_grad) {
         const at::OptionalDeviceGuard guard(logps.device());
         const Tensor loss = f32_like({}, logps);
-        const Tensor unit = logps.requires_grad() ? f32_like(logps.sizes(), logps) : Tensor();
+        const Tensor unit = want_grad ? f32_like(logps.sizes(), logps) : Tensor();
         a->loss = ptr<float>(loss);
         a->stats = ptr<float>(stats);
         a->unit_grad = ptr<float>(unit);
@@ -295,7 +295,7 @@ struct PolicyLoss : Function<PolicyLoss> {
         const Tensor grad = at::empty_like(unit);
         check(api.policy_loss_backward(ptr<float>(unit), ptr<float>(stats), ptr<float>(g), unit.numel(), ptr<float>(grad),
                                        stream_on(unit.device())));
-        return once(incoming, {grad, Tensor(), Tensor()});
+        return once(incoming, {grad, Tensor(), Tensor(), Tensor()});
     }
 };
 
@@ -387,7 +387,7 @@ py::tuple policy_loss(const Tensor& logps_, const Tensor& advantages, const Tens
     a.epsilon_high = epsilon_high;
     a.delta = delta.value_or(0.0);
     a.normalizer = normalizer;
-    const Tensor loss = PolicyLoss::apply(logps, stats, &a);
+    const Tensor loss = PolicyLoss::apply(logps, stats, &a, at::GradMode::is_enabled() && logps.requires_grad());
     const std::vector<Tensor> s = stats.unbind(0);
     return py::make_tuple(loss, s[0], s[1], s[2]);
 }

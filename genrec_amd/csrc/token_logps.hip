@@ -41,6 +41,7 @@ struct TlArgs {
     const float* h;
     void* grad;
     int n_chunks;
+    int row0;                // first row of the launch
 };
 
 // A thread's share: m = largest logit, s = sum of 2^((x - m) k), u = sum of the same times (x - m) k.
@@ -243,7 +244,7 @@ template <int DT, bool ENT>
 __global__ __launch_bounds__(TL_THREADS) void token_logps_grad_kernel(TlArgs a) {
     typedef typename Elem<DT>::T T;
     constexpr int PV = Elem<DT>::kPerVec;
-    const int row = blockIdx.x / a.n_chunks, chunk = blockIdx.x - row * a.n_chunks;
+    const int at_row = blockIdx.x / a.n_chunks, chunk = blockIdx.x - at_row * a.n_chunks, row = a.row0 + at_row;
     const int64_t id = tl_id(a, row);
     T* __restrict__ d = reinterpret_cast<T*>(a.grad) + (int64_t)row * a.V;
     int head = (int)(((16 - ((uintptr_t)d & 15)) & 15) / sizeof(T));
@@ -354,6 +355,7 @@ static TlArgs tl_args(const grx_token_logps_args* p) {
     a.h = p->grad_entropy;
     a.grad = p->grad_logits;
     a.n_chunks = 1;
+    a.row0 = 0;
     return a;
 }
 
@@ -413,7 +415,10 @@ extern "C" int grx_token_logps_backward(const grx_token_logps_args* p, void* str
     const int pv = p->dtype == GRX_F32 ? 4 : 8;
     a.n_chunks = (p->V / pv + TL_CHUNK_VECS - 1) / TL_CHUNK_VECS;
     if (a.n_chunks < 1) a.n_chunks = 1;
-    GRX_REQUIRE(rows * a.n_chunks < (1 << 24), GRX_E_UNSUPPORTED, "%s: too many rows", who);
-    TL_LAUNCH(token_logps_grad_kernel, rows * a.n_chunks, a);
+    const int64_t most = ((1 << 24) - 1) / a.n_chunks;  // a launch holds fewer than 2^32 threads
+    for (int64_t row = 0; row < rows; row += most) {
+        a.row0 = (int)row;
+        TL_LAUNCH(token_logps_grad_kernel, (rows - row < most ? rows - row : most) * a.n_chunks, a);
+    }
     return GRX_OK;
 }

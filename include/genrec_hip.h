@@ -748,9 +748,10 @@ GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* str
  * padding as above, [N] each.  Backward writes grad_hidden [N, H] and / or grad_weight [V, H], bf16,
  * contiguous, 16-byte aligned, all of them (a null one is not computed); the logits' gradient in
  * between is bf16.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
- * H a multiple of 64, operand rows 16-byte aligned.  scratch: the bytes that the matching size
- * function names (backward: a chunk of the logits' gradient, about 1 GB at many rows), 16-byte
- * aligned, contents need no initialisation; calls that may overlap must not share it.
+ * H a multiple of 64, at most 2^34 elements of hidden in the backward pass, operand rows 16-byte
+ * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row;
+ * backward: a chunk of the logits' gradient, up to 1 GB, and 6 to 10 bytes per element of hidden),
+ * 16-byte aligned, contents need no initialisation; calls that may overlap must not share it.
  */
 typedef struct grx_lm_token_logps_args {
     const void* hidden;

@@ -208,6 +208,78 @@ def test_gradient_against_differences():
         assert abs(float(grad[at]) - slope) <= 1e-6 + 4 * _row_rel(37) * 10
 
 
+def test_what_autograd_may_ask():
+    """One of two outputs, a graph kept for a second backward, a second derivative refused, no graph at all."""
+    logits, ids = _case((6, 5), 701, torch.float32, seed=31)
+    x = logits.clone().requires_grad_()
+    lp, ent = token_logps(x, ids, return_entropy=True)
+    g = torch.randn_like(lp)
+    (a,) = torch.autograd.grad(lp, x, g, retain_graph=True)
+    (b,) = torch.autograd.grad(ent, x, g, retain_graph=True)
+    (both,) = torch.autograd.grad([lp, ent], x, [g, g], retain_graph=True)
+    want = [_definition(logits, ids, 1.0, *w)[2] for w in ((g, None), (None, g), (g, g))]
+    bound = (_row_rel(701) + 32 * U) * 8 * (3 * math.log(701) + 8) * float(g.abs().max())  # as _check, for the largest p = 1
+    for got, w in zip((a, b, both), want):
+        assert float((got.double() - w).abs().max()) <= bound
+    (again,) = torch.autograd.grad(lp, x, g)
+    assert torch.equal(a, again)
+    lp = token_logps(x, ids)
+    (d,) = torch.autograd.grad(lp, x, torch.ones_like(lp).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentia"):
+        torch.autograd.grad(d.sum(), x)
+    loss = policy_loss(lp, torch.ones(6, device=x.device), torch.ones_like(lp)).loss
+    (d,) = torch.autograd.grad(loss, lp, torch.ones_like(loss).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentia"):
+        d.sum().backward()
+    with torch.no_grad():
+        assert not token_logps(x, ids).requires_grad
+        assert not policy_loss(lp, torch.ones(6, device=x.device), torch.ones_like(lp)).loss.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(token_logps(x, ids), lp)
+
+
+def test_more_rows_than_one_launch_and_offsets_past_32_bits():
+    """2^23 rows of 4104: the gradient takes more workgroups than a launch may have, and 69 GB."""
+    dev = torch.device("cuda", 0)
+    if torch.cuda.mem_get_info(dev)[0] < 90 << 30:
+        pytest.skip("needs 90 GB of free memory")
+    N, V = 1 << 23, 4104
+    g = torch.Generator(device=dev).manual_seed(33)
+    one = (torch.randn((1, V), generator=g, device=dev) * 3).to(torch.bfloat16)
+    x = one.expand(N, V).detach().requires_grad_()
+    ids = torch.randint(0, V, (N,), generator=g, device=dev)
+    rows = torch.tensor([0, 1, 77, 4194303, 4194304, 8388606, 8388607], device=dev)
+    up = torch.zeros(N, device=dev)
+    up[rows] = torch.randn(rows.shape, generator=g, device=dev)
+    lp = token_logps(x, ids)
+    (grad,) = torch.autograd.grad(lp, x, up)
+    want, _, _ = _definition(one.expand(rows.numel(), V), ids[rows], 1.0)
+    assert ((lp[rows].double() - want).abs() <= _row_rel(V) + 6 * U * want.abs()).all()
+    _, _, d = _check(one.expand(rows.numel(), V), ids[rows], entropy=False, g=up[rows])
+    assert torch.equal(grad[rows], d)
+    assert not grad[2:77].any() and not grad[4194305:4194400].any() and not grad[8388500:8388606].any()
+    far = grad[:: 1 << 22]  # rows 2^22 apart: 1.7e10 elements
+    far.copy_((torch.randn((2, V), generator=g, device=dev) * 3).to(torch.bfloat16))
+    _check(far, torch.tensor([5, 4103], device=dev))
+
+
+def test_called_on_a_stream_of_its_own():
+    """The call follows the current stream, and its backward pass the stream of the call."""
+    logits, ids = _case((300, 4), 20011, torch.bfloat16, seed=35)
+    g = torch.randn(ids.shape, device=logits.device)
+    x = logits.clone().requires_grad_()
+    want = torch.autograd.grad(token_logps(x, ids), x, g)[0]
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        y = logits.detach().requires_grad_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            lp = token_logps(y, ids)
+        torch.cuda.current_stream().wait_stream(side)
+        (got,) = torch.autograd.grad(lp, y, g)  # called with another stream current
+        assert torch.equal(got, want)
+
+
 # ---- the loss ------------------------------------------------------------------------------------------------
 
 
@@ -358,6 +430,27 @@ def test_bounds_and_extreme_ratios():
     res = policy_loss(x, torch.ones(1, device=dev), torch.ones_like(x), torch.zeros_like(x))
     res.loss.backward()
     assert float(res.loss) == pytest.approx(-1.2, abs=1e-6) and float(x.grad) == 0.0
+
+
+@pytest.mark.parametrize("kind,level", [("grpo", "token"), ("bnpo", "sequence"), ("dapo", "token")])
+def test_loss_gradient_against_differences(kind, level):
+    """A step of h = 2^-6 either way, away from the bounds (|d| < 0.15 + h): off by h^2 / 6 of the third derivative
+    (|w A| + beta e^q, below 3 here with its weight below 1) and by the rounding of two losses, 24 u of their size each."""
+    logps, adv, mask, old, ref = _loss_inputs(3, 9, seed=23)
+    old = logps + (old - logps).clamp(-0.15, 0.15)
+    mask[:, 0] = 1
+    o = dict(beta=0.1, loss_type=kind, importance_sampling_level=level, num_items=20)
+    x = logps.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(policy_loss(x, adv, mask, old, ref, **o).loss, x)
+    size = float((adv.abs().max() * 1.2 + 0.1 * 8))
+    h = 2.0 ** -6
+    for r, t in ((0, 0), (1, 0), (2, 0), (0, 4), (1, 3), (2, 8)):
+        up, down = logps.clone(), logps.clone()
+        up[r, t] += h
+        down[r, t] -= h
+        a, b = (float(policy_loss(v, adv, mask, old, ref, **o).loss) for v in (up, down))
+        step = float(up[r, t].double() - down[r, t].double())
+        assert abs((a - b) / step - float(grad[r, t])) <= h * h / 6 * size * 1.1 + 2 * 24 * U * 2 * size / step
 
 
 def test_rows_without_positions_read_nothing():

@@ -136,6 +136,57 @@ def test_shared_tokens_and_the_size_of_the_error(N, tokens):
         assert (got - want).norm() / want.norm() <= 1.25 * own + 1e-6
 
 
+def test_gradient_against_differences():
+    """f = g . logps + h . entropies along single hidden and weight entries, from 1 - 2^-7 to 1 + 2^-7 (exact in bf16).
+    Off by 2^-14 / 6 of the third derivative (sums of |G| |w|^3 and the like: below the bound's 2^-8 sum |G| |w|), by two
+    values' errors over the step, and by the gradient's own bound: bf16 G and a result in bf16."""
+    hidden, weight, ids, g, _ = _inputs((6,), 128, 300, seed=41, pad=0.0)
+    step = 2.0 ** -7
+
+    def value(hid, wei):
+        return float((lm_head_token_logps(hid, wei, ids) * g).double().sum())
+
+    for n, k in ((0, 0), (3, 77), (5, 127)):
+        for of in (0, 1):
+            hid, wei = hidden.clone(), weight.clone()
+            row = n if of == 0 else int(ids[n])
+            (hid, wei)[of][row, k] = 1.0
+            x, w = hid.clone().requires_grad_(), wei.clone().requires_grad_()
+            grad = torch.autograd.grad((lm_head_token_logps(x, w, ids) * g).sum(), [x, w])[of][row, k]
+            ends = []
+            for d in (step, -step):
+                (hid, wei)[of][row, k] = 1.0 + d
+                ends.append(value(hid, wei))
+            _, _, G, flat, wd, err, _, _ = _definition(hid, wei, ids, 1.0, g, None)
+            size = float((G.abs() @ wd.abs())[n, k] if of == 0 else (G.abs().T @ flat.abs())[row, k])
+            values = 2 * float(g.abs().sum()) * (2 * err + (300 / 256 + 160) * U) / (2 * step)
+            assert abs((ends[0] - ends[1]) / (2 * step) - float(grad)) <= 3 * HALF * size + HALF * abs(float(grad)) + values
+
+
+def test_many_rows_of_few_tokens():
+    """20,011 rows over 257 tokens: every row shares its token with about 78 others, from one end to the other."""
+    hidden, weight, ids, g, h = _inputs((20011,), 64, 257, seed=43)
+    _check(hidden, weight, ids, g)
+    _check(hidden, weight, torch.where(ids >= 0, 256, ids), g)
+
+
+def test_what_autograd_may_ask():
+    hidden, weight, ids, g, h = _inputs((70,), 128, 500, seed=45)
+    _, _, dh, dw = _check(hidden, weight, ids, g)
+    x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
+    lp, ent = lm_head_token_logps(x, w, ids, return_entropy=True)
+    a = torch.autograd.grad(lp, [x, w], g, retain_graph=True)  # the entropies unused
+    b = torch.autograd.grad(lp, [x, w], g, retain_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and torch.equal(a[0], dh) and torch.equal(a[1], dw)
+    (d,) = torch.autograd.grad(lp, x, g.clone().requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="differentia"):
+        torch.autograd.grad(d.float().sum(), x)
+    with torch.no_grad():
+        assert not lm_head_token_logps(x, w, ids).requires_grad
+    with torch.inference_mode():
+        assert torch.equal(lm_head_token_logps(x, w, ids), lp)
+
+
 def test_padding_may_hold_anything():
     hidden, weight, ids, g, h = _inputs((4, 20), 128, 900, seed=5, pad=0.4)
     g = torch.where(torch.rand(g.shape, device=g.device) < 0.2, torch.zeros_like(g), g)

@@ -89,6 +89,34 @@ Tensor grad_rows(const Tensor& g) {
     return (g.scalar_type() == at::kFloat ? g : g.to(at::kFloat)).contiguous();
 }
 
+bool recording(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (s == nullptr) return false;  // the default stream cannot be recorded
+    C10_HIP_CHECK(hipStreamIsCapturing(s, &status));
+    return status != hipStreamCaptureStatusNone;
+}
+
+// Called by a backward pass.  Recorded into a HIP graph, its gradients cannot go to a node that was made outside of the
+// recording (a leaf that a living eager graph holds too): autograd would let the recording wait for that node's stream,
+// which ends the process.
+void refuse_nodes_outside(const at::Device& device) {
+    const auto stream = c10::hip::getCurrentHIPStream(device.index());
+    if (!recording(stream.stream())) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const auto& next = node->next_edge(i);
+        if (!next.is_valid() || !node->task_should_compute_output(i)) continue;
+        const auto theirs = next.function->stream();
+        if (!theirs || theirs->device_type() == at::kCPU || theirs->id() == stream.id()) continue;
+        const c10::Device on(stream.device_type(), theirs->device_index());  // whichever name the type goes by
+        const c10::hip::HIPStream other(c10::hip::HIPStream::UNCHECKED, c10::Stream(c10::Stream::UNSAFE, on, theirs->id()));
+        TORCH_CHECK(recording(other.stream()),
+                    "a backward pass recorded into a HIP graph needs leaves of its own: detach().requires_grad_() inside the "
+                    "recording, or drop the graphs made outside of it first");
+    }
+}
+
 // The kernels have no gradient of their own: under create_graph the results carry a node that says so when it is reached.
 variable_list once(const variable_list& incoming, variable_list out) {
     if (!at::GradMode::is_enabled()) return out;
@@ -152,6 +180,7 @@ struct TokenLogps : Function<TokenLogps> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &logits = saved[0], &ids = saved[1], &stats = saved[2], &ent = saved[3];
         const at::OptionalDeviceGuard guard(logits.device());
+        refuse_nodes_outside(logits.device());
         const Tensor g = grad_rows(incoming[0]), h = incoming.size() > 1 ? grad_rows(incoming[1]) : Tensor();
         const Tensor grad = at::empty(logits.sizes(), logits.options());
         grx_token_logps_args a = token_args(logits, ids, ctx->saved_data["temperature"].toDouble());
@@ -234,6 +263,7 @@ struct LmTokenLogps : Function<LmTokenLogps> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &hidden = saved[0], &weight = saved[1], &ids = saved[2], &stats = saved[3], &ent = saved[4];
         const at::OptionalDeviceGuard guard(hidden.device());
+        refuse_nodes_outside(hidden.device());
         const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
         const Tensor g = grad_rows(incoming[0]), h = incoming.size() > 1 ? grad_rows(incoming[1]) : Tensor();
         const Tensor grad_h = want_h ? at::empty(hidden.sizes(), hidden.options()) : Tensor();
@@ -291,6 +321,7 @@ struct PolicyLoss : Function<PolicyLoss> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &unit = saved[0], &stats = saved[1];
         const at::OptionalDeviceGuard guard(unit.device());
+        refuse_nodes_outside(unit.device());
         const Tensor g = grad_rows(incoming[0]);
         const Tensor grad = at::empty_like(unit);
         check(api.policy_loss_backward(ptr<float>(unit), ptr<float>(stats), ptr<float>(g), unit.numel(), ptr<float>(grad),

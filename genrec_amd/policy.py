@@ -53,7 +53,7 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
     id marks padding: its row of logits is not read, results and gradient are 0 whatever it holds.  An id that
     is not below V gives NaN.  Differentiable in ``logits`` (the gradient has their type); rows whose incoming
     gradient is 0 cost one write.  A pass recorded into a HIP graph needs leaves of its own: take
-    ``logits.detach().requires_grad_()`` inside the recording."""
+    ``logits.detach().requires_grad_()`` inside the recording (gradients that would leave it are refused)."""
     return (_ops_module or _ops()).token_logps(logits, token_ids, temperature, return_entropy)
 
 

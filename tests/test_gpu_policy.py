@@ -572,6 +572,39 @@ def test_step_recorded_into_a_graph():
         assert torch.equal(made["out"][0], loss) and torch.equal(made["out"][1], grad)
 
 
+def test_recording_refuses_leaves_of_an_eager_graph():
+    """A leaf that a living eager graph holds: the recorded backward pass is refused before anything waits for the other
+    stream, and with that graph gone, or a leaf of the recording's own, the same pass is recorded."""
+    logits, ids, mask, adv, old, ref = _step_inputs(8)
+    x = token_logps(logits[:, :-1].contiguous(), ids).detach().requires_grad_()
+    y = logits[:, :-1].contiguous().requires_grad_()
+    g = torch.ones_like(x)
+
+    def loss():
+        return torch.autograd.grad(policy_loss(x, adv, mask, old).loss, x)[0]
+
+    def logps():
+        return torch.autograd.grad(token_logps(y, ids), y, g)[0]
+
+    for step in (loss, logps):
+        want = step()
+        alive = (policy_loss(x, adv, mask, old).loss, token_logps(y, ids))
+        with pytest.raises(RuntimeError, match="leaves of its own"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                step()
+        torch.cuda.synchronize()
+        assert torch.equal(step(), want)
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and torch.equal(step(), want)
+
+
 def test_two_streams_at_once():
     a, b = _step_inputs(6, V=20011), _step_inputs(7, V=20011)
     want = [_step(*a), _step(*b)]

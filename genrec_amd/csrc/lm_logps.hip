@@ -625,19 +625,31 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
 static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
 // Rows per tile of the products with the logits' shape (m_tiles x n tiles of 256 x BN): what counts is whole rounds over
-// the CUs.  At H = 2048 a round takes 52 to 56 us with tiles of 256 rows, 33 to 37 with 128, 41 with 64 (two to a CU):
-// 320 rows at V = 152,640 take 240 us in 7 rounds of 128 and 267 in 5 of 256, 400 rows 309 in 10 and 270 in 5.
+// the CUs.  At H = 2048 a round takes 54 us with tiles of 256 rows, 45 with 192, 34 with 128, 41 with 64 (two to a CU).
+// At V = 152,640 320 rows take 230 us in 5 rounds of 192, 237 in 7 of 128 and 270 in 5 of 256; 576 rows 310, 374 and 380;
+// 400 rows 270 in 5 rounds of 256 and 309 in 10 of 128.
+static double ll_cost(int bn) { return bn == 64 ? 0.4 : bn == 128 ? 0.64 : bn == 192 ? 0.84 : 1.0; }
+
 static int ll_bn(int N, int64_t m_tiles) {
     int best = 0;
     double least = 0.0;
-    for (int bn = 64; bn <= 256; bn *= 2) {
-        const int64_t tiles = m_tiles * ((N + bn - 1) / bn), wgs = bn == 64 ? 2 * LL_CUS : LL_CUS;
-        const double cost = (double)((tiles + wgs - 1) / wgs) * (bn == 64 ? 0.8 : bn == 128 ? 0.64 : 1.0);
+    for (int bn = 64; bn <= 256; bn += 64) {
+        const int64_t tiles = m_tiles * ((N + bn - 1) / bn), per_cu = bn == 64 ? 2 : 1, wgs = per_cu * LL_CUS;
+        const double cost = (double)((tiles + wgs - 1) / wgs) * ll_cost(bn) * per_cu;
         if (best == 0 || cost <= least) {
             best = bn;
             least = cost;
         }
     }
+    return best;
+}
+
+// Rows per tile of d hidden, whose sum is split over the columns until the CUs are full: the least work (320 rows: 203 us
+// with 192, 256 with 256 and 260 with 128).
+static int ll_dh_bn(int N) {
+    int best = 64;
+    for (int bn = 128; bn <= 256; bn += 64)
+        if ((N + bn - 1) / bn * ll_cost(bn) <= (N + best - 1) / best * ll_cost(best)) best = bn;
     return best;
 }
 
@@ -647,7 +659,9 @@ struct LlForward {
     size_t partials, weighted, chosen, total;  // byte offsets, total size
 };
 
-static int ll_wm(int bn) { return bn == 64 ? MtShape<64>::WM : bn == 128 ? MtShape<128>::WM : MtShape<256>::WM; }
+static int ll_wm(int bn) {
+    return bn == 64 ? MtShape<64>::WM : bn == 128 ? MtShape<128>::WM : bn == 192 ? MtShape<192>::WM : MtShape<256>::WM;
+}
 
 static LlForward ll_forward(int N, int V, bool ent) {
     LlForward f;
@@ -690,7 +704,7 @@ static int ll_splits(int64_t tiles, int64_t steps) {
 
 static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     LlBackward b;
-    b.dh_bn = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+    b.dh_bn = ll_dh_bn(N);
     b.dh_tiles = (N + b.dh_bn - 1) / b.dh_bn;
     b.h_tiles = (H + MT_BM - 1) / MT_BM;
     b.n_pad = ll_up(N, MT_BK);
@@ -709,7 +723,7 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
         at += (size_t)ll_up(bytes, 256);
         return begin;
     };
-    b.rows = take(ll_up(N, 256) * sizeof(LlRow));  // tiles may reach past n_pad
+    b.rows = take((int64_t)b.n_tiles * b.bn * sizeof(LlRow));  // tiles may reach past n_pad
     b.tok = take((int64_t)N * 4);
     b.rest = take((int64_t)N * 4);
     b.count = take(want_w ? (int64_t)V * 4 : 0);
@@ -790,6 +804,7 @@ static int64_t ll_resident(int bn, int64_t tiles) {
     do {                                                    \
         if ((bn) == 64) LL_ONE(64, (kernel<64>), grid, args);        \
         else if ((bn) == 128) LL_ONE(128, (kernel<128>), grid, args); \
+        else if ((bn) == 192) LL_ONE(192, (kernel<192>), grid, args); \
         else LL_ONE(256, (kernel<256>), grid, args);        \
     } while (0)
 #define LL_EACH_ENT(bn, ent, kernel, grid, args)                                  \
@@ -800,6 +815,9 @@ static int64_t ll_resident(int bn, int64_t tiles) {
         } else if ((bn) == 128) {                                                 \
             if (ent) LL_ONE(128, (kernel<128, true>), grid, args);                \
             else LL_ONE(128, (kernel<128, false>), grid, args);                   \
+        } else if ((bn) == 192) {                                                 \
+            if (ent) LL_ONE(192, (kernel<192, true>), grid, args);                \
+            else LL_ONE(192, (kernel<192, false>), grid, args);                   \
         } else {                                                                  \
             if (ent) LL_ONE(256, (kernel<256, true>), grid, args);                \
             else LL_ONE(256, (kernel<256, false>), grid, args);                   \
@@ -878,7 +896,7 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
 
     LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
                  (float)(1.0 / (double)p->temperature), rows, tok, rest, copy, slot, count};
-    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(ll_up(p->N, 256) / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
+    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_tiles * b.bn / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
                        stream, pr);
     GRX_CHECK_HIP(hipGetLastError());
     const LlGroup gr = {o, tok, rest, slot, count, sums};

@@ -36,6 +36,7 @@ typedef __attribute__((address_space(3))) const mt_s16x8 mt_lds_s16x8;
 template <int BN>
 struct MtShape;
 template <> struct MtShape<256> { static constexpr int WM = 2, WN = 4, MA = 4, NB = 2, DEEP = 3, FLAT = 2, THREADS = 512; };
+template <> struct MtShape<192> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 3, DEEP = 3, FLAT = 2, THREADS = 512; };
 template <> struct MtShape<128> { static constexpr int WM = 4, WN = 2, MA = 2, NB = 2, DEEP = 3, FLAT = 3, THREADS = 512; };
 template <> struct MtShape<64> { static constexpr int WM = 8, WN = 1, MA = 1, NB = 2, DEEP = 2, FLAT = 2, THREADS = 512; };
 

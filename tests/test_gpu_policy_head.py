@@ -97,10 +97,11 @@ def test_logps_and_gradients(shape, H, V):
     _check(hidden, weight, ids, g, h, 0.8)
 
 
-@pytest.mark.parametrize("N", [5, 320])
+@pytest.mark.parametrize("N", [5, 150, 320])
 def test_real_vocabulary(N):
     hidden, weight, ids, g, h = _inputs((N,), 256, 151669, seed=N)
     _check(hidden, weight, ids, g, h, 1.2)
+    _check(hidden, weight, ids, g, None, 0.9)  # 150 and 320 rows: tiles of 192
 
 
 def test_strided_operands_and_one_gradient_only():

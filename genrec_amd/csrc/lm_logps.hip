@@ -6,11 +6,12 @@
 //   d hidden = G x weight (sum over v),    d weight = G^T x hidden (sum over rows)
 // follow with fp32 accumulators.  What rounding takes from a row's largest element, the one at its token, is kept in
 // fp32 and added to both sums (as a multiple of the token's weight row, of the row's hidden state): without it it is
-// an error of up to 2^-8 of a whole row of either gradient.  Four products of 2 N V H; bound by the matrix cores at many rows, by the weight
-// (V H elements read per product, written once) at few.
+// an error of up to 2^-8 of a whole row of either gradient.  Four products of 2 N V H; bound by the matrix cores at many
+// rows, by the weight (V H elements read per product, written once) at few.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.h"
@@ -21,31 +22,197 @@
 #define LL_CUS 256
 #define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk
 
+// The rows that count are brought together first: what follows works on `plan[0]` rows, a number that only the device
+// knows, and padding costs nothing but its place in the scratch memory (1403 rows, half of them padding, H = 3584,
+// V = 151,669, with the gradient of hidden: 1.98 ms, 3.89 with all rows in the products; without padding 320 rows
+// take 16 us more of 1020).
 struct LlOperands {
     const uint16_t* weight;     // [V, H]
     int64_t weight_ld;
+    const uint16_t* hidden;     // [rows, H], the rows that count
+    const int* plan;            // LL_PLAN_*
+    int H, V;
+};
+#define LL_PLAN_ROWS 0          // rows that count
+#define LL_PLAN_SPLITS 1        // splits of d hidden's sum
+
+struct LlCompact {
     const uint16_t* hidden;     // [N, H]
     int64_t hidden_ld;
+    const int64_t* ids;         // [N]
     int N, H, V;
+    const int* offsets;         // [ceil(N / 16)] rows that count in front of every 16; null: each workgroup counts them
+    uint16_t* to;               // [rows, H]
+    int* plan;
+    int* tok;                   // [rows] the row's token
+    // forward: row_of [rows], and the results of the rows that do not count
+    int* row_of;
+    float* logps;
+    float2* stats;
+    float* entropy;
+    // backward
+    const float* g;
+    const float* h;
+    float inv_t;
+    int* pos;                   // [N] place among the rows that count, or -1
+    struct LlRow* rows;
+    float* rest;                // [rows] cleared: what rounding G takes from the element at the token
+    int* slot;                  // [V] cleared to -1; null: no d weight
+    int* count;                 // [V] cleared to 0, with slot
+    int dh_bn, h_tiles, steps, slab_rows;  // what splits are chosen by
 };
+
+// What a row needs to turn a product into its gradient: w = 2^((x - m) k), G = w (alpha + beta (x - m) k) + at at the
+// token.
+struct LlRow {
+    float m, alpha, beta, at;
+    int tok;
+    int pad[3];
+};
+
+// Splits of d hidden's sum: as many as fill the CUs evenly, each at least eight steps long.
+__host__ __device__ static int ll_splits(int rows, int bn, int h_tiles, int steps, int slab_rows) {
+    const int64_t tiles = (int64_t)((rows + bn - 1) / bn) * h_tiles;
+    if (tiles >= 16 * LL_CUS || rows <= 0) return 1;
+    const int by_steps = steps / 8, by_room = slab_rows / rows, both = by_steps < by_room ? by_steps : by_room;
+    const int most = both < 64 ? both : 64;
+    int best = 1;
+    float best_use = 0.f;
+    for (int s = 1; s == 1 || s <= most; ++s) {
+        const int wgs = (int)tiles * s;
+        const float use = (float)wgs / (float)((wgs + LL_CUS - 1) / LL_CUS * LL_CUS);
+        if (use > best_use + 0.04f) {
+            best_use = use;
+            best = s;
+        }
+    }
+    return best;
+}
+
+// Backward, rows whose gradients are 0 do not count either.
+template <bool BACK>
+__device__ __forceinline__ bool ll_counts(const LlCompact& a, int r) {
+    return r < a.N && a.ids[r] >= 0 && (!BACK || (a.g && a.g[r] != 0.f) || (a.h && a.h[r] != 0.f));
+}
+
+template <bool BACK>
+__global__ __launch_bounds__(1024) void lm_logps_offsets_kernel(LlCompact a, int* offsets, int n) {
+    __shared__ int part[16];
+    int all = 0;
+    for (int base = 0; base < n; base += 1024) {
+        const int i = base + threadIdx.x;
+        int mine = 0;
+        if (i < n)
+            for (int j = 0; j < 16; ++j) mine += ll_counts<BACK>(a, i * 16 + j) ? 1 : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(upto, o, 64);
+            if ((threadIdx.x & 63) >= o) upto += x;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) part[threadIdx.x >> 6] = upto;
+        __syncthreads();
+        int before = all + upto - mine;
+        for (int w = 0; w < 16; ++w) {
+            if (w < (int)(threadIdx.x >> 6)) before += part[w];
+            all += part[w];
+        }
+        if (i < n) offsets[i] = before;
+    }
+}
+
+// Workgroup (16 rows, 512 h); the ones behind the last row only help to clear `slot`.
+template <bool BACK>
+__global__ __launch_bounds__(256) void lm_logps_compact_kernel(LlCompact a) {
+    __shared__ int part[4], place[16];
+    const int r0 = blockIdx.x * 16;
+    if (BACK && a.slot != nullptr)
+        for (int64_t v = ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.V;
+             v += (int64_t)gridDim.x * gridDim.y * 256) {
+            a.slot[v] = -1;
+            a.count[v] = 0;
+        }
+    if (r0 >= a.N) return;
+    int before = 0;
+    if (a.offsets == nullptr) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < r0; i += 256) before += ll_counts<BACK>(a, i) ? 1 : 0;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = before;
+        __syncthreads();
+        before = part[0] + part[1] + part[2] + part[3];
+    } else {
+        before = a.offsets[blockIdx.x];
+    }
+    if (threadIdx.x < 64) {
+        const bool counts = threadIdx.x < 16 && ll_counts<BACK>(a, r0 + threadIdx.x);
+        const uint64_t mask = __ballot(counts);
+        const int at = before + __popcll(mask & ((1ull << threadIdx.x) - 1));
+        if (threadIdx.x < 16) place[threadIdx.x] = counts ? at : -1;
+        const int r = r0 + threadIdx.x;
+        if (blockIdx.y == 0 && threadIdx.x < 16 && r < a.N) {
+            if constexpr (BACK) {
+                a.pos[r] = counts ? at : -1;
+                if (counts) {
+                    const int64_t id = a.ids[r];
+                    const float g = a.g ? a.g[r] : 0.f, h = a.h ? a.h[r] : 0.f;
+                    const float2 st = a.stats[r];
+                    const float ln2 = 0.69314718055994531f;
+                    LlRow o = {st.x, 0.f, 0.f, 0.f, 0, {0, 0, 0}};
+                    o.alpha = -(g + (a.h ? h * (a.entropy[r] - log2f(st.y) * ln2) : 0.f)) * a.inv_t / st.y;
+                    o.beta = -h * ln2 * a.inv_t / st.y;
+                    o.at = g * a.inv_t;
+                    if (id >= a.V) o.alpha = NAN;
+                    o.tok = id < a.V ? (int)id : 0;
+                    a.rows[at] = o;
+                    a.tok[at] = o.tok;
+                    a.rest[at] = 0.f;
+                }
+            } else if (counts) {
+                const int64_t id = a.ids[r];
+                a.row_of[at] = r;
+                a.tok[at] = id < a.V ? (int)id : a.V;
+            } else {
+                a.logps[r] = 0.f;
+                a.stats[r] = make_float2(0.f, 1.f);
+                if (a.entropy) a.entropy[r] = 0.f;
+            }
+        }
+        if (r0 + 16 >= a.N && blockIdx.y == 0 && threadIdx.x == 0) {  // the last 16
+            const int rows = before + __popcll(mask);
+            a.plan[LL_PLAN_ROWS] = rows;
+            if (BACK) a.plan[LL_PLAN_SPLITS] = ll_splits(rows, a.dh_bn, a.h_tiles, a.steps, a.slab_rows);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 4 + (threadIdx.x >> 6), at = place[row], h = blockIdx.y * 512 + (threadIdx.x & 63) * 8;
+        if (at >= 0 && h < a.H)
+            *reinterpret_cast<u32x4*>(a.to + (int64_t)at * a.H + h) =
+                *reinterpret_cast<const u32x4*>(a.hidden + (int64_t)(r0 + row) * a.hidden_ld + h);
+    }
+}
 
 struct LlArgs {
     LlOperands o;
-    int m_begin, m_tiles, n_tiles;  // this launch's share of the m tiles
+    int m_tiles;
     float k;                    // log2(e) / temperature
-    const int64_t* ids;         // [N]
+    const int* tok;             // [rows]
     float2* partials;           // [parts][n_pad] (max, sum), parts = m_tiles x waves along m
     float* weighted;            // [parts][n_pad], with entropies
     int64_t n_pad;
-    float* chosen;              // [N] logit of the row's token
+    float* chosen;              // [rows] logit of the row's token
 };
 
 template <int BN>
 using LlLogits = MtPipe<BN, MtAlong<MT_BM, BN>, MtReadAlong, MtAlong<BN, BN>, MtReadAlong>;
 
 template <int BN>
-__device__ __forceinline__ void ll_begin(LlLogits<BN>& pipe, const LlOperands& o, int v0, int r0) {
-    pipe.begin(MtAlong<MT_BM, BN>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN, BN>(o.hidden, o.hidden_ld, o.N, r0, 0), o.H / MT_BK);
+__device__ __forceinline__ void ll_begin(LlLogits<BN>& pipe, const LlOperands& o, int rows, int v0, int r0) {
+    pipe.begin(MtAlong<MT_BM, BN>(o.weight, o.weight_ld, o.V, v0, 0), MtAlong<BN, BN>(o.hidden, o.H, rows, r0, 0), o.H / MT_BK);
 }
 
 // Element `at` of a lane's row n: selected, where branches would make a jump table of stores.
@@ -67,18 +234,19 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
-    const int tiles = a.m_tiles * a.n_tiles;
+    const int rows = a.o.plan[LL_PLAN_ROWS], n_tiles = (rows + BN - 1) / BN, tiles = a.m_tiles * n_tiles;
+    if ((int)blockIdx.x >= tiles) return;
     LlLogits<BN> pipe(lds);
     int tm, tn;
-    mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    ll_begin(pipe, a.o, (a.m_begin + tm) * MT_BM, tn * BN);
+    mt_tile(blockIdx.x, a.m_tiles, n_tiles, tm, tn);
+    ll_begin(pipe, a.o, rows, tm * MT_BM, tn * BN);
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const int v0 = (a.m_begin + tm) * MT_BM, r0 = tn * BN, part = (a.m_begin + tm) * S::WM + wm;
-        int64_t id[S::NB];
+        const int v0 = tm * MT_BM, r0 = tn * BN, part = tm * S::WM + wm;
+        int id[S::NB];
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
-            id[n] = r < a.o.N ? a.ids[r] : -1;
+            id[n] = r < rows ? a.tok[r] : -1;
         }
         typename LlLogits<BN>::Acc acc;
         pipe.clear(acc);
@@ -86,8 +254,8 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(id[n]));  // waited for here, not behind the next copies
         if (tile + (int)gridDim.x < tiles) {
-            mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
-            ll_begin(pipe, a.o, (a.m_begin + tm) * MT_BM, tn * BN);
+            mt_tile(tile + gridDim.x, a.m_tiles, n_tiles, tm, tn);
+            ll_begin(pipe, a.o, rows, tm * MT_BM, tn * BN);
         }
         const int vw = v0 + wm * S::MA * 32 + 4 * half;  // vocabulary entry of m = 0, e = 0
 #pragma unroll
@@ -124,7 +292,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
                 a.partials[(int64_t)part * a.n_pad + r] = make_float2(mx, s);
                 if (ENT) a.weighted[(int64_t)part * a.n_pad + r] = u;
             }
-            const int off = (int)(id[n] - vw);  // runs of four entries, every eight
+            const int off = id[n] - vw;  // runs of four entries, every eight
             if (id[n] >= vw && id[n] < vw + S::MA * 32 && (off & 4) == 0) {
                 const int at = (off >> 5) * 16 + ((off & 31) >> 3) * 4 + (off & 3);
                 a.chosen[r] = ll_pick<S::MA, S::NB>(acc, n, at);
@@ -139,6 +307,7 @@ struct LlJoin {
     float* logps;
     float2* stats;
     float* entropy;
+    const int* row_of;         // [rows]
 };
 
 // Joins a row's partials, ROWS rows per workgroup.
@@ -147,7 +316,8 @@ __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
     constexpr int PER = 256 / ROWS;  // threads a row
     __shared__ float sm[PER][ROWS + 1], ss[PER][ROWS + 1], su[PER][ROWS + 1];
     const int i = threadIdx.x % ROWS, j = threadIdx.x / ROWS;
-    const int r = blockIdx.x * ROWS + i;  // n_pad is a multiple of 64: rows past N read what a clamped row left
+    const int r = blockIdx.x * ROWS + i, rows = a.g.o.plan[LL_PLAN_ROWS];
+    if ((int)blockIdx.x * ROWS >= rows) return;  // rows of the last 16 past the end read what a clamped row left
     const float k = a.g.k;
     float m = -INFINITY, s = 0.f, u = 0.f;
     auto add = [&](float pm, float ps, float pu) {
@@ -176,113 +346,42 @@ __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
             su[j][i] = u;
         }
     }
-    if (j != 0 || r >= a.g.o.N) return;
-    const int64_t id = a.g.ids[r];
+    if (j != 0 || r >= rows) return;
+    const int id = a.g.tok[r], row = a.row_of[r];
     const float ln2 = 0.69314718055994531f;
     const float ls = log2f(s);
-    if (id < 0) {
-        a.logps[r] = 0.f;
-        a.stats[r] = make_float2(0.f, 1.f);
-        if (a.entropy) a.entropy[r] = 0.f;
-        return;
-    }
-    a.logps[r] = id < a.g.o.V ? ((a.g.chosen[r] - m) * k - ls) * ln2 : NAN;
-    a.stats[r] = make_float2(m, s);
-    if (a.entropy) a.entropy[r] = (ls - u / s) * ln2;
+    a.logps[row] = id < a.g.o.V ? ((a.g.chosen[r] - m) * k - ls) * ln2 : NAN;
+    a.stats[row] = make_float2(m, s);
+    if (a.entropy) a.entropy[row] = (ls - u / s) * ln2;
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-// What a row needs to turn a product into its gradient: w = 2^((x - m) k), G = w (alpha + beta (x - m) k) + at at the
-// token.  tok = -1: nothing flows into this row (padding, or both gradients 0); its G is 0 whatever the products are.
-struct LlRow {
-    float m, alpha, beta, at;
-    int tok;
-    int pad[3];
-};
-
-struct LlPrep {
-    LlOperands o;
-    const int64_t* ids;
-    const float2* stats;
-    const float* entropy;
-    const float* g;
-    const float* h;
-    float inv_t;
-    LlRow* rows;               // one per row of the n tiles
-    int* tok;                  // [N] rows[].tok
-    float* rest;               // [N] cleared: what rounding G takes from the element at the token
-    char* copy;                // hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4]; null: no d weight
-    int* slot;                 // [V] cleared to -1, with copy
-    int* count;                // [V] cleared to 0, with copy
-};
-
-// Workgroup (64 rows, 32 h).  The copy holds 0 in the rows that do not count.
-__global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlPrep a) {
-    __shared__ bool live[64];
-    const int r0 = blockIdx.x * 64;
-    if (threadIdx.x < 64) {
-        const int r = r0 + threadIdx.x;
-        float g = 0.f, h = 0.f;
-        int64_t id = -1;
-        if (r < a.o.N) {
-            id = a.ids[r];
-            if (id >= 0) {
-                g = a.g ? a.g[r] : 0.f;
-                h = a.h ? a.h[r] : 0.f;
-            }
-        }
-        const bool counts = g != 0.f || h != 0.f;
-        live[threadIdx.x] = counts;
-        if (blockIdx.y == 0) {
-            LlRow o = {0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}};
-            if (counts) {
-                const float2 st = a.stats[r];
-                const float ln2 = 0.69314718055994531f;
-                o.m = st.x;
-                o.alpha = -(g + (a.h ? h * (a.entropy[r] - log2f(st.y) * ln2) : 0.f)) * a.inv_t / st.y;
-                o.beta = -h * ln2 * a.inv_t / st.y;
-                o.at = g * a.inv_t;
-                if (id >= a.o.V) o.alpha = NAN;
-                o.tok = id < a.o.V ? (int)id : 0;
-            }
-            a.rows[r] = o;
-            if (r < a.o.N) {
-                a.tok[r] = o.tok;
-                a.rest[r] = 0.f;
-            }
-        }
-    }
-    if (a.copy == nullptr) return;
-    for (int64_t v = ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.o.V;
-         v += (int64_t)gridDim.x * gridDim.y * 256) {
-        a.slot[v] = -1;
-        a.count[v] = 0;
-    }
-    if (r0 >= a.o.N) return;
-    __syncthreads();
-    const int lane = threadIdx.x & 63, n0 = (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
-    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
-    u16x8 v;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = live[n0 + j] ? a.o.hidden[(int64_t)(r0 + n0 + j) * a.o.hidden_ld + h] : (uint16_t)0;
-    *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
-}
-
-// Rows that share a token: the first of them stands for all.
+// Hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4], for d weight: workgroup (64 rows, 32 h).  The rows past
+// the end are 0.  Rows that share a token: the first of them stands for all.
 struct LlGroup {
     LlOperands o;
     const int* tok;
     const float* rest;
-    int* slot;                 // [V] N - 1 - the token's first row, -1: no row
+    int* slot;                 // [V] rows - 1 - the token's first row, -1: no row
     int* count;                // [V] rows with the token
-    float* sums;               // [N][H] in a first row: sum over the rows of its token of rest x hidden
+    float* sums;               // [rows][H] in a first row: sum over the rows of its token of rest x hidden
+    char* copy;
 };
 
-__global__ __launch_bounds__(256) void lm_logps_group_kernel(LlGroup a) {
-    const int r = blockIdx.x * 256 + threadIdx.x, t = r < a.o.N ? a.tok[r] : -1;
-    if (t < 0) return;
-    atomicMax(a.slot + t, a.o.N - 1 - r);  // whole numbers: any order gives the same
-    atomicAdd(a.count + t, 1);
+__global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlGroup a) {
+    const int r0 = blockIdx.x * 64, rows = a.o.plan[LL_PLAN_ROWS];
+    if (r0 >= rows) return;
+    if (blockIdx.y == 0 && threadIdx.x < 64 && r0 + (int)threadIdx.x < rows) {  // whole numbers: any order gives the same
+        const int r = r0 + threadIdx.x, t = a.tok[r];
+        atomicMax(a.slot + t, rows - 1 - r);
+        atomicAdd(a.count + t, 1);
+    }
+    const int lane = threadIdx.x & 63, n0 = r0 + (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
+    typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+    u16x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = n0 + j < rows ? a.o.hidden[(int64_t)(n0 + j) * a.o.H + h] : (uint16_t)0;
+    *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
 // The sums of the tokens of one chunk.  Workgroup (rows blockIdx.x, + gridDim.x, ...; 256 h): the rows with the token
@@ -292,9 +391,10 @@ __global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_beg
     __shared__ int list[1024], listed[4];
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, wave = threadIdx.x >> 6;
     const int h = blockIdx.y * 256 + lane * 8;
-    for (int r = blockIdx.x; r < a.o.N; r += gridDim.x) {
+    const int rows = a.o.plan[LL_PLAN_ROWS];
+    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
         const int t = a.tok[r];
-        if (t < v_begin || t >= v_end || a.slot[t] != a.o.N - 1 - r) continue;
+        if (t < v_begin || t >= v_end || a.slot[t] != rows - 1 - r) continue;
         float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         int left = a.count[t];
         for (int base = r; left > 0; base += 1024) {
@@ -308,7 +408,7 @@ __global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_beg
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int i = base + (int)threadIdx.x * 4 + j;
-                    mine |= (i < a.o.N && a.tok[i] == t) ? 1 << j : 0;
+                    mine |= (i < rows && a.tok[i] == t) ? 1 << j : 0;
                 }
                 const int have = __popc(mine);
                 int before = have;
@@ -338,7 +438,7 @@ __global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_beg
                     const int row = list[i];
                     const float w = a.rest[row];
                     float x[8];
-                    Elem<GRX_BF16>::unpack(*reinterpret_cast<const u32x4*>(a.o.hidden + (int64_t)row * a.o.hidden_ld + h), x);
+                    Elem<GRX_BF16>::unpack(*reinterpret_cast<const u32x4*>(a.o.hidden + (int64_t)row * a.o.H + h), x);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) sum[j] = fmaf(w, x[j], sum[j]);
                 }
@@ -361,9 +461,8 @@ __global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_beg
 // already, so a store is 1 KB in one piece, and both products read it in pieces of 8 KB and more.
 struct LlGrad {
     LlOperands o;
-    int m_tiles, n_tiles;
+    int m_tiles;
     int v_begin, v64;          // first column of the chunk, its width in 64s
-    int n_pad;                 // rows of G
     float k;
     const LlRow* rows;
     float* rest;
@@ -376,18 +475,24 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
-    const int tiles = a.m_tiles * a.n_tiles;
+    const int rows = a.o.plan[LL_PLAN_ROWS], n_pad = (rows + 63) / 64 * 64;  // rows of G
+    const int n_tiles = (rows + BN - 1) / BN, tiles = a.m_tiles * n_tiles;
+    if ((int)blockIdx.x >= tiles) return;
     LlLogits<BN> pipe(lds);
     int tm, tn;
-    mt_tile(blockIdx.x, a.m_tiles, a.n_tiles, tm, tn);
-    ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
+    mt_tile(blockIdx.x, a.m_tiles, n_tiles, tm, tn);
+    ll_begin(pipe, a.o, rows, a.v_begin + tm * MT_BM, tn * BN);
     constexpr int STORES = S::MA * S::NB * 2;
     bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int v0 = a.v_begin + tm * MT_BM, r0 = tn * BN;
         LlRow row[S::NB];
 #pragma unroll
-        for (int n = 0; n < S::NB; ++n) row[n] = a.rows[r0 + (wn * S::NB + n) * 32 + (lane & 31)];
+        for (int n = 0; n < S::NB; ++n) {
+            const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+            row[n] = a.rows[r < rows ? r : rows - 1];
+            if (r >= rows) row[n].tok = -1;  // G is 0 whatever the products are
+        }
         const int v64 = tm * 4;
         typename LlLogits<BN>::Acc acc;
         pipe.clear(acc);
@@ -395,16 +500,16 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
 #pragma unroll
         for (int n = 0; n < S::NB; ++n)  // waited for here, not behind the next copies
             asm volatile("" : "+v"(row[n].m), "+v"(row[n].alpha), "+v"(row[n].beta), "+v"(row[n].at), "+v"(row[n].tok));
-        stored = r0 + (wn + 1) * S::NB * 32 <= a.n_pad;
+        stored = r0 + (wn + 1) * S::NB * 32 <= n_pad;
         if (tile + (int)gridDim.x < tiles) {
-            mt_tile(tile + gridDim.x, a.m_tiles, a.n_tiles, tm, tn);
-            ll_begin(pipe, a.o, a.v_begin + tm * MT_BM, tn * BN);
+            mt_tile(tile + gridDim.x, a.m_tiles, n_tiles, tm, tn);
+            ll_begin(pipe, a.o, rows, a.v_begin + tm * MT_BM, tn * BN);
         }
         const int vw = v0 + wm * S::MA * 32 + 4 * half;
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int n32 = r0 / 32 + wn * S::NB + n;
-            if (n32 * 32 >= a.n_pad) continue;
+            if (n32 * 32 >= n_pad) continue;
             char* const out = a.out + ((int64_t)(n32 >> 1) * a.v64 + v64) * 8192 + (n32 & 1) * 4096 + lane * 16;
             const float m0 = row[n].m, alpha = row[n].alpha, beta = row[n].beta;
 #pragma unroll
@@ -456,70 +561,77 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
 struct LlDh {
     LlOperands o;
     const char* g;
-    int m_tiles, n_tiles, splits, steps, steps_per, v_begin, v64, n_pad;
+    int m_tiles, steps, v_begin, v64;
     int add;                   // 1: go on from what the chunk before left
-    float* slabs;              // [splits][N][H]
+    float* slabs;              // [splits][rows][H]
 };
 
 template <int BN>
 __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(LlDh a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
-    // one XCD takes neighbouring tiles: all h tiles of a few n tiles, which share G
-    const int total = a.splits * a.m_tiles * a.n_tiles, xcd = blockIdx.x & 7;
-    const int id = xcd * (total >> 3) + (xcd < (total & 7) ? xcd : total & 7) + (int)(blockIdx.x >> 3);
-    const int tm = id % a.m_tiles, rest = id / a.m_tiles;
-    const int tn = rest % a.n_tiles, split = rest / a.n_tiles;
-    const int h0 = tm * MT_BM, r0 = tn * BN;
-    const int s0 = split * a.steps_per, s1 = s0 + a.steps_per < a.steps ? s0 + a.steps_per : a.steps;
-    MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong> pipe(lds);
-    typename decltype(pipe)::Acc acc;
-    pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
-               MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u, a.n_pad / 32 - r0 / 32),
-               s1 - s0);
+    const int rows = a.o.plan[LL_PLAN_ROWS], splits = a.o.plan[LL_PLAN_SPLITS], n_tiles = (rows + BN - 1) / BN;
+    const int total = splits * a.m_tiles * n_tiles, steps_per = (a.steps + splits - 1) / splits;
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
-    float* slab = a.slabs + (int64_t)split * a.o.N * a.o.H;
-    pipe.clear(acc);
-    if (a.add) {
+    MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong> pipe(lds);
+    for (int block = blockIdx.x; block < total; block += gridDim.x) {
+        // one XCD takes neighbouring tiles: all h tiles of a few n tiles, which share G
+        const int xcd = block & 7;
+        const int id = xcd * (total >> 3) + (xcd < (total & 7) ? xcd : total & 7) + (block >> 3);
+        const int tm = id % a.m_tiles, rest = id / a.m_tiles;
+        const int tn = rest % n_tiles, split = rest / n_tiles;
+        const int h0 = tm * MT_BM, r0 = tn * BN;
+        const int s0 = split * steps_per, s1 = s0 + steps_per < a.steps ? s0 + steps_per : a.steps;
+        typename decltype(pipe)::Acc acc;
+        pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
+                   MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u,
+                                         (rows + 63) / 64 * 2 - r0 / 32),
+                   s1 - s0);
+        float* slab = a.slabs + (int64_t)split * rows * a.o.H;
+        pipe.clear(acc);
+        if (a.add) {
+#pragma unroll
+            for (int n = 0; n < S::NB; ++n) {
+                const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+                if (r >= rows) continue;
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m) {
+                    const int h = h0 + (wm * S::MA + m) * 32;
+                    if (h < a.o.H) pipe.load(acc, m, n, slab + (int64_t)r * a.o.H + h);
+                }
+            }
+        }
+        pipe.run(acc);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
-            if (r >= a.o.N) continue;
+            if (r >= rows) continue;
 #pragma unroll
-            for (int m = 0; m < S::MA; ++m) {
-                const int h = h0 + (wm * S::MA + m) * 32;
-                if (h < a.o.H) pipe.load(acc, m, n, slab + (int64_t)r * a.o.H + h);
-            }
+            for (int m = 0; m < S::MA; ++m)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
+                    if (h >= a.o.H) continue;
+                    mt_f32x4* o = reinterpret_cast<mt_f32x4*>(slab + (int64_t)r * a.o.H + h);
+                    *o = mt_f32x4{acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
+                }
         }
-    }
-    pipe.run(acc);
-#pragma unroll
-    for (int n = 0; n < S::NB; ++n) {
-        const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
-        if (r >= a.o.N) continue;
-#pragma unroll
-        for (int m = 0; m < S::MA; ++m)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int h = h0 + (wm * S::MA + m) * 32 + 8 * q + 4 * half;
-                if (h >= a.o.H) continue;
-                mt_f32x4* o = reinterpret_cast<mt_f32x4*>(slab + (int64_t)r * a.o.H + h);
-                *o = mt_f32x4{acc[m][n][q * 4], acc[m][n][q * 4 + 1], acc[m][n][q * 4 + 2], acc[m][n][q * 4 + 3]};
-            }
     }
 }
 
 // Sum of the slabs in their order and of what rounding took from G at the row's token, rounded once.
-__global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o, const float* slabs, int splits, const int* tok,
-                                                                    const float* rest, uint16_t* out) {
-    const int64_t n = (int64_t)o.N * o.H, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o, int N, const float* slabs, const int* pos,
+                                                                    const int* tok, const float* rest, uint16_t* out) {
+    const int64_t n = (int64_t)N * o.H, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
-    const int r = (int)(i / o.H), h = (int)(i - (int64_t)r * o.H), t = tok[r];
+    const int row = (int)(i / o.H), h = (int)(i - (int64_t)row * o.H), r = pos[row];
     mt_f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (t >= 0) {
-        const mt_b16x4 w = *reinterpret_cast<const mt_b16x4*>(o.weight + (int64_t)t * o.weight_ld + h);
-        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const mt_f32x4*>(slabs + s * n + i);
+    if (r >= 0) {
+        const int splits = o.plan[LL_PLAN_SPLITS];
+        const int64_t slab = (int64_t)o.plan[LL_PLAN_ROWS] * o.H, at = (int64_t)r * o.H + h;
+        const mt_b16x4 w = *reinterpret_cast<const mt_b16x4*>(o.weight + (int64_t)tok[r] * o.weight_ld + h);
+        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const mt_f32x4*>(slabs + s * slab + at);
         v += rest[r] * __builtin_convertvector(w, mt_f32x4);
     }
     *reinterpret_cast<mt_b16x4*>(out + i) = __builtin_convertvector(v, mt_b16x4);
@@ -530,10 +642,10 @@ struct LlDw {
     const char* copy;
     const char* g;
     int H, V;
-    int m_tiles, n_tiles, steps, v_begin, v64;
-    const int* slot;           // [V] as in LlGroup
-    const float* sums;         // [N][H]: what rounding took from G at the rows' tokens, `last` being row N - 1
-    int last;
+    int m_tiles, n_tiles, v_begin, v64;
+    const int* plan;
+    const int* slot;           // [V], sums [rows][H] as in LlGroup: what rounding took from G at the rows' tokens
+    const float* sums;
     uint16_t* out;             // [V][H]
 };
 
@@ -554,10 +666,10 @@ __device__ __forceinline__ void ll_dw_at(const LlDw& a, int tile, int& h0, int& 
 }
 
 template <bool LINES>
-__device__ __forceinline__ void ll_dw_begin(LlDwPipe<LINES>& pipe, const LlDw& a, int tile, int& h0, int& c0) {
+__device__ __forceinline__ void ll_dw_begin(LlDwPipe<LINES>& pipe, const LlDw& a, int rows, int tile, int& h0, int& c0) {
     ll_dw_at(a, tile, h0, c0);
     pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
-               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), a.steps);
+               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), (rows + MT_BK - 1) / MT_BK);
 }
 
 template <bool LINES>
@@ -566,7 +678,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN;
-    const int tiles = a.m_tiles * a.n_tiles;
+    const int tiles = a.m_tiles * a.n_tiles, rows = a.plan[LL_PLAN_ROWS];
     LlDwPipe<LINES> pipe(lds);
     // LINES: behind the 128 KB of the pipe, 4 KB of each wave
     const uint32_t staging = (uint32_t)(uintptr_t)(mt_lds_void*)lds + 4 * MT_BM * MT_BK * 2 + wave * 4096;
@@ -580,7 +692,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
             slot_next[n] = tile < tiles && v < a.V ? a.slot[v] : -1;
         }
     };
-    ll_dw_begin<LINES>(pipe, a, blockIdx.x, h_next, c_next);
+    ll_dw_begin<LINES>(pipe, a, rows, blockIdx.x, h_next, c_next);
     find(blockIdx.x);
     constexpr int STORES = S::MA * S::NB * 2;
     bool stored = false;  // all STORES of the tile before were made
@@ -594,7 +706,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
 #pragma unroll
         for (int n = 0; n < S::NB; ++n)
             if (__any(slot[n] >= 0)) {  // the sum goes on from what rounding took from G
-                const float* const sums = a.sums + (int64_t)(a.last - slot[n]) * a.H;
+                const float* const sums = a.sums + (int64_t)(rows - 1 - slot[n]) * a.H;
 #pragma unroll
                 for (int m = 0; m < S::MA; ++m) {
                     const int h = h0 + (wm * S::MA + m) * 32;
@@ -605,7 +717,7 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
         find(tile + gridDim.x);
         pipe.template run<STORES>(acc, stored);
         stored = a.v_begin + c0 + (wn + 1) * S::NB * 32 <= a.V && h0 + (wm + 1) * S::MA * 32 <= a.H;
-        if (tile + (int)gridDim.x < tiles) ll_dw_begin<LINES>(pipe, a, tile + gridDim.x, h_next, c_next);
+        if (tile + (int)gridDim.x < tiles) ll_dw_begin<LINES>(pipe, a, rows, tile + gridDim.x, h_next, c_next);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int v = a.v_begin + c0 + (wn * S::NB + n) * 32;
@@ -653,54 +765,59 @@ static int ll_dh_bn(int N) {
     return best;
 }
 
+// Bytes in the order in which they are asked for, each on a multiple of 256.
+struct LlLayout {
+    size_t at = 0;
+    size_t take(int64_t bytes) {
+        const size_t begin = at;
+        at += (size_t)ll_up(bytes, 256);
+        return begin;
+    }
+};
+
+// Rows up to which each workgroup counts those in front of it by itself (8192 rows of H = 2048: 31 us with the copy); more
+// take a launch for it (20,000 rows: 22 us, the copy 36).
+#define LL_COUNT_ROWS (1 << 14)
+static int64_t ll_offsets_bytes(int N) { return N > LL_COUNT_ROWS ? (int64_t)((N + 15) / 16) * 4 : 0; }
+
 struct LlForward {
     int bn, m_tiles, n_tiles, parts;
     int64_t n_pad;
-    size_t partials, weighted, chosen, total;  // byte offsets, total size
+    size_t plan, offsets, tok, row_of, hidden, partials, weighted, chosen, total;  // byte offsets, total size
 };
 
 static int ll_wm(int bn) {
     return bn == 64 ? MtShape<64>::WM : bn == 128 ? MtShape<128>::WM : bn == 192 ? MtShape<192>::WM : MtShape<256>::WM;
 }
 
-static LlForward ll_forward(int N, int V, bool ent) {
+static LlForward ll_forward(int N, int H, int V, bool ent) {
     LlForward f;
     f.m_tiles = (V + MT_BM - 1) / MT_BM;
     f.bn = ll_bn(N, f.m_tiles);
     f.n_tiles = (N + f.bn - 1) / f.bn;
     f.parts = f.m_tiles * ll_wm(f.bn);
     f.n_pad = (int64_t)f.n_tiles * f.bn;
-    f.partials = 0;
-    f.weighted = (size_t)f.parts * f.n_pad * sizeof(float2);
-    f.chosen = f.weighted + (ent ? (size_t)f.parts * f.n_pad * sizeof(float) : 0);
-    f.total = f.chosen + (size_t)N * sizeof(float);
+    LlLayout l;
+    f.plan = l.take(8);
+    f.offsets = l.take(ll_offsets_bytes(N));
+    f.tok = l.take((int64_t)N * 4);
+    f.row_of = l.take((int64_t)N * 4);
+    f.hidden = l.take((int64_t)N * H * 2);
+    f.partials = l.take(f.parts * f.n_pad * sizeof(float2));
+    f.weighted = l.take(ent ? f.parts * f.n_pad * sizeof(float) : 0);
+    f.chosen = l.take((int64_t)N * 4);
+    f.total = l.at;
     return f;
 }
 
 struct LlBackward {
     int bn, n_tiles;           // of d logits
-    int dh_bn, dh_tiles, h_tiles;  // of d hidden
+    int dh_bn, dh_tiles, h_tiles, splits, slab_rows;  // of d hidden
     int64_t n_pad;             // rows of G: whole steps of d weight
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
-    int splits;
-    size_t rows, tok, rest, count, slot, sums, copy, g, slabs, total;
+    size_t plan, offsets, pos, rows, tok, rest, count, slot, hidden, sums, copy, g, slabs, total;
 };
-
-// Splits of d hidden's sum: as many as fill the CUs evenly, each at least eight steps long.
-static int ll_splits(int64_t tiles, int64_t steps) {
-    int best = 1;
-    double best_use = 0.0;
-    for (int s = 1; s <= 64 && (s == 1 || steps / s >= 8); ++s) {
-        const int64_t wgs = tiles * s;
-        const double use = (double)wgs / (double)(ll_up(wgs, LL_CUS));
-        if (use > best_use + 0.04) {
-            best_use = use;
-            best = s;
-        }
-    }
-    return best;
-}
 
 static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     LlBackward b;
@@ -716,29 +833,30 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.n_chunks = (int)((v_pad + b.chunk - 1) / b.chunk);
     b.bn = ll_bn(N, b.chunk / MT_BM);
     b.n_tiles = (N + b.bn - 1) / b.bn;
-    b.splits = ll_splits((int64_t)b.h_tiles * b.dh_tiles, b.chunk / MT_BK);
-    size_t at = 0;
-    const auto take = [&](int64_t bytes) {
-        const size_t begin = at;
-        at += (size_t)ll_up(bytes, 256);
-        return begin;
-    };
-    b.rows = take((int64_t)b.n_tiles * b.bn * sizeof(LlRow));  // tiles may reach past n_pad
-    b.tok = take((int64_t)N * 4);
-    b.rest = take((int64_t)N * 4);
-    b.count = take(want_w ? (int64_t)V * 4 : 0);
-    b.slot = take(want_w ? (int64_t)V * 4 : 0);
-    b.sums = take(want_w ? (int64_t)N * H * 4 : 0);
-    b.copy = at;
-    b.g = b.copy + (want_w ? (size_t)b.n_pad * H * 2 : 0);
-    b.slabs = b.g + (size_t)(b.n_pad * b.chunk * 2);
-    b.total = b.slabs + (want_h ? (size_t)b.splits * N * H * sizeof(float) : 0);
+    const int steps = (int)(b.chunk / MT_BK);
+    b.splits = ll_splits(N, b.dh_bn, b.h_tiles, steps, 1 << 30);
+    b.slab_rows = (int)ll_up(N, b.dh_bn) * b.splits;  // fewer rows take more splits, as far as this room goes
+    LlLayout l;
+    b.plan = l.take(8);
+    b.offsets = l.take(ll_offsets_bytes(N));
+    b.pos = l.take((int64_t)N * 4);
+    b.rows = l.take((int64_t)N * sizeof(LlRow));
+    b.tok = l.take((int64_t)N * 4);
+    b.rest = l.take((int64_t)N * 4);
+    b.hidden = l.take((int64_t)N * H * 2);
+    b.count = l.take(want_w ? (int64_t)V * 4 : 0);
+    b.slot = l.take(want_w ? (int64_t)V * 4 : 0);
+    b.sums = l.take(want_w ? (int64_t)N * H * 4 : 0);
+    b.copy = l.take(want_w ? b.n_pad * H * 2 : 0);
+    b.g = l.take(b.n_pad * b.chunk * 2);
+    b.slabs = l.take(want_h ? (int64_t)b.slab_rows * H * 4 : 0);
+    b.total = l.at;
     return b;
 }
 
 extern "C" size_t grx_lm_token_logps_scratch_bytes(int32_t N, int32_t H, int32_t V, int32_t entropy) {
     if (N <= 0 || V <= 0 || H <= 0 || N > GRX_MAX_TOKEN_ROWS || V > (1 << 24)) return 0;
-    return ll_forward(N, V, entropy != 0).total;
+    return ll_forward(N, H, V, entropy != 0).total;
 }
 
 extern "C" size_t grx_lm_token_logps_backward_scratch_bytes(int32_t N, int32_t H, int32_t V, int32_t want_hidden,
@@ -824,9 +942,26 @@ static int64_t ll_resident(int bn, int64_t tiles) {
         }                                                                         \
     } while (0)
 
-static LlOperands ll_operands(const grx_lm_token_logps_args* p) {
-    return {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, reinterpret_cast<const uint16_t*>(p->hidden),
-            p->hidden_stride, p->N, p->H, p->V};
+template <bool BACK>
+static int ll_compact(LlCompact& c, const grx_lm_token_logps_args* p, int* offsets, hipStream_t stream) {
+    c.hidden = reinterpret_cast<const uint16_t*>(p->hidden);
+    c.hidden_ld = p->hidden_stride;
+    c.ids = p->token_ids;
+    c.N = p->N;
+    c.H = p->H;
+    c.V = p->V;
+    c.stats = reinterpret_cast<float2*>(p->row_stats);
+    c.entropy = p->entropy;
+    const int blocks = (p->N + 15) / 16;
+    if (p->N > LL_COUNT_ROWS) {
+        hipLaunchKernelGGL(lm_logps_offsets_kernel<BACK>, dim3(1), dim3(1024), 0, stream, c, offsets, blocks);
+        GRX_CHECK_HIP(hipGetLastError());
+        c.offsets = offsets;
+    }
+    const int grid = c.slot != nullptr && blocks < 64 ? 64 : blocks;
+    hipLaunchKernelGGL(lm_logps_compact_kernel<BACK>, dim3((unsigned)grid, (unsigned)((p->H + 511) / 512)), dim3(256), 0, stream, c);
+    GRX_CHECK_HIP(hipGetLastError());
+    return GRX_OK;
 }
 
 extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratch, size_t scratch_bytes, void* stream_) {
@@ -835,30 +970,37 @@ extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratc
     if (rc != GRX_OK || p->N == 0) return rc;
     GRX_REQUIRE(p->logps != nullptr, GRX_E_INVALID, "%s: null logps", who);
     const bool ent = p->entropy != nullptr;
-    const LlForward f = ll_forward(p->N, p->V, ent);
+    const LlForward f = ll_forward(p->N, p->H, p->V, ent);
     GRX_REQUIRE(scratch != nullptr && scratch_bytes >= f.total, GRX_E_WORKSPACE, "%s: scratch of %zu bytes, need %zu", who,
                 scratch_bytes, f.total);
     GRX_REQUIRE(((uintptr_t)scratch & 15u) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
     GRX_REQUIRE((int64_t)f.m_tiles * f.n_tiles < (1ll << 31) - LL_CUS * 2, GRX_E_UNSUPPORTED, "%s: too many tiles", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
+    LlCompact c = {};
+    c.to = reinterpret_cast<uint16_t*>(s + f.hidden);
+    c.plan = reinterpret_cast<int*>(s + f.plan);
+    c.tok = reinterpret_cast<int*>(s + f.tok);
+    c.row_of = reinterpret_cast<int*>(s + f.row_of);
+    c.logps = p->logps;
+    const int compact = ll_compact<false>(c, p, reinterpret_cast<int*>(s + f.offsets), stream);
+    if (compact != GRX_OK) return compact;
     LlJoin j;
     LlArgs& a = j.g;
-    a.o = ll_operands(p);
-    a.n_tiles = f.n_tiles;
+    a.o = {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, c.to, c.plan, p->H, p->V};
     a.k = (float)(1.4426950408889634 / (double)p->temperature);
-    a.ids = p->token_ids;
+    a.tok = c.tok;
     a.partials = reinterpret_cast<float2*>(s + f.partials);
     a.weighted = ent ? reinterpret_cast<float*>(s + f.weighted) : nullptr;
     a.n_pad = f.n_pad;
     a.chosen = reinterpret_cast<float*>(s + f.chosen);
-    a.m_begin = 0;
     a.m_tiles = f.m_tiles;
     LL_EACH_ENT(f.bn, ent, lm_logps_kernel, ll_resident(f.bn, (int64_t)a.m_tiles * f.n_tiles), a);
     j.parts = f.parts;
     j.logps = p->logps;
     j.stats = reinterpret_cast<float2*>(p->row_stats);
     j.entropy = p->entropy;
+    j.row_of = c.row_of;
     if (p->N <= 1024) hipLaunchKernelGGL(lm_logps_join_kernel<1>, dim3((unsigned)p->N), dim3(256), 0, stream, j);
     else hipLaunchKernelGGL(lm_logps_join_kernel<16>, dim3((unsigned)((p->N + 15) / 16)), dim3(256), 0, stream, j);
     GRX_CHECK_HIP(hipGetLastError());
@@ -883,54 +1025,56 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     GRX_REQUIRE((int64_t)p->N * p->H / 1024 < (1 << 24), GRX_E_UNSUPPORTED, "%s: more than 2^34 hidden elements", who);
     hipStream_t stream = (hipStream_t)stream_;
     char* s = reinterpret_cast<char*>(scratch);
-    LlRow* rows = reinterpret_cast<LlRow*>(s + b.rows);
-    int* tok = reinterpret_cast<int*>(s + b.tok);
-    float* rest = reinterpret_cast<float*>(s + b.rest);
-    int* slot = reinterpret_cast<int*>(s + b.slot);
-    int* count = reinterpret_cast<int*>(s + b.count);
-    float* sums = reinterpret_cast<float*>(s + b.sums);
-    char* copy = want_w ? s + b.copy : nullptr;
+    LlCompact k = {};
+    k.to = reinterpret_cast<uint16_t*>(s + b.hidden);
+    k.plan = reinterpret_cast<int*>(s + b.plan);
+    k.tok = reinterpret_cast<int*>(s + b.tok);
+    k.g = p->grad_logps;
+    k.h = p->grad_entropy;
+    k.inv_t = (float)(1.0 / (double)p->temperature);
+    k.pos = reinterpret_cast<int*>(s + b.pos);
+    k.rows = reinterpret_cast<LlRow*>(s + b.rows);
+    k.rest = reinterpret_cast<float*>(s + b.rest);
+    k.slot = want_w ? reinterpret_cast<int*>(s + b.slot) : nullptr;
+    k.count = want_w ? reinterpret_cast<int*>(s + b.count) : nullptr;
+    k.dh_bn = b.dh_bn;
+    k.h_tiles = b.h_tiles;
+    k.steps = (int)(b.chunk / MT_BK);
+    k.slab_rows = b.slab_rows;
+    const int compact = ll_compact<true>(k, p, reinterpret_cast<int*>(s + b.offsets), stream);
+    if (compact != GRX_OK) return compact;
+    const LlOperands o = {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, k.to, k.plan, p->H, p->V};
     char* g = s + b.g;
     float* slabs = reinterpret_cast<float*>(s + b.slabs);
-    const LlOperands o = ll_operands(p);
-
-    LlPrep pr = {o, p->token_ids, reinterpret_cast<const float2*>(p->row_stats), p->entropy, p->grad_logps, p->grad_entropy,
-                 (float)(1.0 / (double)p->temperature), rows, tok, rest, copy, slot, count};
-    hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_tiles * b.bn / 64), (unsigned)(want_w ? p->H / 32 : 1)), dim3(256), 0,
-                       stream, pr);
-    GRX_CHECK_HIP(hipGetLastError());
-    const LlGroup gr = {o, tok, rest, slot, count, sums};
+    const LlGroup gr = {o, k.tok, k.rest, k.slot, k.count, reinterpret_cast<float*>(s + b.sums), s + b.copy};
     if (want_w) {
-        hipLaunchKernelGGL(lm_logps_group_kernel, dim3((unsigned)((p->N + 255) / 256)), dim3(256), 0, stream, gr);
+        hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_pad / 64), (unsigned)(p->H / 32)), dim3(256), 0, stream, gr);
         GRX_CHECK_HIP(hipGetLastError());
     }
     for (int c = 0; c < b.n_chunks; ++c) {
         const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
-        LlGrad d = {o, (int)(cols / MT_BM), b.n_tiles, v0, v64, (int)b.n_pad, (float)(1.4426950408889634 / (double)p->temperature),
-                    rows, rest, g};
-        LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * d.n_tiles), d);
+        LlGrad d = {o, (int)(cols / MT_BM), v0, v64, (float)(1.4426950408889634 / (double)p->temperature), k.rows, k.rest, g};
+        LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * b.n_tiles), d);
         if (want_h) {
-            const int steps = (int)(cols / MT_BK);
-            LlDh x = {o, g, b.h_tiles, b.dh_tiles, b.splits, steps, (steps + b.splits - 1) / b.splits, v0, v64, (int)b.n_pad, c > 0,
-                      slabs};
-            LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, b.splits * b.h_tiles * b.dh_tiles, x);
+            LlDh x = {o, g, b.h_tiles, (int)(cols / MT_BK), v0, v64, c > 0, slabs};
+            LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, std::max<int64_t>((int64_t)b.splits * b.h_tiles * b.dh_tiles, LL_CUS), x);
         }
         if (want_w) {
             hipLaunchKernelGGL(lm_logps_rest_kernel, dim3((unsigned)(p->N < 1024 ? p->N : 1024), (unsigned)((p->H + 255) / 256)),
                                dim3(256), 0, stream, gr, v0, (int)(v0 + cols));
             GRX_CHECK_HIP(hipGetLastError());
-            LlDw x = {copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), (int)(b.n_pad / MT_BK), v0, v64, slot, sums, p->N - 1,
+            LlDw x = {gr.copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), v0, v64, k.plan, k.slot, gr.sums,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
             const int64_t wgs = ll_resident(256, (int64_t)x.m_tiles * x.n_tiles);
-            if (x.steps <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
+            if (b.n_pad / MT_BK <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
             else LL_ONE(256, lm_logps_dweight_kernel<false>, wgs, x);
         }
     }
     if (want_h) {
         const int64_t n = (int64_t)p->N * p->H;
-        hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, o, slabs,
-                           b.splits, tok, rest, reinterpret_cast<uint16_t*>(p->grad_hidden));
+        hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, o, p->N, slabs,
+                           k.pos, k.tok, k.rest, reinterpret_cast<uint16_t*>(p->grad_hidden));
         GRX_CHECK_HIP(hipGetLastError());
     }
     return GRX_OK;

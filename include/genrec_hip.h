@@ -749,9 +749,10 @@ GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* str
  * contiguous, 16-byte aligned, all of them (a null one is not computed); the logits' gradient in
  * between is bf16.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
  * H a multiple of 64, at most 2^34 elements of hidden in the backward pass, operand rows 16-byte
- * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row;
- * backward: a chunk of the logits' gradient, up to 1 GB, and 6 to 10 bytes per element of hidden),
- * 16-byte aligned, contents need no initialisation; calls that may overlap must not share it.
+ * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row
+ * and 2 per element of hidden; backward: a chunk of the logits' gradient, up to 1 GB, and about 12
+ * per element of hidden), 16-byte aligned, contents need no initialisation; calls that may overlap
+ * must not share it.
  */
 typedef struct grx_lm_token_logps_args {
     const void* hidden;

@@ -171,6 +171,20 @@ def test_many_rows_of_few_tokens():
     _check(hidden, weight, torch.where(ids >= 0, 256, ids), g)
 
 
+@pytest.mark.parametrize("N,H", [(40, 640), (1403, 64), (2100, 128)])
+def test_rows_that_do_not_count(N, H):
+    """Half the rows padding, at the ends and between; gradients of 0; all but one row out; the wide row in front of 16s."""
+    hidden, weight, ids, g, h = _inputs((N,), H, 2003, seed=N, pad=0.5)
+    _check(hidden, weight, ids, g)
+    g0 = torch.where(torch.rand(g.shape, device=g.device) < 0.5, torch.zeros_like(g), g)
+    _check(hidden, weight, ids, g0, h)
+    _check(hidden, weight, ids, g0, torch.zeros_like(h))
+    for first, last in ((17, N), (0, N - 18), (N - 1, N), (0, 1), (15, 17)):
+        some = torch.full_like(ids, -1)
+        some[first:last] = ids[first:last].abs() % 2003
+        _check(hidden, weight, some, g, h)
+
+
 def test_what_autograd_may_ask():
     hidden, weight, ids, g, h = _inputs((70,), 128, 500, seed=45)
     _, _, dh, dw = _check(hidden, weight, ids, g)

@@ -156,25 +156,30 @@ grx_token_logps_args token_args(const Tensor& logits, const Tensor& ids, double 
     return a;
 }
 
+// stats: where a backward pass wants them; null: in the scratch tensor.
+variable_list token_forward(const Tensor& logits, const Tensor& ids, double temperature, bool entropy, float* stats) {
+    const at::OptionalDeviceGuard guard(logits.device());
+    const int64_t B = ids.size(0), T = ids.size(1);
+    variable_list out = {f32_like({B, T}, logits)};
+    if (entropy) out.push_back(f32_like({B, T}, logits));
+    grx_token_logps_args a = token_args(logits, ids, temperature);
+    const size_t n = api.token_logps_scratch_bytes(B * T, a.V, a.dtype);  // a multiple of 16
+    const Tensor s = scratch(n + (stats ? 0 : B * T * 2 * sizeof(float)), logits.device());
+    a.logps = ptr<float>(out[0]);
+    a.row_stats = stats ? stats : reinterpret_cast<float*>(ptr<char>(s) + n);
+    a.entropy = entropy ? ptr<float>(out[1]) : nullptr;
+    check(api.token_logps(&a, ptr<void>(s), n, stream_on(logits.device())));
+    return out;
+}
+
 struct TokenLogps : Function<TokenLogps> {
     static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& ids, double temperature, bool entropy) {
-        const at::OptionalDeviceGuard guard(logits.device());
-        const int64_t B = ids.size(0), T = ids.size(1);
-        const Tensor logps = f32_like({B, T}, logits), stats = f32_like({B, T, 2}, logits);
-        const Tensor ent = entropy ? f32_like({B, T}, logits) : Tensor();
-        grx_token_logps_args a = token_args(logits, ids, temperature);
-        a.logps = ptr<float>(logps);
-        a.row_stats = ptr<float>(stats);
-        a.entropy = ptr<float>(ent);
-        const size_t n = api.token_logps_scratch_bytes(B * T, a.V, a.dtype);
-        const Tensor s = scratch(n, logits.device());
-        check(api.token_logps(&a, ptr<void>(s), n, stream_on(logits.device())));
-        if (logits.requires_grad()) {
-            ctx->save_for_backward({logits, ids, stats, ent});
-            ctx->saved_data["temperature"] = temperature;
-            ctx->set_materialize_grads(false);
-        }
-        return entropy ? variable_list{logps, ent} : variable_list{logps};
+        const Tensor stats = f32_like({ids.size(0), ids.size(1), 2}, logits);
+        const variable_list out = token_forward(logits, ids, temperature, entropy, ptr<float>(stats));
+        ctx->save_for_backward({logits, ids, stats, entropy ? out[1] : Tensor()});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         const variable_list saved = ctx->get_saved_variables();
@@ -210,6 +215,8 @@ py::object token_logps(const Tensor& logits_, const Tensor& token_ids, double te
     const Tensor ids = token_ids_of(token_ids, logits_.device());
     require_cuda(logits_, "logits");
     const Tensor logits = logits_.size(-1) > 1 && logits_.stride(-1) != 1 ? logits_.contiguous() : logits_;
+    if (!at::GradMode::is_enabled() || !logits.requires_grad())
+        return outputs(token_forward(logits, ids, temperature, entropy, nullptr), token_ids.sizes());
     return outputs(TokenLogps::apply(logits, ids, temperature, entropy), token_ids.sizes());
 }
 
@@ -238,26 +245,31 @@ grx_lm_token_logps_args lm_args(const Tensor& hidden, const Tensor& weight, cons
     return a;
 }
 
+variable_list lm_forward(const Tensor& hidden, const Tensor& weight, const Tensor& ids, double temperature, bool entropy,
+                         const Tensor& stats) {
+    const at::OptionalDeviceGuard guard(hidden.device());
+    const int64_t N = hidden.size(0);
+    variable_list out = {f32_like({N}, hidden)};
+    if (entropy) out.push_back(f32_like({N}, hidden));
+    grx_lm_token_logps_args a = lm_args(hidden, weight, ids, temperature);
+    a.logps = ptr<float>(out[0]);
+    a.row_stats = ptr<float>(stats);
+    a.entropy = entropy ? ptr<float>(out[1]) : nullptr;
+    const size_t n = api.lm_token_logps_scratch_bytes(a.N, a.H, a.V, entropy);
+    const Tensor s = scratch(n, hidden.device());
+    check(api.lm_token_logps(&a, ptr<void>(s), n, stream_on(hidden.device())));
+    return out;
+}
+
 struct LmTokenLogps : Function<LmTokenLogps> {
     static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
                                  double temperature, bool entropy) {
-        const at::OptionalDeviceGuard guard(hidden.device());
-        const int64_t N = hidden.size(0);
-        const Tensor logps = f32_like({N}, hidden), stats = f32_like({N, 2}, hidden);
-        const Tensor ent = entropy ? f32_like({N}, hidden) : Tensor();
-        grx_lm_token_logps_args a = lm_args(hidden, weight, ids, temperature);
-        a.logps = ptr<float>(logps);
-        a.row_stats = ptr<float>(stats);
-        a.entropy = ptr<float>(ent);
-        const size_t n = api.lm_token_logps_scratch_bytes(a.N, a.H, a.V, entropy);
-        const Tensor s = scratch(n, hidden.device());
-        check(api.lm_token_logps(&a, ptr<void>(s), n, stream_on(hidden.device())));
-        if (hidden.requires_grad() || weight.requires_grad()) {
-            ctx->save_for_backward({hidden, weight, ids, stats, ent});
-            ctx->saved_data["temperature"] = temperature;
-            ctx->set_materialize_grads(false);
-        }
-        return entropy ? variable_list{logps, ent} : variable_list{logps};
+        const Tensor stats = f32_like({hidden.size(0), 2}, hidden);
+        const variable_list out = lm_forward(hidden, weight, ids, temperature, entropy, stats);
+        ctx->save_for_backward({hidden, weight, ids, stats, entropy ? out[1] : Tensor()});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->set_materialize_grads(false);
+        return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list incoming) {
         const variable_list saved = ctx->get_saved_variables();
@@ -298,8 +310,10 @@ py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const
     const Tensor ids = token_ids_of(token_ids, hidden.device()).reshape({-1}).contiguous();
     same_device(weight, hidden.device(), "weight");
     require_cuda(hidden, "hidden");
-    const Tensor rows = aligned_rows(hidden.dim() == 2 ? hidden : hidden.reshape({ids.numel(), H}));
-    return outputs(LmTokenLogps::apply(rows, aligned_rows(weight), ids, temperature, entropy), token_ids.sizes());
+    const Tensor rows = aligned_rows(hidden.dim() == 2 ? hidden : hidden.reshape({ids.numel(), H})), w = aligned_rows(weight);
+    if (!at::GradMode::is_enabled() || !(rows.requires_grad() || w.requires_grad()))
+        return outputs(lm_forward(rows, w, ids, temperature, entropy, f32_like({rows.size(0), 2}, rows)), token_ids.sizes());
+    return outputs(LmTokenLogps::apply(rows, w, ids, temperature, entropy), token_ids.sizes());
 }
 
 // ---- the loss ------------------------------------------------------------------------------------------------

@@ -70,6 +70,7 @@ EXPORTED_SYMBOLS = (
     "grx_token_logps_backward",
     "grx_lm_token_logps_scratch_bytes",
     "grx_lm_token_logps_backward_scratch_bytes",
+    "grx_lm_token_logps_kept_bytes",
     "grx_lm_token_logps",
     "grx_lm_token_logps_backward",
     "grx_policy_loss_scratch_bytes",
@@ -279,6 +280,7 @@ class GrxLmTokenLogpsArgs(C.Structure):
         ("grad_entropy", C.c_void_p),
         ("grad_hidden", C.c_void_p),
         ("grad_weight", C.c_void_p),
+        ("kept", C.c_void_p),
     ]
 
 
@@ -433,6 +435,8 @@ def _declare(lib: C.CDLL) -> None:
     lib.grx_lm_token_logps_scratch_bytes.argtypes = [i32, i32, i32, i32]
     lib.grx_lm_token_logps_backward_scratch_bytes.restype = C.c_size_t
     lib.grx_lm_token_logps_backward_scratch_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.grx_lm_token_logps_kept_bytes.restype = C.c_size_t
+    lib.grx_lm_token_logps_kept_bytes.argtypes = [i32, i32]
     lib.grx_lm_token_logps.restype = C.c_int
     lib.grx_lm_token_logps.argtypes = [C.POINTER(GrxLmTokenLogpsArgs), vp, C.c_size_t, vp]
     lib.grx_lm_token_logps_backward.restype = C.c_int

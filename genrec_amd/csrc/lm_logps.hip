@@ -60,10 +60,11 @@ struct LlCompact {
     int* slot;                  // [V] cleared to -1; null: no d weight
     int* count;                 // [V] cleared to 0, with slot
     int dh_bn, h_tiles, steps, slab_rows;  // what splits are chosen by
+    bool kept;                  // rows are as in the forward pass: those whose gradients are 0 keep their places
 };
 
 // What a row needs to turn a product into its gradient: w = 2^((x - m) k), G = w (alpha + beta (x - m) k) + at at the
-// token.
+// token; tok = -1: nothing flows into this row, its G is 0 whatever the products are.
 struct LlRow {
     float m, alpha, beta, at;
     int tok;
@@ -89,10 +90,11 @@ __host__ __device__ static int ll_splits(int rows, int bn, int h_tiles, int step
     return best;
 }
 
-// Backward, rows whose gradients are 0 do not count either.
+// Backward, rows whose gradients are 0 do not count either (but for their places, with kept logits).
+__device__ __forceinline__ bool ll_live(const LlCompact& a, int r) { return (a.g && a.g[r] != 0.f) || (a.h && a.h[r] != 0.f); }
 template <bool BACK>
 __device__ __forceinline__ bool ll_counts(const LlCompact& a, int r) {
-    return r < a.N && a.ids[r] >= 0 && (!BACK || (a.g && a.g[r] != 0.f) || (a.h && a.h[r] != 0.f));
+    return r < a.N && a.ids[r] >= 0 && (!BACK || a.kept || ll_live(a, r));
 }
 
 template <bool BACK>
@@ -154,8 +156,14 @@ __global__ __launch_bounds__(256) void lm_logps_compact_kernel(LlCompact a) {
         const int r = r0 + threadIdx.x;
         if (blockIdx.y == 0 && threadIdx.x < 16 && r < a.N) {
             if constexpr (BACK) {
-                a.pos[r] = counts ? at : -1;
-                if (counts) {
+                const bool live = counts && ll_live(a, r);
+                a.pos[r] = live ? at : -1;
+                if (counts && !live) {
+                    a.rows[at] = {0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}};
+                    a.tok[at] = -1;
+                    a.rest[at] = 0.f;
+                }
+                if (live) {
                     const int64_t id = a.ids[r];
                     const float g = a.g ? a.g[r] : 0.f, h = a.h ? a.h[r] : 0.f;
                     const float2 st = a.stats[r];
@@ -205,6 +213,7 @@ struct LlArgs {
     float* weighted;            // [parts][n_pad], with entropies
     int64_t n_pad;
     float* chosen;              // [rows] logit of the row's token
+    float* kept;                // null, or all products as they lie in the registers: [V / 32][n_pad / 32][4][64 lanes][4]
 };
 
 template <int BN>
@@ -230,8 +239,8 @@ __device__ __forceinline__ float ll_pick(const mt_f32x16 (&acc)[MA][NB], int n, 
 // turns to its own results.  Those stay inside the wave: a row's sums over the wave's columns are one partial.
 // H = 2048, V = 152,640: 8192 rows 3.70 ms (1.38 PFLOP/s; the library's product of these operands alone 3.72 ms), 320
 // rows 227 us, 64 rows and fewer 147 us (4.3 TB/s of weight: rows are fetched 128 bytes at a time).
-template <int BN, bool ENT>
-__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a) {
+template <int BN, bool ENT, bool KEEP>
+__device__ __forceinline__ void ll_forward_tiles(const LlArgs& a) {
     typedef MtShape<BN> S;
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = mt_wave();
@@ -252,7 +261,8 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
         }
         typename LlLogits<BN>::Acc acc;
         pipe.clear(acc);
-        pipe.template run<S::NB>(acc, tile != (int)blockIdx.x);  // the stores of the tile before's sums
+        // the stores of the tile before's sums, and products
+        pipe.template run<S::NB + (KEEP ? S::MA * S::NB * 4 : 0)>(acc, tile != (int)blockIdx.x);
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(id[n]));  // waited for here, not behind the next copies
         if (tile + (int)gridDim.x < tiles) {
@@ -263,6 +273,17 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
 #pragma unroll
         for (int n = 0; n < S::NB; ++n) {
             const int r = r0 + (wn * S::NB + n) * 32 + (lane & 31);
+            if constexpr (KEEP) {
+                const int n32 = r0 / 32 + wn * S::NB + n;
+#pragma unroll
+                for (int m = 0; m < S::MA; ++m) {
+                    float* const to = a.kept + ((int64_t)((v0 >> 5) + wm * S::MA + m) * (a.n_pad >> 5) + n32) * 1024 + lane * 4;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<mt_f32x4*>(to + q * 256) =
+                            mt_f32x4{acc[m][n][4 * q], acc[m][n][4 * q + 1], acc[m][n][4 * q + 2], acc[m][n][4 * q + 3]};
+                }
+            }
             if (v0 + MT_BM > a.o.V) {  // the last tile
 #pragma unroll
                 for (int m = 0; m < S::MA; ++m)
@@ -301,6 +322,16 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a
             }
         }
     }
+}
+
+template <int BN, bool ENT>
+__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_kernel(LlArgs a) {
+    ll_forward_tiles<BN, ENT, false>(a);
+}
+
+template <int BN, bool ENT>
+__global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_keep_kernel(LlArgs a) {
+    ll_forward_tiles<BN, ENT, true>(a);
 }
 
 struct LlJoin {
@@ -375,14 +406,16 @@ __global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlGroup a) {
     if (r0 >= rows) return;
     if (blockIdx.y == 0 && threadIdx.x < 64 && r0 + (int)threadIdx.x < rows) {  // whole numbers: any order gives the same
         const int r = r0 + threadIdx.x, t = a.tok[r];
-        atomicMax(a.slot + t, rows - 1 - r);
-        atomicAdd(a.count + t, 1);
+        if (t >= 0) {
+            atomicMax(a.slot + t, rows - 1 - r);
+            atomicAdd(a.count + t, 1);
+        }
     }
     const int lane = threadIdx.x & 63, n0 = r0 + (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     u16x8 v;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = n0 + j < rows ? a.o.hidden[(int64_t)(n0 + j) * a.o.H + h] : (uint16_t)0;
+    for (int j = 0; j < 8; ++j) v[j] = n0 + j < rows && a.tok[n0 + j] >= 0 ? a.o.hidden[(int64_t)(n0 + j) * a.o.H + h] : (uint16_t)0;
     *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
@@ -557,6 +590,51 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
                     *reinterpret_cast<mt_u32x4*>(out + (v16 >> 2) * 8192 + (v16 & 3) * 1024) = mt_pack8(x, y);
                 }
         }
+    }
+}
+
+// G from the products that the forward pass kept: a wave takes blocks of 32 v x 32 n.
+template <bool ENT>
+__global__ __launch_bounds__(256) void lm_logps_kept_kernel(LlGrad a, const float* kept, int n32s) {
+    const int lane = threadIdx.x & 63, wave = mt_wave(), half = lane >> 5;
+    const int n32 = blockIdx.y, rows = a.o.plan[LL_PLAN_ROWS], r = n32 * 32 + (lane & 31);
+    if ((n32 & ~1) * 32 >= rows) return;  // G has whole pairs of blocks
+    LlRow row = a.rows[r < rows ? r : rows - 1];
+    if (r >= rows) row.tok = -1;
+    const int v32 = blockIdx.x * 4 + wave;  // of the chunk
+    if (v32 >= a.m_tiles * 8) return;
+    const int vw = a.v_begin + v32 * 32 + 4 * half;
+    float x[16];
+    const float* const from = kept + ((int64_t)((a.v_begin >> 5) + v32) * n32s + n32) * 1024 + lane * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const mt_f32x4 v = __builtin_nontemporal_load(reinterpret_cast<const mt_f32x4*>(from + q * 256));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * q + j] = v[j];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const float t = (x[e] - row.m) * a.k;
+        x[e] = fast_exp2(t) * (ENT ? fmaf(row.beta, fmaxf(t, LL_FLOOR), row.alpha) : row.alpha);
+    }
+    const int off = row.tok - vw;  // runs of four entries, every eight
+    if (row.tok >= 0 && off >= 0 && off < 32 && (off & 4) == 0) {
+        const int at = (off >> 3) * 4 + (off & 3);
+        float whole = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (e == at) whole = x[e] += row.at;
+        a.rest[r] = whole - (float)(__bf16)whole;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (row.tok < 0 || vw + (e & 3) + 8 * (e >> 2) >= a.o.V) x[e] = 0.f;
+    char* const out = a.out + ((int64_t)(n32 >> 1) * a.v64 + (v32 >> 1)) * 8192 + (n32 & 1) * 4096 + (v32 & 1) * 2048 + lane * 16;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const mt_f32x4 lo = {x[8 * q], x[8 * q + 1], x[8 * q + 2], x[8 * q + 3]};
+        const mt_f32x4 hi = {x[8 * q + 4], x[8 * q + 5], x[8 * q + 6], x[8 * q + 7]};
+        *reinterpret_cast<mt_u32x4*>(out + q * 1024) = mt_pack8(lo, hi);
     }
 }
 
@@ -871,6 +949,16 @@ extern "C" size_t grx_lm_token_logps_backward_scratch_bytes(int32_t N, int32_t H
     return ll_backward(N, H, V, want_hidden != 0, want_weight != 0).total;
 }
 
+// The products of few rows are kept for the backward pass, in fp32, where they fit the cache behind the L2s (256 MB).
+#define LL_KEPT_BYTES (256ll << 20)
+static int64_t ll_kept_bytes(const LlForward& f) { return (int64_t)f.m_tiles * MT_BM * f.n_pad * 4; }
+
+extern "C" size_t grx_lm_token_logps_kept_bytes(int32_t N, int32_t V) {
+    if (N <= 0 || V <= 0 || N > GRX_MAX_TOKEN_ROWS || V > (1 << 24)) return 0;
+    const int64_t bytes = ll_kept_bytes(ll_forward(N, 64, V, false));
+    return bytes <= LL_KEPT_BYTES ? (size_t)bytes : 0;
+}
+
 static int ll_check(const char* who, const grx_lm_token_logps_args* p) {
     GRX_REQUIRE(p != nullptr, GRX_E_INVALID, "%s: null args", who);
     GRX_REQUIRE(p->N >= 0 && p->V >= 1 && p->H >= 1, GRX_E_INVALID, "%s: bad shape", who);
@@ -885,8 +973,10 @@ static int ll_check(const char* who, const grx_lm_token_logps_args* p) {
     if (p->N == 0) return GRX_OK;
     GRX_REQUIRE(p->hidden != nullptr && p->weight != nullptr && p->token_ids != nullptr && p->row_stats != nullptr, GRX_E_INVALID,
                 "%s: null buffer", who);
-    GRX_REQUIRE((((uintptr_t)p->hidden | (uintptr_t)p->weight) & 15u) == 0 && ((uintptr_t)p->row_stats & 7u) == 0, GRX_E_INVALID,
+    GRX_REQUIRE((((uintptr_t)p->hidden | (uintptr_t)p->weight | (uintptr_t)p->kept) & 15u) == 0 && ((uintptr_t)p->row_stats & 7u) == 0, GRX_E_INVALID,
                 "%s: misaligned buffer", who);
+    GRX_REQUIRE(p->kept == nullptr || grx_lm_token_logps_kept_bytes(p->N, p->V) > 0, GRX_E_UNSUPPORTED,
+                "%s: more products than can be kept", who);
     return GRX_OK;
 }
 
@@ -1001,7 +1091,10 @@ extern "C" int grx_lm_token_logps(const grx_lm_token_logps_args* p, void* scratc
     a.n_pad = f.n_pad;
     a.chosen = reinterpret_cast<float*>(s + f.chosen);
     a.m_tiles = f.m_tiles;
-    LL_EACH_ENT(f.bn, ent, lm_logps_kernel, ll_resident(f.bn, (int64_t)a.m_tiles * f.n_tiles), a);
+    a.kept = p->kept;
+    const int64_t wgs = ll_resident(f.bn, (int64_t)a.m_tiles * f.n_tiles);
+    if (p->kept) LL_EACH_ENT(f.bn, ent, lm_logps_keep_kernel, wgs, a);
+    else LL_EACH_ENT(f.bn, ent, lm_logps_kernel, wgs, a);
     j.parts = f.parts;
     j.logps = p->logps;
     j.stats = reinterpret_cast<float2*>(p->row_stats);
@@ -1047,6 +1140,7 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     k.h_tiles = b.h_tiles;
     k.steps = (int)(b.chunk / MT_BK);
     k.slab_rows = b.slab_rows;
+    k.kept = p->kept != nullptr;
     const int compact = ll_compact<true>(k, p, reinterpret_cast<int*>(s + b.offsets), stream);
     if (compact != GRX_OK) return compact;
     const LlOperands o = {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, k.to, k.plan, p->H, p->V};
@@ -1061,7 +1155,15 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
         const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
         LlGrad d = {o, (int)(cols / MT_BM), v0, v64, (float)(1.4426950408889634 / (double)p->temperature), k.rows, k.rest, g};
-        LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * b.n_tiles), d);
+        if (p->kept) {
+            const int n32s = (int)(ll_forward(p->N, p->H, p->V, false).n_pad / 32);
+            const dim3 grid((unsigned)(d.m_tiles * 2), (unsigned)(b.n_pad / 32));
+            if (ent) hipLaunchKernelGGL(lm_logps_kept_kernel<true>, grid, dim3(256), 0, stream, d, p->kept, n32s);
+            else hipLaunchKernelGGL(lm_logps_kept_kernel<false>, grid, dim3(256), 0, stream, d, p->kept, n32s);
+            GRX_CHECK_HIP(hipGetLastError());
+        } else {
+            LL_EACH_ENT(b.bn, ent, lm_logps_dlogits_kernel, ll_resident(b.bn, (int64_t)d.m_tiles * b.n_tiles), d);
+        }
         if (want_h) {
             LlDh x = {o, g, b.h_tiles, (int)(cols / MT_BK), v0, v64, c > 0, slabs};
             LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, std::max<int64_t>((int64_t)b.splits * b.h_tiles * b.dh_tiles, LL_CUS), x);

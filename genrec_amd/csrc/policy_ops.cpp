@@ -29,6 +29,7 @@ struct Api {
     decltype(&grx_token_logps_backward) token_logps_backward;
     decltype(&grx_lm_token_logps_scratch_bytes) lm_token_logps_scratch_bytes;
     decltype(&grx_lm_token_logps_backward_scratch_bytes) lm_token_logps_backward_scratch_bytes;
+    decltype(&grx_lm_token_logps_kept_bytes) lm_token_logps_kept_bytes;
     decltype(&grx_lm_token_logps) lm_token_logps;
     decltype(&grx_lm_token_logps_backward) lm_token_logps_backward;
     decltype(&grx_policy_loss_scratch_bytes) policy_loss_scratch_bytes;
@@ -246,7 +247,7 @@ grx_lm_token_logps_args lm_args(const Tensor& hidden, const Tensor& weight, cons
 }
 
 variable_list lm_forward(const Tensor& hidden, const Tensor& weight, const Tensor& ids, double temperature, bool entropy,
-                         const Tensor& stats) {
+                         const Tensor& stats, const Tensor& kept) {
     const at::OptionalDeviceGuard guard(hidden.device());
     const int64_t N = hidden.size(0);
     variable_list out = {f32_like({N}, hidden)};
@@ -255,6 +256,7 @@ variable_list lm_forward(const Tensor& hidden, const Tensor& weight, const Tenso
     a.logps = ptr<float>(out[0]);
     a.row_stats = ptr<float>(stats);
     a.entropy = entropy ? ptr<float>(out[1]) : nullptr;
+    a.kept = ptr<float>(kept);
     const size_t n = api.lm_token_logps_scratch_bytes(a.N, a.H, a.V, entropy);
     const Tensor s = scratch(n, hidden.device());
     check(api.lm_token_logps(&a, ptr<void>(s), n, stream_on(hidden.device())));
@@ -265,8 +267,10 @@ struct LmTokenLogps : Function<LmTokenLogps> {
     static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
                                  double temperature, bool entropy) {
         const Tensor stats = f32_like({hidden.size(0), 2}, hidden);
-        const variable_list out = lm_forward(hidden, weight, ids, temperature, entropy, stats);
-        ctx->save_for_backward({hidden, weight, ids, stats, entropy ? out[1] : Tensor()});
+        const size_t n = api.lm_token_logps_kept_bytes((int32_t)hidden.size(0), (int32_t)weight.size(0));
+        const Tensor kept = scratch(n, hidden.device());
+        const variable_list out = lm_forward(hidden, weight, ids, temperature, entropy, stats, kept);
+        ctx->save_for_backward({hidden, weight, ids, stats, entropy ? out[1] : Tensor(), kept});
         ctx->saved_data["temperature"] = temperature;
         ctx->set_materialize_grads(false);
         return out;
@@ -286,6 +290,7 @@ struct LmTokenLogps : Function<LmTokenLogps> {
         a.entropy = ptr<float>(ent);
         a.grad_logps = ptr<float>(g);
         a.grad_entropy = ptr<float>(h);
+        a.kept = ptr<float>(saved[5]);
         a.grad_hidden = ptr<void>(grad_h);
         a.grad_weight = ptr<void>(grad_w);
         const size_t n = api.lm_token_logps_backward_scratch_bytes(a.N, a.H, a.V, want_h, want_w);
@@ -312,7 +317,7 @@ py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const
     require_cuda(hidden, "hidden");
     const Tensor rows = aligned_rows(hidden.dim() == 2 ? hidden : hidden.reshape({ids.numel(), H})), w = aligned_rows(weight);
     if (!at::GradMode::is_enabled() || !(rows.requires_grad() || w.requires_grad()))
-        return outputs(lm_forward(rows, w, ids, temperature, entropy, f32_like({rows.size(0), 2}, rows)), token_ids.sizes());
+        return outputs(lm_forward(rows, w, ids, temperature, entropy, f32_like({rows.size(0), 2}, rows), Tensor()), token_ids.sizes());
     return outputs(LmTokenLogps::apply(rows, w, ids, temperature, entropy), token_ids.sizes());
 }
 
@@ -447,6 +452,7 @@ void bind(py::object error, py::dict addresses) {
     GRX_BIND(token_logps_backward);
     GRX_BIND(lm_token_logps_scratch_bytes);
     GRX_BIND(lm_token_logps_backward_scratch_bytes);
+    GRX_BIND(lm_token_logps_kept_bytes);
     GRX_BIND(lm_token_logps);
     GRX_BIND(lm_token_logps_backward);
     GRX_BIND(policy_loss_scratch_bytes);

@@ -65,7 +65,8 @@ def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: t
     ``hidden`` [B, T, H] or [N, H] and ``weight`` [V, H] (``lm_head.weight``, no bias), bf16, H a multiple of 64, on
     the GPU; ``token_ids`` [B, T] or [N], negative for padding.  Differentiable in both; a frozen weight costs
     nothing.  The logits' gradient passes through bf16 on its way to the two products, as it does under autograd.
-    Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Scratch
+    Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Up to 256 MB
+    of products (fp32, a few hundred rows) are kept for the backward pass, more are formed again.  Scratch
     tensors: about V / 16 bytes a row forward; up to 1 GB and 12 bytes per element of ``hidden`` backward.  A pass recorded into a HIP graph needs leaves of its own (``detach().requires_grad_()`` inside
     the recording)."""
     return (_ops_module or _ops()).lm_head_token_logps(hidden, weight, token_ids, temperature, return_entropy)

@@ -165,6 +165,8 @@ def test_lm_head_token_logps_refuses(hidden, weight, ids, error, match):
     (dict(weight_stride=56), -1, b"operand rows"),
     (dict(weight=None), -1, b"null buffer"),
     (dict(hidden=0x10008), -1, b"misaligned"),
+    (dict(kept=0x70004), -1, b"misaligned"),
+    (dict(N=5000, V=152640, kept=0x70000), -3, b"kept"),
 ])
 def test_lm_head_c_entries_refuse(over, code, match):
     lib = _lib.lib()

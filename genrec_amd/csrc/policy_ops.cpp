@@ -265,10 +265,10 @@ variable_list lm_forward(const Tensor& hidden, const Tensor& weight, const Tenso
 
 struct LmTokenLogps : Function<LmTokenLogps> {
     static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
-                                 double temperature, bool entropy) {
+                                 double temperature, bool entropy, int64_t keep_bytes) {
         const Tensor stats = f32_like({hidden.size(0), 2}, hidden);
         const size_t n = api.lm_token_logps_kept_bytes((int32_t)hidden.size(0), (int32_t)weight.size(0));
-        const Tensor kept = scratch(n, hidden.device());
+        const Tensor kept = (int64_t)n <= keep_bytes ? scratch(n, hidden.device()) : Tensor();
         const variable_list out = lm_forward(hidden, weight, ids, temperature, entropy, stats, kept);
         ctx->save_for_backward({hidden, weight, ids, stats, entropy ? out[1] : Tensor(), kept});
         ctx->saved_data["temperature"] = temperature;
@@ -296,12 +296,14 @@ struct LmTokenLogps : Function<LmTokenLogps> {
         const size_t n = api.lm_token_logps_backward_scratch_bytes(a.N, a.H, a.V, want_h, want_w);
         const Tensor s = scratch(n, hidden.device());
         check(api.lm_token_logps_backward(&a, ptr<void>(s), n, stream_on(hidden.device())));
-        return once(incoming, {grad_h, grad_w, Tensor(), Tensor(), Tensor()});
+        return once(incoming, {grad_h, grad_w, Tensor(), Tensor(), Tensor(), Tensor()});
     }
 };
 
-py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const Tensor& token_ids, double temperature, bool entropy) {
+py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const Tensor& token_ids, double temperature, bool entropy,
+                               int64_t keep_bytes) {
     temperature = temperature_of(temperature);
+    TORCH_CHECK_VALUE(keep_bytes >= 0, "keep_bytes must not be negative, got ", keep_bytes);
     TORCH_CHECK_TYPE(hidden.scalar_type() == at::kBFloat16 && weight.scalar_type() == at::kBFloat16,
                      "hidden states and weight must be bfloat16, got ", hidden.scalar_type(), " and ", weight.scalar_type());
     TORCH_CHECK_VALUE((hidden.dim() == 2 || hidden.dim() == 3) && token_ids.sizes() == hidden.sizes().slice(0, hidden.dim() - 1),
@@ -318,7 +320,7 @@ py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const
     const Tensor rows = aligned_rows(hidden.dim() == 2 ? hidden : hidden.reshape({ids.numel(), H})), w = aligned_rows(weight);
     if (!at::GradMode::is_enabled() || !(rows.requires_grad() || w.requires_grad()))
         return outputs(lm_forward(rows, w, ids, temperature, entropy, f32_like({rows.size(0), 2}, rows), Tensor()), token_ids.sizes());
-    return outputs(LmTokenLogps::apply(rows, w, ids, temperature, entropy), token_ids.sizes());
+    return outputs(LmTokenLogps::apply(rows, w, ids, temperature, entropy, keep_bytes), token_ids.sizes());
 }
 
 // ---- the loss ------------------------------------------------------------------------------------------------

@@ -58,18 +58,20 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
 
 
 def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor, temperature: float = 1.0,
-                        return_entropy: bool = False):
-    """:func:`token_logps` of ``logits = hidden @ weight.T`` without the logits: the product runs on the matrix cores
-    and is consumed tile by tile, forward and backward (the backward pass forms it again).
+                        return_entropy: bool = False, keep_bytes: int = 8 << 30):
+    """:func:`token_logps` of ``logits = hidden @ weight.T``: the product runs on the matrix cores and is consumed tile
+    by tile, forward and backward.  Where a backward pass follows and the products take up to ``keep_bytes`` in fp32
+    (N x V x 4 and the tiles' margins), they are kept for it; otherwise, with 0 always, it forms them again and no
+    logits are ever held (8192 rows of a vocabulary of 152,640, H = 2048: 5 GB kept, 13.6 ms with both gradients;
+    nothing kept, 15.4 ms).
 
     ``hidden`` [B, T, H] or [N, H] and ``weight`` [V, H] (``lm_head.weight``, no bias), bf16, H a multiple of 64, on
     the GPU; ``token_ids`` [B, T] or [N], negative for padding.  Differentiable in both; a frozen weight costs
     nothing.  The logits' gradient passes through bf16 on its way to the two products, as it does under autograd.
-    Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Up to 256 MB
-    of products (fp32, a few hundred rows) are kept for the backward pass, more are formed again.  Scratch
-    tensors: about V / 16 bytes a row forward; up to 1 GB and 12 bytes per element of ``hidden`` backward.  A pass recorded into a HIP graph needs leaves of its own (``detach().requires_grad_()`` inside
-    the recording)."""
-    return (_ops_module or _ops()).lm_head_token_logps(hidden, weight, token_ids, temperature, return_entropy)
+    Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Scratch
+    tensors: about V / 16 bytes a row forward; up to 1 GB and 12 bytes per element of ``hidden`` backward.  A pass
+    recorded into a HIP graph needs leaves of its own (``detach().requires_grad_()`` inside the recording)."""
+    return (_ops_module or _ops()).lm_head_token_logps(hidden, weight, token_ids, temperature, return_entropy, keep_bytes)
 
 
 class PolicyLoss:

@@ -752,9 +752,9 @@ GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* str
  * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row
  * and 2 per element of hidden; backward: a chunk of the logits' gradient, up to 1 GB, and about 12
  * per element of hidden), 16-byte aligned, contents need no initialisation; calls that may overlap
- * must not share it.  kept (grx_lm_token_logps_kept_bytes(N, V) bytes, 16-byte aligned; that is 0
- * where the products are more than 256 MB: pass null): the forward pass leaves its products there,
- * and the backward pass of the same N, V and token ids takes them instead of forming them again.
+ * must not share it.  kept (or null; grx_lm_token_logps_kept_bytes(N, V) bytes, 16-byte aligned, up
+ * to 2^20 rows): the forward pass leaves its products there in fp32, and the backward pass of the
+ * same N, V and token ids takes them instead of forming them again.
  */
 typedef struct grx_lm_token_logps_args {
     const void* hidden;

@@ -55,12 +55,23 @@ def _definition(hidden, weight, ids, temperature, g, h):
 
 
 def _check(hidden, weight, ids, g, h=None, temperature=1.0):
+    """Once with the products kept for the backward pass (the results are returned), once with them formed again."""
     x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
-    made = lm_head_token_logps(x, w, ids, temperature, return_entropy=h is not None)
-    logps, ent = made if h is not None else (made, None)
-    assert logps.dtype == torch.float32 and logps.shape == ids.shape
-    dh, dw = torch.autograd.grad([logps] + ([ent] if h is not None else []), [x, w], [g] + ([h] if h is not None else []))
-    want, want_ent, G, flat, wd, err, p, lp = _definition(hidden, weight, ids, temperature, g, h)
+    made = []
+    for keep in ({}, {"keep_bytes": 0}):
+        out = lm_head_token_logps(x, w, ids, temperature, return_entropy=h is not None, **keep)
+        logps, ent = out if h is not None else (out, None)
+        assert logps.dtype == torch.float32 and logps.shape == ids.shape
+        dh, dw = torch.autograd.grad([logps] + ([ent] if h is not None else []), [x, w], [g] + ([h] if h is not None else []))
+        made.append((logps.detach(), None if ent is None else ent.detach(), dh, dw))
+    want = _definition(hidden, weight, ids, temperature, g, h)
+    for m in made:
+        _compare(*m, want, hidden, weight, ids, g, h, temperature)
+    return made[0]
+
+
+def _compare(logps, ent, dh, dw, definition, hidden, weight, ids, g, h, temperature):
+    want, want_ent, G, flat, wd, err, p, lp = definition
     N, V = G.shape
     rel = (V / 256 + 160) * U
     assert ((logps.double().reshape(-1) - want).abs() <= 2 * err + rel + 6 * U * want.abs()).all()
@@ -84,7 +95,6 @@ def _check(hidden, weight, ids, g, h=None, temperature=1.0):
     off = (dw.double() - want_w).abs() - HALF * want_w.abs() - bound_w * (1 + HALF) - 1e-37
     assert (off <= 0).all(), float(off.max())
     assert (dh[ids < 0] == 0).all()
-    return logps, ent, dh, dw
 
 
 # row tiles of 64, 128 and 256, tails of both axes, H below and above one tile, several chunks of columns are below
@@ -179,6 +189,12 @@ def test_rows_that_do_not_count(N, H):
     g0 = torch.where(torch.rand(g.shape, device=g.device) < 0.5, torch.zeros_like(g), g)
     _check(hidden, weight, ids, g0, h)
     _check(hidden, weight, ids, g0, torch.zeros_like(h))
+    keeps = ({}, {"keep_bytes": 0})
+    clean, dirty = [], torch.where((g0 == 0)[:, None], torch.full_like(hidden, math.nan), hidden)
+    for kw in keeps + keeps:  # whatever the rows without a gradient hold
+        x, w = (hidden if len(clean) < 2 else dirty).detach().requires_grad_(), weight.detach().requires_grad_()
+        clean.append(torch.autograd.grad(lm_head_token_logps(x, w, ids, **kw), [x, w], g0))
+    assert all(torch.equal(a, b) for i in (0, 1) for a, b in zip(clean[i], clean[i + 2]))
     for first, last in ((17, N), (0, N - 18), (N - 1, N), (0, 1), (15, 17)):
         some = torch.full_like(ids, -1)
         some[first:last] = ids[first:last].abs() % 2003
@@ -233,11 +249,12 @@ def test_agrees_with_the_logits_form():
     assert (a[0] - b[0]).abs().max() <= 4 * tol + 1e-5 and (a[1] - b[1]).abs().max() <= 40 * tol + 1e-4
 
 
-def test_several_chunks_of_columns(monkeypatch):
+@pytest.mark.parametrize("keep_bytes", [8 << 30, 0])
+def test_several_chunks_of_columns(keep_bytes):
     """More rows than one chunk of the logits' gradient holds at this vocabulary: 16,000 x 40,000."""
     hidden, weight, ids, g, h = _inputs((16000,), 64, 40000, seed=7)
     x, w = hidden.detach().requires_grad_(), weight.detach().requires_grad_()
-    lp = lm_head_token_logps(x, w, ids)
+    lp = lm_head_token_logps(x, w, ids, keep_bytes=keep_bytes)
     dh, dw = torch.autograd.grad(lp, [x, w], [g])
     rows = torch.arange(0, 16000, 61, device=ids.device)
     want, _, G, flat, wd, err, p, lpa = _definition(hidden[rows], weight, ids[rows], 1.0, g[rows], None)

@@ -155,6 +155,11 @@ def test_lm_head_token_logps_refuses(hidden, weight, ids, error, match):
         policy.lm_head_token_logps(hidden, weight, ids)
 
 
+def test_lm_head_token_logps_refuses_a_negative_budget():
+    with pytest.raises(ValueError, match="keep_bytes"):
+        policy.lm_head_token_logps(_bf(2, 64), _bf(8, 64), torch.zeros(2, dtype=torch.int64), keep_bytes=-1)
+
+
 @pytest.mark.parametrize("over,code,match", [
     (dict(V=0), -1, b"bad shape"),
     (dict(H=96), -3, b"multiple of 64"),
@@ -166,7 +171,7 @@ def test_lm_head_token_logps_refuses(hidden, weight, ids, error, match):
     (dict(weight=None), -1, b"null buffer"),
     (dict(hidden=0x10008), -1, b"misaligned"),
     (dict(kept=0x70004), -1, b"misaligned"),
-    (dict(N=5000, V=152640, kept=0x70000), -3, b"kept"),
+    (dict(N=(1 << 20) + 1, kept=0x70000), -3, b"kept"),
 ])
 def test_lm_head_c_entries_refuse(over, code, match):
     lib = _lib.lib()

@@ -780,6 +780,8 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
     };
     ll_dw_begin<LINES>(pipe, a, rows, blockIdx.x, h_next, c_next);
     find(blockIdx.x);
+#pragma unroll
+    for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(slot_next[n]));
     constexpr int STORES = S::MA * S::NB * 2;
     bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -802,6 +804,8 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
             }
         find(tile + gridDim.x);
         pipe.template run<STORES>(acc, stored);
+#pragma unroll
+        for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(slot_next[n]));  // waited for here, not behind the stores
         stored = a.v_begin + c0 + (wn + 1) * S::NB * 32 <= a.V && h0 + (wm + 1) * S::MA * 32 <= a.H;
         if (tile + (int)gridDim.x < tiles) ll_dw_begin<LINES>(pipe, a, rows, tile + gridDim.x, h_next, c_next);
 #pragma unroll

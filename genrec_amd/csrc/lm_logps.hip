@@ -723,7 +723,7 @@ __global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o
 
 // d weight of the chunk: C[v][h] = sum over the rows of G[n][v] hidden[n][h].  8192 rows: 3.97 ms (1.29 PFLOP/s; the
 // library's product 4.40 ms).  At few rows the stores come on top of the products (a wave's copies are counted together
-// with its stores, so the copies of a tile's third step wait for the stores of the tile before): 320 rows 316 us.
+// with its stores, so the copies of a tile's third step wait for the stores of the tile before): 320 rows 312 us.
 struct LlDw {
     const char* copy;
     const char* g;
@@ -737,8 +737,8 @@ struct LlDw {
 
 // LINES: two buffers of either operand, and the LDS left holds the results on their way to whole lines of 128 bytes;
 // otherwise three buffers of G and stores of the 16 bytes that a lane holds.  Up to LL_LINES_STEPS steps the stores weigh
-// more: at H = 2048 and V = 152,640 (625 MB to write) 64 rows take 155 us against 208, 512 rows 419 against 464, 1024 rows
-// 675 against 677, 2048 rows 1221 against 1177, 4096 rows 2280 against 2176.
+// more: at H = 2048 and V = 152,640 (625 MB to write) 64 rows take 140 us against 199, 512 rows 405 against 443, 1024 rows
+// 645 against 665, 1536 rows 911 against 896, 4096 rows 2160 against 2080.
 #define LL_LINES_STEPS 16
 template <bool LINES>
 using LlDwPipe = MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, !LINES, LINES ? 2 : 3>;

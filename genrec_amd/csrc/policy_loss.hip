@@ -105,7 +105,8 @@ __device__ __forceinline__ PlTerm pl_term(const PlArgs& a, double d, float w, fl
     return r;
 }
 
-// What the call returns, from the sums over all tokens.  global: the factor that the stored gradient still lacks.
+// What the call returns, from the sums over all tokens.  stats[3]: the factor that the stored gradient still lacks, 1
+// where the weight was known before (it is in the gradient then, rounded once with it).
 __device__ __forceinline__ void pl_finish(const PlArgs& a, const double* s) {
     const double tokens = s[4] > 1.0 ? s[4] : 1.0;
     const double global = a.constant != 0.0 ? a.constant : 1.0 / tokens;
@@ -113,7 +114,7 @@ __device__ __forceinline__ void pl_finish(const PlArgs& a, const double* s) {
     a.p.stats[0] = (float)(s[1] / tokens);
     a.p.stats[1] = (float)(s[2] / tokens);
     a.p.stats[2] = (float)(s[3] / tokens);
-    a.p.stats[3] = (float)global;
+    a.p.stats[3] = a.constant != 0.0 ? 1.f : (float)global;
 }
 
 __device__ __forceinline__ void pl_count(PlShare& s, const PlTerm& k) {
@@ -180,6 +181,7 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
             }
         }
         double row_w = 1.0, inv_n = 1.0, row_d = 0.0;
+        const double known = a.constant != 0.0 ? a.constant : 1.0;
         float seq_w = 1.f;
         if (p.row_mean || p.sequence_level) {
             double n = 0.0, d = 0.0;
@@ -222,7 +224,7 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
         for (int e = 0; e < E; ++e) {
             const int t = lane + e * LANES;
             if (t < p.T)
-                grad[t] = valid[e] ? (float)(row_w * ((p.sequence_level ? slope : (double)x[e]) + (double)old[e])) : 0.f;
+                grad[t] = valid[e] ? (float)(row_w * known * ((p.sequence_level ? slope : (double)x[e]) + (double)old[e])) : 0.f;
         }
     }
     pl_totals<THREADS>(a, share, lds);
@@ -241,6 +243,7 @@ __global__ __launch_bounds__(LANES) void policy_loss_kernel(PlArgs a) {
         const float* ref = p.ref_logps ? p.ref_logps + r * p.ref_stride : nullptr;
         float* grad = p.unit_grad ? p.unit_grad + r * p.T : nullptr;
         double row_w = 1.0, row_d = 0.0, inv_n = 1.0;
+        const double known = a.constant != 0.0 ? a.constant : 1.0;
         if (p.row_mean || p.sequence_level) {
             double n = 0.0, d = 0.0;
             for (int t = lane; t < p.T; t += LANES)
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(LANES) void policy_loss_kernel(PlArgs a) {
                 if (pass == 1) {
                     float rise = 0.f;
                     if (p.beta != 0.f) pl_kl(q, rise);
-                    grad[t] = (float)(row_w * (seq_slope + (double)(-p.beta * rise)));
+                    grad[t] = (float)(row_w * known * (seq_slope + (double)(-p.beta * rise)));
                     continue;
                 }
                 double d = row_d;
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(LANES) void policy_loss_kernel(PlArgs a) {
                 if (p.sequence_level)
                     seq_slope += (double)k.slope;
                 else
-                    grad[t] = (float)(row_w * ((double)k.slope + (double)k.kl_slope));
+                    grad[t] = (float)(row_w * known * ((double)k.slope + (double)k.kl_slope));
             }
         }
         share.total += row_w * share.loss;

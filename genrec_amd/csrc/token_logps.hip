@@ -15,6 +15,7 @@
 
 #define TL_THREADS 256
 #define TL_WAVES (TL_THREADS / GRX_WAVE)
+#define TL_WIDE 1024
 #define TL_UNROLL 4          // 16-byte loads in flight per thread
 #define TL_MAX_PARTS 64
 // Rows are split until there are this many workgroups (eight of them run on a CU): 1280 rows, 41 % of them padding, take
@@ -87,7 +88,7 @@ __device__ __forceinline__ void share_add(Share& a, const float* x, float k) {
     a.m = m;
 }
 
-template <bool ENT>
+template <bool ENT, int THREADS>
 __device__ __forceinline__ Share share_block(Share a, float k, Share* lds) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -101,7 +102,7 @@ __device__ __forceinline__ Share share_block(Share a, float k, Share* lds) {
     __syncthreads();
     a = lds[0];
 #pragma unroll
-    for (int w = 1; w < TL_WAVES; ++w) a = share_merge<ENT>(a, lds[w], k);
+    for (int w = 1; w < THREADS / GRX_WAVE; ++w) a = share_merge<ENT>(a, lds[w], k);
     return a;
 }
 
@@ -134,11 +135,11 @@ __device__ __forceinline__ void tl_finish_padding(const TlArgs& a, int row) {
     if (a.entropy) a.entropy[row] = 0.f;
 }
 
-template <int DT, bool ENT>
-__global__ __launch_bounds__(TL_THREADS) void token_logps_kernel(TlArgs a) {
+template <int DT, bool ENT, int THREADS>
+__device__ __forceinline__ void tl_forward(const TlArgs& a) {
     typedef typename Elem<DT>::T T;
     constexpr int PV = Elem<DT>::kPerVec;
-    __shared__ Share lds[TL_WAVES];
+    __shared__ Share lds[THREADS / GRX_WAVE];
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const int64_t id = tl_id(a, row);
     if (id < 0) {
@@ -156,16 +157,16 @@ __global__ __launch_bounds__(TL_THREADS) void token_logps_kernel(TlArgs a) {
     Share sh = {-INFINITY, 0.f, 0.f};
     const u32x4* __restrict__ body = reinterpret_cast<const u32x4*>(x + head);
     int i = v0 + threadIdx.x;
-    for (; i + (TL_UNROLL - 1) * TL_THREADS < v1; i += TL_UNROLL * TL_THREADS) {
+    for (; i + (TL_UNROLL - 1) * THREADS < v1; i += TL_UNROLL * THREADS) {
         u32x4 q[TL_UNROLL];
 #pragma unroll
-        for (int j = 0; j < TL_UNROLL; ++j) q[j] = __builtin_nontemporal_load(body + i + j * TL_THREADS);
+        for (int j = 0; j < TL_UNROLL; ++j) q[j] = __builtin_nontemporal_load(body + i + j * THREADS);
         float f[TL_UNROLL * PV];
 #pragma unroll
         for (int j = 0; j < TL_UNROLL; ++j) Elem<DT>::unpack(q[j], f + j * PV);
         share_add<ENT, TL_UNROLL * PV>(sh, f, a.k);
     }
-    for (; i < v1; i += TL_THREADS) {
+    for (; i < v1; i += THREADS) {
         float f[PV];
         Elem<DT>::unpack(body[i], f);
         share_add<ENT, PV>(sh, f, a.k);
@@ -179,13 +180,23 @@ __global__ __launch_bounds__(TL_THREADS) void token_logps_kernel(TlArgs a) {
         const float f = Elem<DT>::to_float(x[tail]);
         share_add<ENT, 1>(sh, &f, a.k);
     }
-    sh = share_block<ENT>(sh, a.k, lds);
+    sh = share_block<ENT, THREADS>(sh, a.k, lds);
     if (threadIdx.x == 0) {
         if (a.parts == 1)
             tl_finish<DT>(a, row, id, sh);
         else
             a.partials[(int64_t)row * a.parts + part] = make_float4(sh.m, sh.s, sh.u, 0.f);
     }
+}
+
+template <int DT, bool ENT>
+__global__ __launch_bounds__(TL_THREADS) void token_logps_kernel(TlArgs a) {
+    tl_forward<DT, ENT, TL_THREADS>(a);
+}
+
+template <int DT, bool ENT>
+__global__ __launch_bounds__(TL_WIDE) void token_logps_wide_kernel(TlArgs a) {
+    tl_forward<DT, ENT, TL_WIDE>(a);
 }
 
 // Joins the parts of split rows, one wave per row (at most TL_MAX_PARTS = 64 parts).
@@ -301,7 +312,18 @@ __global__ __launch_bounds__(TL_THREADS) void token_logps_grad_kernel(TlArgs a) 
 }
 
 // ---- host ------------------------------------------------------------------------------------------
+// Rows that fill the CUs once, or twice to three quarters and more (a CU holds two workgroups of 1024 threads), and are
+// long enough for a turn of the loop: whole, in one launch.  V = 152,640 bf16, whole and split: 112 rows 12.9 and 12.6 us, 160
+// rows 13.1 and 15.9, 256 rows 16.6 and 21.0, 320 rows 24.4 and 24.0, 400 rows 25.3 and 27.9, 512 rows 27.9 and 31.6; V =
+// 16,000 512 rows 7.6 and 7.1.  With more rows, half of them padding, workgroups that find nothing to do cost more than
+// what is won (1280 rows 52 and 49).
+static bool tl_wide(int64_t rows, int V, int dtype) {
+    const int64_t bytes = (int64_t)V * (dtype == GRX_F32 ? 4 : 2);
+    return rows >= 128 && rows <= 512 && (rows <= 256 || rows >= 384) && bytes >= TL_WIDE * TL_UNROLL * 16;
+}
+
 static int tl_parts(int64_t rows, int V, int dtype) {
+    if (tl_wide(rows, V, dtype)) return 1;
     const int64_t vecs = ((int64_t)V * (dtype == GRX_F32 ? 4 : 2) + 15) / 16;
     int64_t p = rows > 0 ? (TL_TARGET_WGS + rows - 1) / rows : 1;
     // at least one turn of the loop per part; of few rows, at least one load per thread
@@ -359,9 +381,9 @@ static TlArgs tl_args(const grx_token_logps_args* p) {
     return a;
 }
 
-#define TL_LAUNCH(kernel, grid, ...)                                                                              \
+#define TL_LAUNCH(kernel, grid, threads, ...)                                                                     \
     do {                                                                                                          \
-        const dim3 g_((unsigned)(grid)), b_(TL_THREADS);                                                          \
+        const dim3 g_((unsigned)(grid)), b_(threads);                                                             \
         if (p->dtype == GRX_F32) {                                                                                \
             if (ent) hipLaunchKernelGGL((kernel<GRX_F32, true>), g_, b_, 0, stream, __VA_ARGS__);                  \
             else hipLaunchKernelGGL((kernel<GRX_F32, false>), g_, b_, 0, stream, __VA_ARGS__);                     \
@@ -393,8 +415,12 @@ extern "C" int grx_token_logps(const grx_token_logps_args* p, void* scratch, siz
         GRX_REQUIRE(((uintptr_t)scratch & 15) == 0, GRX_E_INVALID, "%s: misaligned scratch", who);
         a.partials = reinterpret_cast<float4*>(scratch);
     }
-    TL_LAUNCH(token_logps_kernel, rows * a.parts, a);
-    if (a.parts > 1) TL_LAUNCH(token_logps_join_kernel, (rows + TL_WAVES - 1) / TL_WAVES, a, (int)rows);
+    if (tl_wide(rows, p->V, p->dtype)) {
+        TL_LAUNCH(token_logps_wide_kernel, rows, TL_WIDE, a);
+        return GRX_OK;
+    }
+    TL_LAUNCH(token_logps_kernel, rows * a.parts, TL_THREADS, a);
+    if (a.parts > 1) TL_LAUNCH(token_logps_join_kernel, (rows + TL_WAVES - 1) / TL_WAVES, TL_THREADS, a, (int)rows);
     return GRX_OK;
 }
 
@@ -418,7 +444,7 @@ extern "C" int grx_token_logps_backward(const grx_token_logps_args* p, void* str
     const int64_t most = ((1 << 24) - 1) / a.n_chunks;  // a launch holds fewer than 2^32 threads
     for (int64_t row = 0; row < rows; row += most) {
         a.row0 = (int)row;
-        TL_LAUNCH(token_logps_grad_kernel, (rows - row < most ? rows - row : most) * a.n_chunks, a);
+        TL_LAUNCH(token_logps_grad_kernel, (rows - row < most ? rows - row : most) * a.n_chunks, TL_THREADS, a);
     }
     return GRX_OK;
 }

@@ -107,7 +107,7 @@ def test_logps_and_gradient(shape, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("rows,V", [(2500, 517), (9, 33003)])
+@pytest.mark.parametrize("rows,V", [(2500, 517), (9, 33003), (130, 40001), (400, 33003)])
 def test_rows_whole_and_split(rows, V, dtype):
     """Many rows (one workgroup each) and few (several workgroups each)."""
     _check(*_case((rows,), V, dtype, seed=rows), seed=rows)

@@ -1,13 +1,16 @@
 // Log-probabilities and entropies of tokens from hidden states [N, H] and the output projection [V, H]: what
 // token_logps.hip computes from logits.  Forward, the products of a 256 x BN tile are consumed where they are: a row
 // keeps (max, sum of exponentials, weighted sum) per 256 columns and its own token's logit.  Backward, the products --
-// kept in fp32 if the caller gave room, or formed again -- are turned into the logits' gradient G = dL/dlogits in bf16
-// -- the type autograd would hold it in -- in chunks of columns, and
+// kept in fp32 if the caller gave room, or formed again -- are turned into the logits' gradient G = dL/dlogits in chunks of
+// columns, and
 //   d hidden = G x weight (sum over v),    d weight = G^T x hidden (sum over rows)
-// follow with fp32 accumulators.  What rounding takes from a row's largest element, the one at its token, is kept in
-// fp32 and added to both sums (as a multiple of the token's weight row, of the row's hidden state): without it it is
-// an error of up to 2^-8 of a whole row of either gradient.  Three or four products of 2 N V H; bound by the matrix
-// cores at many rows, by the weight (V H elements read per product, written once) at few.
+// follow with fp32 accumulators.  The matrix cores take G in bf16 or not at all, and bf16 alone is not enough: rounded to it
+// once, elements that cancel (rows that share a hidden state and whose gradients add up to 0, as a group's do at its first
+// token) leave 2^-8 of what they were.  So G is held in two bf16 pieces, its rounding and what that leaves: off by at most
+// 2^-16 of each element, and each of its two products is made twice, with the same accumulators.  Five or six products of
+// 2 N V H where three (or four, formed again) would do in bf16: 8192 rows of H = 2048, V = 152,640 with both gradients 21.1 ms,
+// 13.7 with G in bf16.  Bound by the matrix cores at many rows, by the weight (V H elements read per product, written
+// once) at few.
 #include <hip/hip_runtime.h>
 #include <math.h>
 
@@ -20,12 +23,11 @@
 
 #define LL_FLOOR (-200.f)           // 2^-200 is 0 in fp32: keeps 0 * -inf out of the entropy sums
 #define LL_CUS 256
-#define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk
+#define LL_CHUNK_BYTES (1ll << 30)  // G of one chunk, both pieces
 
 // The rows that count are brought together first: what follows works on `plan[0]` rows, a number that only the device
-// knows, and padding costs nothing but its place in the scratch memory (1403 rows, half of them padding, H = 3584,
-// V = 151,669, with the gradient of hidden: 1.98 ms, 3.89 with all rows in the products; without padding 320 rows
-// take 16 us more of 1020).
+// knows, and padding costs nothing but its place in the scratch memory (1403 rows, H = 3584, V = 151,669, with the gradient
+// of hidden, nothing kept: half of them padding 2.7 ms, none 5.1; bringing 320 rows together takes 15 us of 1320).
 struct LlOperands {
     const uint16_t* weight;     // [V, H]
     int64_t weight_ld;
@@ -56,9 +58,6 @@ struct LlCompact {
     float inv_t;
     int* pos;                   // [N] place among the rows that count, or -1
     struct LlRow* rows;
-    float* rest;                // [rows] cleared: what rounding G takes from the element at the token
-    int* slot;                  // [V] cleared to -1; null: no d weight
-    int* count;                 // [V] cleared to 0, with slot
     int dh_bn, h_tiles, steps, slab_rows;  // what splits are chosen by
     bool kept;                  // rows are as in the forward pass: those whose gradients are 0 keep their places
 };
@@ -124,18 +123,11 @@ __global__ __launch_bounds__(1024) void lm_logps_offsets_kernel(LlCompact a, int
     }
 }
 
-// Workgroup (16 rows, 512 h); the ones behind the last row only help to clear `slot`.
+// Workgroup (16 rows, 512 h).
 template <bool BACK>
 __global__ __launch_bounds__(256) void lm_logps_compact_kernel(LlCompact a) {
     __shared__ int part[4], place[16];
     const int r0 = blockIdx.x * 16;
-    if (BACK && a.slot != nullptr)
-        for (int64_t v = ((int64_t)blockIdx.x * gridDim.y + blockIdx.y) * 256 + threadIdx.x; v < a.V;
-             v += (int64_t)gridDim.x * gridDim.y * 256) {
-            a.slot[v] = -1;
-            a.count[v] = 0;
-        }
-    if (r0 >= a.N) return;
     int before = 0;
     if (a.offsets == nullptr) {
 #pragma unroll 4
@@ -161,7 +153,6 @@ __global__ __launch_bounds__(256) void lm_logps_compact_kernel(LlCompact a) {
                 if (counts && !live) {
                     a.rows[at] = {0.f, 0.f, 0.f, 0.f, -1, {0, 0, 0}};
                     a.tok[at] = -1;
-                    a.rest[at] = 0.f;
                 }
                 if (live) {
                     const int64_t id = a.ids[r];
@@ -176,7 +167,6 @@ __global__ __launch_bounds__(256) void lm_logps_compact_kernel(LlCompact a) {
                     o.tok = id < a.V ? (int)id : 0;
                     a.rows[at] = o;
                     a.tok[at] = o.tok;
-                    a.rest[at] = 0.f;
                 }
             } else if (counts) {
                 const int64_t id = a.ids[r];
@@ -389,119 +379,28 @@ __global__ __launch_bounds__(256) void lm_logps_join_kernel(LlJoin a) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
-// Hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4], for d weight: workgroup (64 rows, 32 h).  The rows past
-// the end are 0.  Rows that share a token: the first of them stands for all.
-struct LlGroup {
-    LlOperands o;
-    const int* tok;
-    const float* rest;
-    int* slot;                 // [V] rows - 1 - the token's first row, -1: no row
-    int* count;                // [V] rows with the token
-    float* sums;               // [rows][H] in a first row: sum over the rows of its token of rest x hidden
-    char* copy;
-};
-
-__global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlGroup a) {
-    const int r0 = blockIdx.x * 64, rows = a.o.plan[LL_PLAN_ROWS];
+// Hidden in fragment blocks of 32 h x 16 n, [64 n][H / 32][4], for d weight: workgroup (64 rows, 32 h).  Rows past the
+// end, and rows without a gradient, are 0.
+__global__ __launch_bounds__(256) void lm_logps_prepare_kernel(LlOperands o, const int* tok, char* copy) {
+    const int r0 = blockIdx.x * 64, rows = o.plan[LL_PLAN_ROWS];
     if (r0 >= rows) return;
-    if (blockIdx.y == 0 && threadIdx.x < 64 && r0 + (int)threadIdx.x < rows) {  // whole numbers: any order gives the same
-        const int r = r0 + threadIdx.x, t = a.tok[r];
-        if (t >= 0) {
-            atomicMax(a.slot + t, rows - 1 - r);
-            atomicAdd(a.count + t, 1);
-        }
-    }
     const int lane = threadIdx.x & 63, n0 = r0 + (threadIdx.x >> 6) * 16 + (lane >> 5) * 8, h = blockIdx.y * 32 + (lane & 31);
     typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
     u16x8 v;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = n0 + j < rows && a.tok[n0 + j] >= 0 ? a.o.hidden[(int64_t)(n0 + j) * a.o.H + h] : (uint16_t)0;
-    *reinterpret_cast<u16x8*>(a.copy + ((int64_t)blockIdx.x * (a.o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
+    for (int j = 0; j < 8; ++j) v[j] = n0 + j < rows && tok[n0 + j] >= 0 ? o.hidden[(int64_t)(n0 + j) * o.H + h] : (uint16_t)0;
+    *reinterpret_cast<u16x8*>(copy + ((int64_t)blockIdx.x * (o.H / 32) + blockIdx.y) * 4096 + threadIdx.x * 16) = v;
 }
 
-// The sums of the tokens of one chunk.  Workgroup (rows blockIdx.x, + gridDim.x, ...; 256 h): the rows with the token
-// are listed 1024 at a time, in their order; eight groups of 32 lanes take every eighth of the list, a lane eight h.
-__global__ __launch_bounds__(256) void lm_logps_rest_kernel(LlGroup a, int v_begin, int v_end) {
-    __shared__ float part[8][32][9];
-    __shared__ int list[1024], listed[4];
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, wave = threadIdx.x >> 6;
-    const int h = blockIdx.y * 256 + lane * 8;
-    const int rows = a.o.plan[LL_PLAN_ROWS];
-    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-        const int t = a.tok[r];
-        if (t < v_begin || t >= v_end || a.slot[t] != rows - 1 - r) continue;
-        float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        int left = a.count[t];
-        for (int base = r; left > 0; base += 1024) {
-            int n = 1;
-            if (left == 1 && base == r) {  // the usual case: nobody else
-                __syncthreads();
-                if (threadIdx.x == 0) list[0] = r;
-            } else {
-                // thread i looks at rows base + 4 i .. + 3: lanes, then waves in order
-                int mine = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int i = base + (int)threadIdx.x * 4 + j;
-                    mine |= (i < rows && a.tok[i] == t) ? 1 << j : 0;
-                }
-                const int have = __popc(mine);
-                int before = have;
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const int x = __shfl_up(before, o, 64);
-                    if ((threadIdx.x & 63) >= o) before += x;
-                }
-                __syncthreads();  // the list before has been read
-                if ((threadIdx.x & 63) == 63) listed[wave] = before;
-                __syncthreads();
-                int at = before - have;
-                n = 0;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    if (w < wave) at += listed[w];
-                    n += listed[w];
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (mine >> j & 1) list[at++] = base + (int)threadIdx.x * 4 + j;
-            }
-            __syncthreads();
-            if (h < a.o.H)
-#pragma unroll 4
-                for (int i = group; i < n; i += 8) {
-                    const int row = list[i];
-                    const float w = a.rest[row];
-                    float x[8];
-                    Elem<GRX_BF16>::unpack(*reinterpret_cast<const u32x4*>(a.o.hidden + (int64_t)row * a.o.H + h), x);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[j] = fmaf(w, x[j], sum[j]);
-                }
-            left -= n;
-        }
-        __syncthreads();  // the parts of the row before have been read
-#pragma unroll
-        for (int j = 0; j < 8; ++j) part[group][lane][j] = sum[j];
-        __syncthreads();
-        if (group != 0 || h >= a.o.H) continue;
-        for (int g = 1; g < 8; ++g)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum[j] += part[g][lane][j];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) a.sums[(int64_t)r * a.o.H + h + j] = sum[j];
-    }
-}
-
-// G of a chunk of columns, in fragment blocks of 32 n x 16 v, [64 n][64 v][2][4]: a wave's results are such blocks
-// already, so a store is 1 KB in one piece, and both products read it in pieces of 8 KB and more.  8192 rows as above:
-// 3.80 ms (1.35 PFLOP/s).
+// G of a chunk of columns, in fragment blocks of 32 n x 16 v, [64 n][2 pieces][64 v][2][4]: a wave's results are such
+// blocks already, so a store is 1 KB at a time, and both products read it 8 KB and more at a time.  8192 rows as
+// above: 4.30 ms (1.19 PFLOP/s; one piece 3.80).
 struct LlGrad {
     LlOperands o;
     int m_tiles;
     int v_begin, v64;          // first column of the chunk, its width in 64s
     float k;
     const LlRow* rows;
-    float* rest;
     char* out;
 };
 
@@ -513,12 +412,13 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
     const int rows = a.o.plan[LL_PLAN_ROWS], n_pad = (rows + 63) / 64 * 64;  // rows of G
     const int n_tiles = (rows + BN - 1) / BN, tiles = a.m_tiles * n_tiles;
+    const int64_t piece = (int64_t)a.v64 * 8192;  // from the first to the second
     if ((int)blockIdx.x >= tiles) return;
     LlLogits<BN> pipe(lds);
     int tm, tn;
     mt_tile(blockIdx.x, a.m_tiles, n_tiles, tm, tn);
     ll_begin(pipe, a.o, rows, a.v_begin + tm * MT_BM, tn * BN);
-    constexpr int STORES = S::MA * S::NB * 2;
+    constexpr int STORES = S::MA * S::NB * 4;
     bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int v0 = a.v_begin + tm * MT_BM, r0 = tn * BN;
@@ -546,7 +446,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
         for (int n = 0; n < S::NB; ++n) {
             const int n32 = r0 / 32 + wn * S::NB + n;
             if (n32 * 32 >= n_pad) continue;
-            char* const out = a.out + ((int64_t)(n32 >> 1) * a.v64 + v64) * 8192 + (n32 & 1) * 4096 + lane * 16;
+            char* const out = a.out + ((int64_t)(n32 >> 1) * 2 * a.v64 + v64) * 8192 + (n32 & 1) * 4096 + lane * 16;
             const float m0 = row[n].m, alpha = row[n].alpha, beta = row[n].beta;
 #pragma unroll
             for (int m = 0; m < S::MA; ++m)
@@ -562,8 +462,6 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
                 for (int m = 0; m < S::MA; ++m)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) acc[m][n][e] += m * 16 + e == at ? row[n].at : 0.f;
-                const float whole = ll_pick<S::MA, S::NB>(acc, n, at);
-                a.rest[n32 * 32 + (lane & 31)] = whole - (float)(__bf16)whole;
             }
             const bool dead = row[n].tok < 0;
             if (__any(dead)) {
@@ -587,14 +485,16 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dlogits_kernel(
                     const mt_f32x4 x = {c[8 * q], c[8 * q + 1], c[8 * q + 2], c[8 * q + 3]};
                     const mt_f32x4 y = {c[8 * q + 4], c[8 * q + 5], c[8 * q + 6], c[8 * q + 7]};
                     const int v16 = (wm * S::MA + m) * 2 + q;
-                    *reinterpret_cast<mt_u32x4*>(out + (v16 >> 2) * 8192 + (v16 & 3) * 1024) = mt_pack8(x, y);
+                    char* const to = out + (v16 >> 2) * 8192 + (v16 & 3) * 1024;
+                    *reinterpret_cast<mt_u32x4*>(to) = mt_pack8(x, y);
+                    *reinterpret_cast<mt_u32x4*>(to + piece) = mt_pack8(mt_rest(x), mt_rest(y));
                 }
         }
     }
 }
 
-// G from the products that the forward pass kept, a wave a block of 32 v x 32 n: bound by HBM.  8192 rows as above: 1.29
-// ms (7.5 GB, 5.8 TB/s) instead of 3.80; keeping them adds 0.4 ms to the forward pass.  320 rows: 47 us instead of 236, 44
+// G from the products that the forward pass kept, a wave a block of 32 v x 32 n: bound by HBM.  8192 rows as above: 1.62
+// ms (10 GB, 6.2 TB/s) instead of 4.30; keeping them adds 0.4 ms to the forward pass.  320 rows: 61 us instead of 255, 44
 // more forward.
 template <bool ENT>
 __global__ __launch_bounds__(256) void lm_logps_kept_kernel(LlGrad a, const float* kept, int n32s) {
@@ -622,26 +522,25 @@ __global__ __launch_bounds__(256) void lm_logps_kept_kernel(LlGrad a, const floa
     const int off = row.tok - vw;  // runs of four entries, every eight
     if (row.tok >= 0 && off >= 0 && off < 32 && (off & 4) == 0) {
         const int at = (off >> 3) * 4 + (off & 3);
-        float whole = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (e == at) whole = x[e] += row.at;
-        a.rest[r] = whole - (float)(__bf16)whole;
+        for (int e = 0; e < 16; ++e) x[e] += e == at ? row.at : 0.f;
     }
 #pragma unroll
     for (int e = 0; e < 16; ++e)
         if (row.tok < 0 || vw + (e & 3) + 8 * (e >> 2) >= a.o.V) x[e] = 0.f;
-    char* const out = a.out + ((int64_t)(n32 >> 1) * a.v64 + (v32 >> 1)) * 8192 + (n32 & 1) * 4096 + (v32 & 1) * 2048 + lane * 16;
+    const int64_t piece = (int64_t)a.v64 * 8192;  // from the first to the second
+    char* const out = a.out + ((int64_t)(n32 >> 1) * 2 * a.v64 + (v32 >> 1)) * 8192 + (n32 & 1) * 4096 + (v32 & 1) * 2048 + lane * 16;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         const mt_f32x4 lo = {x[8 * q], x[8 * q + 1], x[8 * q + 2], x[8 * q + 3]};
         const mt_f32x4 hi = {x[8 * q + 4], x[8 * q + 5], x[8 * q + 6], x[8 * q + 7]};
         *reinterpret_cast<mt_u32x4*>(out + q * 1024) = mt_pack8(lo, hi);
+        *reinterpret_cast<mt_u32x4*>(out + piece + q * 1024) = mt_pack8(mt_rest(lo), mt_rest(hi));
     }
 }
 
 // d hidden: C[n][h] = sum over the chunk's columns of G[n][v] weight[v][h], fp32 slabs, one per split of the columns.
-// 8192 rows: 3.65 ms (1.40 PFLOP/s; the library's product 3.62 ms).
+// Both pieces of G: 8192 rows 7.67 ms (1.34 PFLOP/s; the library's product with one 3.62 ms).
 struct LlDh {
     LlOperands o;
     const char* g;
@@ -658,6 +557,7 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     const int total = splits * a.m_tiles * n_tiles, steps_per = (a.steps + splits - 1) / splits;
     const int lane = threadIdx.x & 63, wave = mt_wave();
     const int wm = wave / S::WN, wn = wave % S::WN, half = lane >> 5;
+    const int64_t piece = (int64_t)a.v64 * 8192;
     MtPipe<BN, MtAcross<BN>, MtReadAcross, MtBlocksAlong<BN, BN>, MtReadBlocksAlong> pipe(lds);
     for (int block = blockIdx.x; block < total; block += gridDim.x) {
         // one XCD takes neighbouring tiles: all h tiles of a few n tiles, which share G
@@ -669,9 +569,9 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
         const int s0 = split * steps_per, s1 = s0 + steps_per < a.steps ? s0 + steps_per : a.steps;
         typename decltype(pipe)::Acc acc;
         pipe.begin(MtAcross<BN>(a.o.weight + (int64_t)a.v_begin * a.o.weight_ld, a.o.weight_ld, a.o.H, a.o.V - a.v_begin, h0, s0 * MT_BK),
-                   MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * a.v64 + s0) * 8192, 8192, (uint32_t)a.v64 * 8192u,
-                                         (rows + 63) / 64 * 2 - r0 / 32),
-                   s1 - s0);
+                   MtBlocksAlong<BN, BN>(a.g + ((int64_t)(r0 / 64) * 2 * a.v64 + s0) * 8192, piece, 8192 - piece,
+                                         (uint32_t)a.v64 * 16384u, (rows + 63) / 64 * 2 - r0 / 32),
+                   (s1 - s0) * 2);
         float* slab = a.slabs + (int64_t)split * rows * a.o.H;
         pipe.clear(acc);
         if (a.add) {
@@ -704,9 +604,9 @@ __global__ __launch_bounds__(MtShape<BN>::THREADS) void lm_logps_dhidden_kernel(
     }
 }
 
-// Sum of the slabs in their order and of what rounding took from G at the row's token, rounded once.
+// Sum of the slabs in their order, rounded once.
 __global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o, int N, const float* slabs, const int* pos,
-                                                                    const int* tok, const float* rest, uint16_t* out) {
+                                                                    uint16_t* out) {
     const int64_t n = (int64_t)N * o.H, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (i >= n) return;
     const int row = (int)(i / o.H), h = (int)(i - (int64_t)row * o.H), r = pos[row];
@@ -714,31 +614,28 @@ __global__ __launch_bounds__(256) void lm_logps_dhidden_join_kernel(LlOperands o
     if (r >= 0) {
         const int splits = o.plan[LL_PLAN_SPLITS];
         const int64_t slab = (int64_t)o.plan[LL_PLAN_ROWS] * o.H, at = (int64_t)r * o.H + h;
-        const mt_b16x4 w = *reinterpret_cast<const mt_b16x4*>(o.weight + (int64_t)tok[r] * o.weight_ld + h);
         for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const mt_f32x4*>(slabs + s * slab + at);
-        v += rest[r] * __builtin_convertvector(w, mt_f32x4);
     }
     *reinterpret_cast<mt_b16x4*>(out + i) = __builtin_convertvector(v, mt_b16x4);
 }
 
-// d weight of the chunk: C[v][h] = sum over the rows of G[n][v] hidden[n][h].  8192 rows: 3.97 ms (1.29 PFLOP/s; the
-// library's product 4.40 ms).  At few rows the stores come on top of the products (a wave's copies are counted together
-// with its stores, so the copies of a tile's third step wait for the stores of the tile before): 320 rows 312 us.
+// d weight of the chunk: C[v][h] = sum over the rows of G[n][v] hidden[n][h], both pieces of G.  8192 rows: 7.7 ms (1.33
+// PFLOP/s; the library's product with one 4.40 ms).  At few rows the stores come on top of the products (a wave's copies are
+// counted together with its stores, so the copies of a tile's third step wait for the stores of the tile before): 320 rows 430 us.
 struct LlDw {
     const char* copy;
     const char* g;
     int H, V;
     int m_tiles, n_tiles, v_begin, v64;
     const int* plan;
-    const int* slot;           // [V], sums [rows][H] as in LlGroup: what rounding took from G at the rows' tokens
-    const float* sums;
     uint16_t* out;             // [V][H]
 };
 
 // LINES: two buffers of either operand, and the LDS left holds the results on their way to whole lines of 128 bytes;
-// otherwise three buffers of G and stores of the 16 bytes that a lane holds.  Up to LL_LINES_STEPS steps the stores weigh
-// more: at H = 2048 and V = 152,640 (625 MB to write) 64 rows take 140 us against 199, 512 rows 405 against 443, 1024 rows
-// 645 against 665, 1536 rows 911 against 896, 4096 rows 2160 against 2080.
+// otherwise three buffers of G and stores of the 16 bytes that a lane holds.  Up to LL_LINES_STEPS steps (two for every 64
+// rows) the stores weigh more: the backward pass for d weight alone takes, with lines and without, at H = 2048 and V = 152,640
+// (625 MB to write) 64 rows 158 and 244 us, 320 rows 427 and 530, 512 rows 710 and 731, 768 rows 1011 and 997, 1024 rows 1310
+// and 1277; at H = 3584 and V = 40,000 64 rows 84 and 101, 512 rows 296 and 323, 1024 rows 525 and 552.
 #define LL_LINES_STEPS 16
 template <bool LINES>
 using LlDwPipe = MtPipe<256, MtBlocksAlong<MT_BM, 256>, MtReadBlocksAlong, MtBlocksAcross, MtReadBlocksAcross, !LINES, LINES ? 2 : 3>;
@@ -754,8 +651,8 @@ __device__ __forceinline__ void ll_dw_at(const LlDw& a, int tile, int& h0, int& 
 template <bool LINES>
 __device__ __forceinline__ void ll_dw_begin(LlDwPipe<LINES>& pipe, const LlDw& a, int rows, int tile, int& h0, int& c0) {
     ll_dw_at(a, tile, h0, c0);
-    pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
-               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), (rows + MT_BK - 1) / MT_BK);
+    pipe.begin(MtBlocksAlong<MT_BM, 256>(a.copy + (int64_t)(h0 / 32) * 4096, 0, (int64_t)(a.H / 32) * 4096, 8192u, a.H / 32 - h0 / 32),
+               MtBlocksAcross(a.g + (int64_t)(c0 / 64) * 8192, (int64_t)a.v64 * 8192), (rows + MT_BK - 1) / MT_BK * 2);
 }
 
 template <bool LINES>
@@ -768,44 +665,15 @@ __global__ __launch_bounds__(MtShape<256>::THREADS) void lm_logps_dweight_kernel
     LlDwPipe<LINES> pipe(lds);
     // LINES: behind the 128 KB of the pipe, 4 KB of each wave
     const uint32_t staging = (uint32_t)(uintptr_t)(mt_lds_void*)lds + 4 * MT_BM * MT_BK * 2 + wave * 4096;
-    int h_next, c_next, slot_next[S::NB];
-    const auto find = [&](int tile) {  // a tile ahead, so that nobody waits for it
-        int h0, c0;
-        ll_dw_at(a, tile, h0, c0);
-#pragma unroll
-        for (int n = 0; n < S::NB; ++n) {
-            const int v = a.v_begin + c0 + (wn * S::NB + n) * 32 + (lane & 31);
-            slot_next[n] = tile < tiles && v < a.V ? a.slot[v] : -1;
-        }
-    };
+    int h_next, c_next;
     ll_dw_begin<LINES>(pipe, a, rows, blockIdx.x, h_next, c_next);
-    find(blockIdx.x);
-#pragma unroll
-    for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(slot_next[n]));
     constexpr int STORES = S::MA * S::NB * 2;
     bool stored = false;  // all STORES of the tile before were made
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
         const int h0 = h_next, c0 = c_next;
-        int slot[S::NB];
-#pragma unroll
-        for (int n = 0; n < S::NB; ++n) slot[n] = slot_next[n];
         typename LlDwPipe<LINES>::Acc acc;
         pipe.clear(acc);
-#pragma unroll
-        for (int n = 0; n < S::NB; ++n)
-            if (__any(slot[n] >= 0)) {  // the sum goes on from what rounding took from G
-                const float* const sums = a.sums + (int64_t)(rows - 1 - slot[n]) * a.H;
-#pragma unroll
-                for (int m = 0; m < S::MA; ++m) {
-                    const int h = h0 + (wm * S::MA + m) * 32;
-                    if (slot[n] >= 0 && h < a.H) pipe.load(acc, m, n, sums + h);
-                    asm volatile("" : "+v"(acc[m][n]));  // waited for here, and not by the waves without a token
-                }
-            }
-        find(tile + gridDim.x);
         pipe.template run<STORES>(acc, stored);
-#pragma unroll
-        for (int n = 0; n < S::NB; ++n) asm volatile("" : "+v"(slot_next[n]));  // waited for here, not behind the stores
         stored = a.v_begin + c0 + (wn + 1) * S::NB * 32 <= a.V && h0 + (wm + 1) * S::MA * 32 <= a.H;
         if (tile + (int)gridDim.x < tiles) ll_dw_begin<LINES>(pipe, a, rows, tile + gridDim.x, h_next, c_next);
 #pragma unroll
@@ -846,8 +714,8 @@ static int ll_bn(int N, int64_t m_tiles) {
     return best;
 }
 
-// Rows per tile of d hidden, whose sum is split over the columns until the CUs are full: the least work (320 rows: 203 us
-// with 192, 256 with 256 and 260 with 128).
+// Rows per tile of d hidden, whose sum is split over the columns until the CUs are full: the least work (backward pass for d
+// hidden alone, 320 rows: 459 us with 192, 565 with 256 and 513 with 128; 576 rows 715, 876 and 825; 400 rows 628, 559, 599).
 static int ll_dh_bn(int N) {
     int best = 64;
     for (int bn = 128; bn <= 256; bn += 64)
@@ -906,7 +774,7 @@ struct LlBackward {
     int64_t n_pad;             // rows of G: whole steps of d weight
     int64_t chunk;             // columns of G: a multiple of 256
     int n_chunks;
-    size_t plan, offsets, pos, rows, tok, rest, count, slot, hidden, sums, copy, g, slabs, total;
+    size_t plan, offsets, pos, rows, tok, hidden, copy, g, slabs, total;
 };
 
 static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
@@ -916,7 +784,7 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.h_tiles = (H + MT_BM - 1) / MT_BM;
     b.n_pad = ll_up(N, MT_BK);
     const int64_t v_pad = ll_up(V, MT_BM);
-    int64_t most = LL_CHUNK_BYTES / 2 / b.n_pad / MT_BM * MT_BM;
+    int64_t most = LL_CHUNK_BYTES / 4 / b.n_pad / MT_BM * MT_BM;
     if (most < MT_BM) most = MT_BM;
     b.n_chunks = (int)((v_pad + most - 1) / most);
     b.chunk = ll_up((v_pad + b.n_chunks - 1) / b.n_chunks, MT_BM);
@@ -932,13 +800,9 @@ static LlBackward ll_backward(int N, int H, int V, bool want_h, bool want_w) {
     b.pos = l.take((int64_t)N * 4);
     b.rows = l.take((int64_t)N * sizeof(LlRow));
     b.tok = l.take((int64_t)N * 4);
-    b.rest = l.take((int64_t)N * 4);
     b.hidden = l.take((int64_t)N * H * 2);
-    b.count = l.take(want_w ? (int64_t)V * 4 : 0);
-    b.slot = l.take(want_w ? (int64_t)V * 4 : 0);
-    b.sums = l.take(want_w ? (int64_t)N * H * 4 : 0);
     b.copy = l.take(want_w ? b.n_pad * H * 2 : 0);
-    b.g = l.take(b.n_pad * b.chunk * 2);
+    b.g = l.take(b.n_pad * b.chunk * 4);
     b.slabs = l.take(want_h ? (int64_t)b.slab_rows * H * 4 : 0);
     b.total = l.at;
     return b;
@@ -1056,8 +920,7 @@ static int ll_compact(LlCompact& c, const grx_lm_token_logps_args* p, int* offse
         GRX_CHECK_HIP(hipGetLastError());
         c.offsets = offsets;
     }
-    const int grid = c.slot != nullptr && blocks < 64 ? 64 : blocks;
-    hipLaunchKernelGGL(lm_logps_compact_kernel<BACK>, dim3((unsigned)grid, (unsigned)((p->H + 511) / 512)), dim3(256), 0, stream, c);
+    hipLaunchKernelGGL(lm_logps_compact_kernel<BACK>, dim3((unsigned)blocks, (unsigned)((p->H + 511) / 512)), dim3(256), 0, stream, c);
     GRX_CHECK_HIP(hipGetLastError());
     return GRX_OK;
 }
@@ -1135,9 +998,6 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     k.inv_t = (float)(1.0 / (double)p->temperature);
     k.pos = reinterpret_cast<int*>(s + b.pos);
     k.rows = reinterpret_cast<LlRow*>(s + b.rows);
-    k.rest = reinterpret_cast<float*>(s + b.rest);
-    k.slot = want_w ? reinterpret_cast<int*>(s + b.slot) : nullptr;
-    k.count = want_w ? reinterpret_cast<int*>(s + b.count) : nullptr;
     k.dh_bn = b.dh_bn;
     k.h_tiles = b.h_tiles;
     k.steps = (int)(b.chunk / MT_BK);
@@ -1148,15 +1008,15 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
     const LlOperands o = {reinterpret_cast<const uint16_t*>(p->weight), p->weight_stride, k.to, k.plan, p->H, p->V};
     char* g = s + b.g;
     float* slabs = reinterpret_cast<float*>(s + b.slabs);
-    const LlGroup gr = {o, k.tok, k.rest, k.slot, k.count, reinterpret_cast<float*>(s + b.sums), s + b.copy};
     if (want_w) {
-        hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_pad / 64), (unsigned)(p->H / 32)), dim3(256), 0, stream, gr);
+        hipLaunchKernelGGL(lm_logps_prepare_kernel, dim3((unsigned)(b.n_pad / 64), (unsigned)(p->H / 32)), dim3(256), 0, stream, o, k.tok,
+                           s + b.copy);
         GRX_CHECK_HIP(hipGetLastError());
     }
     for (int c = 0; c < b.n_chunks; ++c) {
         const int v0 = (int)(c * b.chunk), v64 = (int)(b.chunk / 64);
         const int64_t cols = ll_up(p->V - v0 < b.chunk ? p->V - v0 : b.chunk, MT_BM);
-        LlGrad d = {o, (int)(cols / MT_BM), v0, v64, (float)(1.4426950408889634 / (double)p->temperature), k.rows, k.rest, g};
+        LlGrad d = {o, (int)(cols / MT_BM), v0, v64, (float)(1.4426950408889634 / (double)p->temperature), k.rows, g};
         if (p->kept) {
             const int n32s = (int)(ll_forward(p->N, p->H, p->V, false).n_pad / 32);
             const dim3 grid((unsigned)(d.m_tiles * 2), (unsigned)(b.n_pad / 32));
@@ -1171,20 +1031,17 @@ extern "C" int grx_lm_token_logps_backward(const grx_lm_token_logps_args* p, voi
             LL_EACH(b.dh_bn, lm_logps_dhidden_kernel, std::max<int64_t>((int64_t)b.splits * b.h_tiles * b.dh_tiles, LL_CUS), x);
         }
         if (want_w) {
-            hipLaunchKernelGGL(lm_logps_rest_kernel, dim3((unsigned)(p->N < 1024 ? p->N : 1024), (unsigned)((p->H + 255) / 256)),
-                               dim3(256), 0, stream, gr, v0, (int)(v0 + cols));
-            GRX_CHECK_HIP(hipGetLastError());
-            LlDw x = {gr.copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), v0, v64, k.plan, k.slot, gr.sums,
+            LlDw x = {s + b.copy, g, p->H, p->V, b.h_tiles, (int)(cols / 256), v0, v64, k.plan,
                       reinterpret_cast<uint16_t*>(p->grad_weight)};
             const int64_t wgs = ll_resident(256, (int64_t)x.m_tiles * x.n_tiles);
-            if (b.n_pad / MT_BK <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
+            if (b.n_pad / MT_BK * 2 <= LL_LINES_STEPS) LL_ONE(256, lm_logps_dweight_kernel<true>, wgs, x);
             else LL_ONE(256, lm_logps_dweight_kernel<false>, wgs, x);
         }
     }
     if (want_h) {
         const int64_t n = (int64_t)p->N * p->H;
         hipLaunchKernelGGL(lm_logps_dhidden_join_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, stream, o, p->N, slabs,
-                           k.pos, k.tok, k.rest, reinterpret_cast<uint16_t*>(p->grad_hidden));
+                           k.pos, reinterpret_cast<uint16_t*>(p->grad_hidden));
         GRX_CHECK_HIP(hipGetLastError());
     }
     return GRX_OK;

@@ -6,6 +6,8 @@
 //   MtAcross         rows of k, m along them
 //   MtBlocksAlong    blocks of 32 m (n) x 16 k in fragment order
 //   MtBlocksAcross   such blocks made for the other axis: 32 k x 16 n
+// An operand may lie in two bf16 pieces whose sum it is (16 bits of each element instead of 8): the pieces take turns as steps
+// of k, and the other operand's k are taken twice.
 // A fragment block is the 1 KB that one wave holds of a 32 x 16 operand: lane l has row l & 31, k = 8 (l >> 5) + 0 .. 7.
 //
 // C/D layout of the instruction: element e of lane l is m = (e & 3) + 8 (e >> 2) + 4 (l >> 5), n = l & 31: a lane
@@ -89,7 +91,7 @@ struct MtAlong {
 };
 
 // Row k of a buffer: 256 m in 32 chunks, chunk c at c ^ (4 (k & 3)).  Columns past the end (a multiple of 8) read the
-// last eight; rows past the end read the last one, where the other operand is 0.
+// last eight; rows past the end read the last one, where the other operand is 0.  Every 64 k make two steps.
 template <int BN>
 struct MtAcross {
     static constexpr int N = 2048 / MtShape<BN>::THREADS;
@@ -97,11 +99,13 @@ struct MtAcross {
     uint32_t off[N];
     int64_t ld;
     int left;  // rows of k from the step's first on
+    bool again;  // the step is the second one of its k
     __device__ __forceinline__ MtAcross() {}
     __device__ __forceinline__ MtAcross(const uint16_t* p, int64_t ld_, int cols, int k_rows, int at, int k0) {
         const int lane = threadIdx.x & 63, wave = mt_wave();
         ld = ld_;
         left = k_rows - k0;
+        again = false;
         base = reinterpret_cast<const char*>(p + (int64_t)k0 * ld + at);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -118,25 +122,31 @@ struct MtAcross {
         mt_copy_from(base + off[i] - back, to + (mt_wave() * N + i) * 1024);
     }
     __device__ __forceinline__ void advance() {
-        base += ld * (MT_BK * 2);
-        left -= MT_BK;
+        base += again ? ld * (MT_BK * 2) : 0;
+        left -= again ? MT_BK : 0;
+        again = !again;
     }
-    __device__ __forceinline__ int whole_steps(int nk) const { return nk < left / MT_BK ? nk : left / MT_BK; }
+    __device__ __forceinline__ int whole_steps(int nk) const {
+        const int whole = left >= MT_BK ? left / MT_BK * 2 - (again ? 1 : 0) : 0;
+        return nk < whole ? nk : whole;
+    }
 };
 
 // W / 32 x 4 blocks a step: the four of a group of 32 rows in one piece, the groups of a pair one behind the other,
-// pairs `pair_bytes` apart (less than 2^31 in all).  Groups past `groups` read the last one.
+// pairs `pair_bytes` apart (less than 2^31 in all).  Groups past `groups` read the last one.  Odd steps stand `odd_bytes`
+// behind even ones, those `even_bytes` behind odd ones.
 template <int W, int BN>
 struct MtBlocksAlong {
     static constexpr int N = W * MT_BK * 2 / 16 / MtShape<BN>::THREADS;
     const char* base;
     uint32_t off[N];
-    int64_t step;
+    int64_t step, then;
     __device__ __forceinline__ MtBlocksAlong() {}
     // p: the step's first block; groups: groups of 32 rows that are there from it on
-    __device__ __forceinline__ MtBlocksAlong(const char* p, int64_t step_bytes, uint32_t pair_bytes, int groups) {
+    __device__ __forceinline__ MtBlocksAlong(const char* p, int64_t odd_bytes, int64_t even_bytes, uint32_t pair_bytes, int groups) {
         base = p;
-        step = step_bytes;
+        step = odd_bytes;
+        then = even_bytes;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int block = mt_wave() * N + i;
@@ -146,11 +156,17 @@ struct MtBlocksAlong {
     }
     __device__ __forceinline__ void issue(int i, uint32_t to) const { mt_copy(base, off[i], to + (mt_wave() * N + i) * 1024); }
     __device__ __forceinline__ void issue_any(int i, uint32_t to) const { issue(i, to); }
-    __device__ __forceinline__ void advance() { base += step; }
+    __device__ __forceinline__ void advance() {
+        base += step;
+        const int64_t s = step;
+        step = then;
+        then = s;
+    }
     __device__ __forceinline__ int whole_steps(int nk) const { return nk; }
 };
 
-// G as d weight reads it: blocks of 32 n x 16 v, in memory [64 n][64 v][2][4], a step being 64 n of 256 v.
+// G as d weight reads it: blocks of 32 n x 16 v, in memory [64 n][2 pieces][64 v][2][4], a step being one piece of 64 n of
+// 256 v.
 // In a buffer, [64 v][32 n][16 v] blocks whose unit of 16 bytes (n, 8 v h) stands at (2 n + h) ^ (8 in odd blocks): the
 // 32 lanes of a transposing read take 16 different units of a bank row.
 struct MtBlocksAcross {
@@ -437,6 +453,11 @@ __device__ __forceinline__ mt_u32x4 mt_pack8(mt_f32x4 x, mt_f32x4 y) {
     const auto p = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
     const auto q = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
     return mt_u32x4{p[0], q[0], p[1], q[1]};
+}
+
+// What rounding to bf16 takes from x: the second piece.
+__device__ __forceinline__ mt_f32x4 mt_rest(mt_f32x4 x) {
+    return x - __builtin_convertvector(__builtin_convertvector(x, mt_b16x4), mt_f32x4);
 }
 
 // Two blocks of results (m rows of 32 and the next 32, 32 n) rounded to bf16 and stored as 32 rows n of 64 m.

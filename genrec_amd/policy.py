@@ -62,12 +62,13 @@ def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: t
     """:func:`token_logps` of ``logits = hidden @ weight.T``: the product runs on the matrix cores and is consumed tile
     by tile, forward and backward.  Where a backward pass follows and the products take up to ``keep_bytes`` in fp32
     (N x V x 4 and the tiles' margins), they are kept for it; otherwise, with 0 always, it forms them again and no
-    logits are ever held (8192 rows of a vocabulary of 152,640, H = 2048: 5 GB kept, 13.6 ms with both gradients;
-    nothing kept, 15.4 ms).
+    logits are ever held (8192 rows of a vocabulary of 152,640, H = 2048: 5 GB kept, 21.1 ms with both gradients;
+    nothing kept, 23.4 ms).
 
     ``hidden`` [B, T, H] or [N, H] and ``weight`` [V, H] (``lm_head.weight``, no bias), bf16, H a multiple of 64, on
     the GPU; ``token_ids`` [B, T] or [N], negative for padding.  Differentiable in both; a frozen weight costs
-    nothing.  The logits' gradient passes through bf16 on its way to the two products, as it does under autograd.
+    nothing.  The logits' gradient reaches the two products in two bf16 pieces (16 bits of each element, where autograd's bf16
+    logits would hold 8), so that rows whose gradients cancel leave nothing but the rounding of 32-bit sums.
     Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Scratch
     tensors: about V / 16 bytes a row forward; up to 1 GB and 12 bytes per element of ``hidden`` backward.  A pass
     recorded into a HIP graph needs leaves of its own (``detach().requires_grad_()`` inside the recording)."""

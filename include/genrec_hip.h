@@ -747,7 +747,7 @@ GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* str
  * weight^T [H, V] / temperature (bf16 operands, fp32 sums; nn.Linear.weight, no bias).  Outputs and
  * padding as above, [N] each.  Backward writes grad_hidden [N, H] and / or grad_weight [V, H], bf16,
  * contiguous, 16-byte aligned, all of them (a null one is not computed); the logits' gradient in
- * between is bf16.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
+ * between is the sum of two bf16 numbers, within 2^-16 of each element.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
  * H a multiple of 64, at most 2^34 elements of hidden in the backward pass, operand rows 16-byte
  * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row
  * and 2 per element of hidden; backward: a chunk of the logits' gradient, up to 1 GB, and about 12

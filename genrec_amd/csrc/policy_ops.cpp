@@ -3,6 +3,7 @@
 // own: without Python in it a launcher-sized loss with its gradient takes a third of the time on the host.  The
 // library's entry points are handed over by address (bind), so this module calls the copy that genrec_amd._lib loaded.
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <ATen/DeviceGuard.h>
@@ -119,16 +120,24 @@ void refuse_nodes_outside(const at::Device& device) {
 }
 
 // The kernels have no gradient of their own: under create_graph the results carry a node that says so when it is reached.
+// It stands where the derivative's node would, in front of all that the results depend on -- the inputs of the node that runs
+// and what came in -- whether or not the incoming gradients are constants, so that no second-order term is left out unsaid.
 variable_list once(const variable_list& incoming, variable_list out) {
     if (!at::GradMode::is_enabled()) return out;
-    bool any = false;
-    for (const Tensor& g : incoming) any = any || (g.defined() && g.requires_grad());
-    if (!any) return out;
-    for (Tensor& t : out)
-        if (t.defined()) t = t.detach().set_requires_grad(true);
-    auto error = std::make_shared<torch::autograd::DelayedError>(
-        "trying to differentiate twice a function of genrec_amd.policy, which is differentiable once", (int64_t)out.size());
-    return (*error)(std::move(out));
+    torch::autograd::edge_list next;
+    if (const auto node = torch::autograd::get_current_node())
+        for (const auto& edge : node->next_edges())
+            if (edge.is_valid()) next.push_back(edge);
+    for (const Tensor& g : incoming)
+        if (g.defined() && g.requires_grad()) next.push_back(torch::autograd::impl::gradient_edge(g));
+    const auto error = std::make_shared<torch::autograd::Error>(
+        "trying to differentiate twice a function of genrec_amd.policy, which is differentiable once", std::move(next));
+    for (Tensor& t : out) {
+        if (!t.defined()) continue;
+        t = t.detach();
+        torch::autograd::set_history(t, error);
+    }
+    return out;
 }
 
 int dtype_code(const Tensor& t) {

@@ -1,0 +1,82 @@
+"""GPU: what autograd may ask of ``genrec_amd.policy`` besides a gradient: a second derivative is refused however it is
+reached."""
+
+import pytest
+import torch
+
+from genrec_amd.policy import lm_head_token_logps, policy_loss, token_logps
+
+pytestmark = pytest.mark.gpu
+
+
+def _logits(B=4, T=5, V=301, seed=1):
+    dev = torch.device("cuda", 0)
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    x = torch.randn((B, T, V), generator=gen, device=dev, requires_grad=True)
+    return x, torch.randint(0, V, (B, T), generator=gen, device=dev), torch.randn((B,), generator=gen, device=dev)
+
+
+def _head(N=40, H=128, V=301, seed=2):
+    dev = torch.device("cuda", 0)
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    h = torch.randn((N, H), generator=gen, device=dev).to(torch.bfloat16).requires_grad_()
+    w = (torch.randn((V, H), generator=gen, device=dev) * 0.1).to(torch.bfloat16).requires_grad_()
+    return h, w, torch.randint(0, V, (N,), generator=gen, device=dev)
+
+
+def _first(kind):
+    """(a value, its leaves)"""
+    if kind == "logits":
+        x, ids, _ = _logits()
+        return token_logps(x, ids).sum(), [x]
+    if kind == "entropy":
+        x, ids, _ = _logits()
+        return token_logps(x, ids, return_entropy=True)[1].sum(), [x]
+    if kind == "loss":
+        x = torch.zeros((4, 5), device="cuda", requires_grad=True)
+        return policy_loss(x, torch.ones(4, device="cuda"), torch.ones((4, 5), device="cuda")).loss, [x]
+    if kind == "loss of logits":
+        x, ids, adv = _logits()
+        return policy_loss(token_logps(x, ids), adv, torch.ones_like(ids)).loss, [x]
+    h, w, ids = _head()
+    if kind == "head":
+        return lm_head_token_logps(h, w, ids).sum(), [h, w]
+    return lm_head_token_logps(h, w.detach(), ids).sum(), [h]
+
+
+KINDS = ["logits", "entropy", "loss", "loss of logits", "head", "head, frozen weight"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_second_derivative_of_a_plain_sum_is_refused(kind):
+    """The incoming gradient is a constant, and the result still depends on the leaves."""
+    value, leaves = _first(kind)
+    first = torch.autograd.grad(value, leaves, create_graph=True)
+    for d in first:
+        assert d.requires_grad
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad(d.float().pow(2).sum(), leaves, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            torch.autograd.grad(d.float().pow(2).sum(), leaves, retain_graph=True, allow_unused=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):  # a penalty on the gradient, beside the loss
+        (value + sum(d.float().pow(2).sum() for d in first)).backward()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_graph_of_the_gradient_changes_nothing_else(kind):
+    value, leaves = _first(kind)
+    want = torch.autograd.grad(value, leaves, retain_graph=True)
+    got = torch.autograd.grad(value, leaves, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert not any(d.requires_grad for d in want)
+    for d in got:  # a constant made of it is fine
+        assert not d.detach().requires_grad and torch.isfinite(d.detach().float()).all()
+
+
+def test_second_derivative_with_respect_to_the_incoming_gradient_is_refused():
+    x, ids, _ = _logits()
+    lp = token_logps(x, ids)
+    g = torch.ones_like(lp).requires_grad_()
+    (d,) = torch.autograd.grad(lp, x, g, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        torch.autograd.grad(d.sum(), g)

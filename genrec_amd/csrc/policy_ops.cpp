@@ -140,6 +140,10 @@ variable_list once(const variable_list& incoming, variable_list out) {
     return out;
 }
 
+// No gradient is asked of t, in either direction: a call may go without a node.  (A forward-mode tangent has to reach the
+// node, which refuses it.)
+bool constant(const Tensor& t) { return !(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined(); }
+
 int dtype_code(const Tensor& t) {
     switch (t.scalar_type()) {
         case at::kFloat: return GRX_F32;
@@ -225,7 +229,7 @@ py::object token_logps(const Tensor& logits_, const Tensor& token_ids, double te
     const Tensor ids = token_ids_of(token_ids, logits_.device());
     require_cuda(logits_, "logits");
     const Tensor logits = logits_.size(-1) > 1 && logits_.stride(-1) != 1 ? logits_.contiguous() : logits_;
-    if (!at::GradMode::is_enabled() || !logits.requires_grad())
+    if (constant(logits))
         return outputs(token_forward(logits, ids, temperature, entropy, nullptr), token_ids.sizes());
     return outputs(TokenLogps::apply(logits, ids, temperature, entropy), token_ids.sizes());
 }
@@ -327,7 +331,7 @@ py::object lm_head_token_logps(const Tensor& hidden, const Tensor& weight, const
     same_device(weight, hidden.device(), "weight");
     require_cuda(hidden, "hidden");
     const Tensor rows = aligned_rows(hidden.dim() == 2 ? hidden : hidden.reshape({ids.numel(), H})), w = aligned_rows(weight);
-    if (!at::GradMode::is_enabled() || !(rows.requires_grad() || w.requires_grad()))
+    if (constant(rows) && constant(w))
         return outputs(lm_forward(rows, w, ids, temperature, entropy, f32_like({rows.size(0), 2}, rows), Tensor()), token_ids.sizes());
     return outputs(LmTokenLogps::apply(rows, w, ids, temperature, entropy, keep_bytes), token_ids.sizes());
 }

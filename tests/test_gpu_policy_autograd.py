@@ -1,8 +1,9 @@
 """GPU: what autograd may ask of ``genrec_amd.policy`` besides a gradient: a second derivative is refused however it is
-reached."""
+reached, and so is a derivative in forward mode."""
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from genrec_amd.policy import lm_head_token_logps, policy_loss, token_logps
 
@@ -80,3 +81,27 @@ def test_second_derivative_with_respect_to_the_incoming_gradient_is_refused():
     (d,) = torch.autograd.grad(lp, x, g, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiate twice"):
         torch.autograd.grad(d.sum(), g)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("kind", ["logits", "logits, transposed vocabulary", "hidden", "weight", "loss"])
+def test_forward_mode_is_refused(kind, grad):
+    """A dual tensor must not come back without its tangent, whether a gradient is recorded or not."""
+    x, ids, adv = (t.detach() for t in _logits())
+    h, w, tokens = (t.detach() for t in _head())
+
+    def call(t):
+        if kind == "logits":
+            return token_logps(t(x), ids, return_entropy=True)
+        if kind == "logits, transposed vocabulary":
+            return token_logps(t(x.transpose(1, 2)).transpose(1, 2), ids)
+        if kind == "hidden":
+            return lm_head_token_logps(t(h), w, tokens)
+        if kind == "weight":
+            return lm_head_token_logps(h, t(w), tokens)
+        return policy_loss(t(x[..., 0].contiguous()), adv, torch.ones_like(ids)).loss
+
+    call(lambda t: t)  # the same call without a tangent
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+            call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))

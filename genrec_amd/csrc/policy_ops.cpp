@@ -453,7 +453,8 @@ py::tuple policy_loss(const Tensor& logps_, const Tensor& advantages, const Tens
     a.delta = delta.value_or(0.0);
     a.normalizer = normalizer;
     const Tensor loss = PolicyLoss::apply(logps, stats, &a, at::GradMode::is_enabled() && logps.requires_grad());
-    const std::vector<Tensor> s = stats.unbind(0);
+    // with a version counter of their own: the backward pass reads the fourth number, and the caller may write over the others
+    const std::vector<Tensor> s = stats.variable_data().unbind(0);
     return py::make_tuple(loss, s[0], s[1], s[2]);
 }
 

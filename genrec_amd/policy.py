@@ -78,7 +78,7 @@ def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: t
 class PolicyLoss:
     """Result of :func:`policy_loss`: ``loss`` (0-d, differentiable) and, as 0-d fp32 tensors without gradient,
     ``kl`` (mean of the KL estimate over valid tokens), ``clip_low`` and ``clip_high`` (shares of valid tokens cut
-    at the lower and the upper bound)."""
+    at the lower and the upper bound).  They are the caller's: averaging them in place before ``loss.backward()`` is fine."""
 
     __slots__ = ("loss", "kl", "clip_low", "clip_high")
 

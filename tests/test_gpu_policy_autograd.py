@@ -1,5 +1,5 @@
 """GPU: what autograd may ask of ``genrec_amd.policy`` besides a gradient: a second derivative is refused however it is
-reached, and so is a derivative in forward mode."""
+reached, and so is a derivative in forward mode; the statistics of a loss are the caller's."""
 
 import pytest
 import torch
@@ -105,3 +105,28 @@ def test_forward_mode_is_refused(kind, grad):
     with forward_ad.dual_level(), torch.set_grad_enabled(grad):
         with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
             call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("kind", ["grpo", "bnpo"])  # the gradient's factor known beforehand, and only at the end
+def test_statistics_may_be_written_over_before_the_backward_pass(kind):
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    old = torch.randn((30, 7), generator=gen, device="cuda") - 2
+    mask = torch.ones_like(old)
+    mask[::3, 4:] = 0
+
+    def step():
+        x = (old + 0.3).requires_grad_()
+        return x, policy_loss(x, torch.ones(30, device="cuda"), mask, old, old, beta=0.1, loss_type=kind)
+
+    x, res = step()
+    (want,) = torch.autograd.grad(res.loss, x)
+    values = res.kl.clone(), res.clip_low.clone(), res.clip_high.clone()
+    x, res = step()
+    res.kl.div_(2)
+    res.clip_low.fill_(9)
+    res.clip_high.neg_()
+    assert torch.equal(res.kl, values[0] / 2) and torch.equal(res.clip_high, -values[2]) and float(res.clip_low) == 9
+    (got,) = torch.autograd.grad(res.loss, x)
+    assert torch.equal(got, want)
+    with torch.inference_mode():
+        assert torch.equal(step()[1].kl, values[0])

@@ -276,12 +276,22 @@ variable_list lm_forward(const Tensor& hidden, const Tensor& weight, const Tenso
     return out;
 }
 
+// Room for the products, if that many bytes may be kept and are there: without them the backward pass forms them again.
+Tensor room_to_keep(size_t bytes, int64_t keep_bytes, const at::Device& d) {
+    if ((int64_t)bytes > keep_bytes) return Tensor();
+    try {
+        return scratch(bytes, d);
+    } catch (const c10::OutOfMemoryError&) {
+        return Tensor();
+    }
+}
+
 struct LmTokenLogps : Function<LmTokenLogps> {
     static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& ids,
                                  double temperature, bool entropy, int64_t keep_bytes) {
         const Tensor stats = f32_like({hidden.size(0), 2}, hidden);
         const size_t n = api.lm_token_logps_kept_bytes((int32_t)hidden.size(0), (int32_t)weight.size(0));
-        const Tensor kept = (int64_t)n <= keep_bytes ? scratch(n, hidden.device()) : Tensor();
+        const Tensor kept = room_to_keep(n, keep_bytes, hidden.device());
         const variable_list out = lm_forward(hidden, weight, ids, temperature, entropy, stats, kept);
         ctx->save_for_backward({hidden, weight, ids, stats, entropy ? out[1] : Tensor(), kept});
         ctx->saved_data["temperature"] = temperature;

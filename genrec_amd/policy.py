@@ -60,10 +60,12 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
 def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: torch.Tensor, temperature: float = 1.0,
                         return_entropy: bool = False, keep_bytes: int = 8 << 30):
     """:func:`token_logps` of ``logits = hidden @ weight.T``: the product runs on the matrix cores and is consumed tile
-    by tile, forward and backward.  Where a backward pass follows and the products take up to ``keep_bytes`` in fp32
-    (N x V x 4 and the tiles' margins), they are kept for it; otherwise, with 0 always, it forms them again and no
-    logits are ever held (8192 rows of a vocabulary of 152,640, H = 2048: 5 GB kept, 21.1 ms with both gradients;
-    nothing kept, 23.4 ms).
+    by tile, forward and backward.  Where a backward pass follows, and N x V x 4 bytes (and the tiles' margins; all N rows,
+    padding too) are at most ``keep_bytes`` and are to be had, the products are kept for it in fp32 until its graph is gone:
+    by default this trades the memory that the operator saves for a tenth of the time and more.  **With ``keep_bytes=0`` no
+    logits are ever held** and the backward pass forms them again (8192 rows of a vocabulary of 152,640, H = 2048, both
+    gradients: 5 GB kept, 21.1 ms; nothing kept, 23.4 ms): the choice where memory is short or several graphs are alive at
+    a time.
 
     ``hidden`` [B, T, H] or [N, H] and ``weight`` [V, H] (``lm_head.weight``, no bias), bf16, H a multiple of 64, on
     the GPU; ``token_ids`` [B, T] or [N], negative for padding.  Differentiable in both; a frozen weight costs

@@ -52,13 +52,17 @@ __device__ __forceinline__ int mt_wave() { return __builtin_amdgcn_readfirstlane
 // `to` (uniform) + 16 x lane.  As instructions of our own because the compiler, which cannot tell the buffers apart,
 // puts a wait for all copies under way in front of every transposing LDS read; here they have no register result, and
 // what has to be waited for is written out (mt_meet).  The compiler's own counts of loads under way come out too low
-// beside them, which only makes its waits longer; M0 holds nothing of its own on this target.
+// beside them, which only makes its waits longer.  M0 is declared, so that nothing of the compiler's own is left in it across a
+// copy; the warning that it is a register with a purpose of its own is expected.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void mt_copy(const char* base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory", "m0");
 }
 __device__ __forceinline__ void mt_copy_from(const char* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(from) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 // ---- stages.  N: copies per wave and step (1 KB each); issue(i, to): the i-th of them into the buffer at
 // `to`; advance(): on to the next step.  The addresses are a uniform base plus lane offsets that stay.  A copy writes

@@ -95,13 +95,14 @@ __device__ __forceinline__ PlTerm pl_term(const PlArgs& a, double d, float w, fl
     r.kl = ref ? pl_kl(q, rise) : 0.f;
     r.kl_slope = a.p.beta != 0.f ? -a.p.beta * rise : 0.f;  // without beta an infinite KL is reported and not added
     const bool below = d < a.log_low, above = d > a.log_high, capped = d > a.log_delta;
-    const float first = (capped ? a.delta : w) * adv;
-    const float second = (below ? a.low : above ? a.high : w) * adv;
+    const float weighed = adv == 0.f && d < (double)INFINITY ? 0.f : w * adv;  // exp(d) may overflow where it is finite
+    const float first = capped ? a.delta * adv : weighed;
+    const float second = below ? a.low * adv : above ? a.high * adv : weighed;
     const float least = second < first ? second : first;  // a NaN of either stays
     r.loss = a.p.beta != 0.f ? fmaf(a.p.beta, r.kl, -least) : -least;
     r.cut_low = below && adv < 0.f;
     r.cut_high = above && adv > 0.f;
-    r.slope = (r.cut_low || r.cut_high || capped) ? 0.f : -w * adv;
+    r.slope = (r.cut_low || r.cut_high || capped) ? 0.f : -weighed;
     return r;
 }
 

@@ -176,11 +176,13 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
             adv[e] = row_adv;
             if (valid[e]) {
                 x[e] = p.logps[r * p.logps_stride + t];
-                old[e] = p.old_logps ? p.old_logps[r * p.old_stride + t] : x[e];
+                if (p.old_logps) old[e] = p.old_logps[r * p.old_stride + t];
                 if (p.ref_logps) ref[e] = p.ref_logps[r * p.ref_stride + t];
                 if (p.adv_pos_stride != 0) adv[e] = p.advantages[r * p.adv_row_stride + (int64_t)t * p.adv_pos_stride];
             }
         }
+        // the log ratio of a valid token; without an old policy 0, also where its log-probability is -inf
+        const auto ratio = [&](int e) { return p.old_logps ? (double)x[e] - (double)old[e] : 0.0; };
         double row_w = 1.0, inv_n = 1.0, row_d = 0.0;
         const double known = a.constant != 0.0 ? a.constant : 1.0;
         float seq_w = 1.f;
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 n += valid[e] ? 1.0 : 0.0;
-                if (valid[e]) d += (double)x[e] - (double)old[e];
+                if (valid[e]) d += ratio(e);
             }
             n = pl_row_sum<LANES>(n, lds);
             inv_n = 1.0 / (n > 1.0 ? n : 1.0);
@@ -207,7 +209,7 @@ __global__ __launch_bounds__(THREADS) void policy_loss_row_kernel(PlArgs a) {
                 double d = row_d;
                 float w = seq_w;
                 if (!p.sequence_level) {
-                    d = (double)x[e] - (double)old[e];
+                    d = ratio(e);
                     w = expf((float)d);
                 }
                 const PlTerm k = pl_term(a, d, w, adv[e], p.ref_logps != nullptr, (float)((double)ref[e] - (double)x[e]));

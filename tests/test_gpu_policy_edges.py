@@ -36,3 +36,17 @@ def test_no_advantage_and_a_ratio_that_overflows(T, level, gap, delta):
     # without a finite ratio there is nothing to multiply
     bad = policy_loss(_column(math.inf, T), adv, torch.ones_like(x), torch.zeros_like(x), delta=None)
     assert torch.isnan(bad.loss)
+
+
+@pytest.mark.parametrize("level", ["token", "sequence"])
+@pytest.mark.parametrize("T", [5, 200, 1500])
+def test_no_old_policy_and_a_token_ruled_out(T, level):
+    """Without an old policy the ratio is 1 whatever the log-probability is, -inf (a token that the policy rules out) too."""
+    x = (_column(-math.inf, T) - 1.0).requires_grad_()
+    adv = torch.tensor([1.0, -3.0], device="cuda")
+    res = policy_loss(x, adv, torch.ones_like(x), importance_sampling_level=level)
+    (g,) = torch.autograd.grad(res.loss, x)
+    assert float(res.loss) == 1.0  # (-1 + 3) / 2
+    want = -adv[:, None].expand(2, T) / (2 * T)
+    assert (g - want).abs().max() <= 2 * U * 1.5 / T
+    assert float(res.clip_low) == 0 and float(res.clip_high) == 0 and float(res.kl) == 0

@@ -12,6 +12,7 @@
 // 13.7 with G in bf16.  Bound by the matrix cores at many rows, by the weight (V H elements read per product, written
 // once) at few.
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -831,7 +832,8 @@ static int ll_check(const char* who, const grx_lm_token_logps_args* p) {
     GRX_REQUIRE(p->H % 64 == 0, GRX_E_UNSUPPORTED, "%s: H must be a multiple of 64", who);
     GRX_REQUIRE(p->H <= (1 << 16) && p->V <= (1 << 24) && p->N <= GRX_MAX_TOKEN_ROWS, GRX_E_UNSUPPORTED,
                 "%s: H above 2^16, V above 2^24 or more than %d rows", who, GRX_MAX_TOKEN_ROWS);
-    GRX_REQUIRE(p->temperature > 0.f && p->temperature < INFINITY, GRX_E_INVALID, "%s: temperature must be positive", who);
+    // its inverse has to be finite too
+    GRX_REQUIRE(p->temperature >= FLT_MIN && p->temperature < INFINITY, GRX_E_INVALID, "%s: temperature must be at least 2^-126", who);
     GRX_REQUIRE(p->hidden_stride >= p->H && p->weight_stride >= p->H && p->hidden_stride % 8 == 0 && p->weight_stride % 8 == 0,
                 GRX_E_INVALID, "%s: operand rows must be 16-byte aligned and at least H long", who);
     GRX_REQUIRE(p->hidden_stride <= (1 << 22) && p->weight_stride <= (1 << 22), GRX_E_UNSUPPORTED,

@@ -9,6 +9,7 @@
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cfloat>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -68,8 +69,8 @@ template <typename T>
 T* ptr(const Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
 
 double temperature_of(double t) {
-    TORCH_CHECK_VALUE(t > 0.0 && std::isfinite(t) && (float)t > 0.f && std::isfinite((float)t),
-                      "temperature must be positive and finite, got ", t);
+    // its inverse has to be finite in fp32 too
+    TORCH_CHECK_VALUE((float)t >= FLT_MIN && std::isfinite((float)t), "temperature must be at least 2^-126 and finite, got ", t);
     return t;
 }
 

@@ -8,6 +8,7 @@
 // The rows are larger than the caches between one pass and the next, so loads and stores are non-temporal: 8192 rows
 // of 152,640 bf16 forward 363 us (6.9 TB/s, what a plain read of them reaches), with ordinary ones 449 us.
 #include <hip/hip_runtime.h>
+#include <float.h>
 #include <math.h>
 
 #include "common.h"
@@ -347,7 +348,8 @@ static int tl_check(const char* who, const grx_token_logps_args* p) {
     GRX_REQUIRE((int64_t)p->B * p->T <= GRX_MAX_TOKEN_ROWS, GRX_E_UNSUPPORTED, "%s: more than %d rows", who,
                 GRX_MAX_TOKEN_ROWS);
     GRX_REQUIRE(p->V <= (1 << 24), GRX_E_UNSUPPORTED, "%s: vocabulary above 2^24", who);
-    GRX_REQUIRE(p->temperature > 0.f && p->temperature < INFINITY, GRX_E_INVALID, "%s: temperature must be positive", who);
+    // its inverse has to be finite too
+    GRX_REQUIRE(p->temperature >= FLT_MIN && p->temperature < INFINITY, GRX_E_INVALID, "%s: temperature must be at least 2^-126", who);
     if ((int64_t)p->B * p->T == 0) return GRX_OK;
     GRX_REQUIRE(p->logits != nullptr && p->token_ids != nullptr && p->row_stats != nullptr, GRX_E_INVALID,
                 "%s: null buffer", who);

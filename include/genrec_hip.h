@@ -729,7 +729,7 @@ typedef struct grx_token_logps_args {
     int64_t ids_stride;
     int32_t B, T, V;
     int32_t dtype;             /* GRX_F32 / GRX_BF16 / GRX_F16                        */
-    float temperature;         /* > 0                                                 */
+    float temperature;         /* at least 2^-126                                     */
     int32_t reserved;
     float* logps;
     float* row_stats;

@@ -76,6 +76,7 @@ EXPORTED_SYMBOLS = (
     "grx_policy_loss_scratch_bytes",
     "grx_policy_loss",
     "grx_policy_loss_backward",
+    "grx_policy_struct_bytes",
 )
 
 
@@ -447,6 +448,8 @@ def _declare(lib: C.CDLL) -> None:
     lib.grx_policy_loss.argtypes = [C.POINTER(GrxPolicyLossArgs), vp, C.c_size_t, vp]
     lib.grx_policy_loss_backward.restype = C.c_int
     lib.grx_policy_loss_backward.argtypes = [vp, vp, vp, i64, vp, vp]
+    lib.grx_policy_struct_bytes.restype = C.c_size_t
+    lib.grx_policy_struct_bytes.argtypes = [i32]
 
 
 def lib() -> C.CDLL:

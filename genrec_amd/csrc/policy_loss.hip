@@ -434,3 +434,7 @@ extern "C" int grx_policy_loss_backward(const float* unit_grad, const float* sta
     GRX_CHECK_HIP(hipGetLastError());
     return GRX_OK;
 }
+
+extern "C" size_t grx_policy_struct_bytes(int32_t which) {
+    return which == 0 ? sizeof(grx_token_logps_args) : which == 1 ? sizeof(grx_lm_token_logps_args) : which == 2 ? sizeof(grx_policy_loss_args) : 0;
+}

@@ -491,6 +491,7 @@ void bind(py::object error, py::dict addresses) {
 
 PYBIND11_MODULE(_policy_ops, m) {
     m.attr("abi_version") = GRX_ABI_VERSION;
+    m.attr("struct_bytes") = py::make_tuple(sizeof(grx_token_logps_args), sizeof(grx_lm_token_logps_args), sizeof(grx_policy_loss_args));
     m.def("bind", &bind);
     m.def("token_logps", &token_logps);
     m.def("lm_head_token_logps", &lm_head_token_logps);

@@ -35,7 +35,8 @@ def _ops():
             from . import _policy_ops
         except ImportError as e:
             raise _lib.GenrecHipError(f"genrec_amd/_policy_ops.so cannot be loaded ({e}): run `make -C genrec_amd/csrc`") from e
-        if _policy_ops.abi_version != lib.grx_abi_version():
+        built = tuple(lib.grx_policy_struct_bytes(i) for i in range(3))
+        if _policy_ops.abi_version != lib.grx_abi_version() or _policy_ops.struct_bytes != built:
             raise _lib.GenrecHipError("genrec_amd/_policy_ops.so and libgenrec_hip.so are of different builds: run "
                                       "`make -C genrec_amd/csrc`")
         names = [n for n in _lib.EXPORTED_SYMBOLS if "token_logps" in n or "policy_loss" in n] + ["grx_last_error"]

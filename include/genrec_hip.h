@@ -823,6 +823,12 @@ GRX_API int grx_policy_loss(const grx_policy_loss_args* args, void* scratch, siz
 GRX_API int grx_policy_loss_backward(const float* unit_grad, const float* stats, const float* upstream, int64_t n,
                                      float* grad_logps, void* stream);
 
+/*
+ * Sizes that the library was built with: 0 grx_token_logps_args, 1 grx_lm_token_logps_args, 2 grx_policy_loss_args; else 0.
+ * A caller whose own sizes differ was built from another version of these three structs.
+ */
+GRX_API size_t grx_policy_struct_bytes(int32_t which);
+
 #ifdef __cplusplus
 }
 #endif

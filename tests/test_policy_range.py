@@ -1,5 +1,5 @@
 """Policy-training operators: arguments at the ends of their range, on the host (every call here is refused before it
-touches a device)."""
+touches a device), and libraries that do not belong together."""
 
 import ctypes as C
 
@@ -32,3 +32,17 @@ def test_temperatures_without_a_finite_inverse_are_refused(temperature):
 def test_the_smallest_temperature_is_taken():
     with pytest.raises(_lib.GenrecHipError, match="must live on the GPU"):
         policy.token_logps(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64), 2.0 ** -126)
+
+
+def test_libraries_of_different_builds_are_refused(monkeypatch):
+    """The number of the C ABI stays where a struct only grew: the sizes tell."""
+    lib = _lib.lib()
+    sizes = tuple(lib.grx_policy_struct_bytes(i) for i in range(3))
+    assert sizes == tuple(C.sizeof(s) for s in (_lib.GrxTokenLogpsArgs, _lib.GrxLmTokenLogpsArgs, _lib.GrxPolicyLossArgs))
+    assert lib.grx_policy_struct_bytes(3) == 0 and lib.grx_policy_struct_bytes(-1) == 0
+    ops = policy._ops()
+    assert ops.struct_bytes == sizes
+    monkeypatch.setattr(policy, "_ops_module", None)
+    monkeypatch.setattr(ops, "struct_bytes", (sizes[0], sizes[1] - 8, sizes[2]))
+    with pytest.raises(_lib.GenrecHipError, match="different builds"):
+        policy.token_logps(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))

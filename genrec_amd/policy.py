@@ -5,7 +5,9 @@ token_prefix_grpo_trainer.py:196-278) to the loss of their base class, which com
 log-probabilities from the model's logits and a clipped surrogate with a KL term on them.  Here both are HIP
 kernels with hand-written gradients, on autograd tensors:
 
-    logps = token_logps(logits[:, :-1], completion_ids.masked_fill(completion_mask == 0, -1))
+    ids = input_ids.new_full(logits.shape[:2], -1)      # -1: padding, prompt and last position
+    ids[:, -T - 1 : -1] = completion_ids.masked_fill(completion_mask == 0, -1)
+    logps = token_logps(logits, ids)[:, -T - 1 : -1]
     res = policy_loss(logps, rollout.local_advantages, completion_mask, old_logps, ref_logps, beta=0.04)
     res.loss.backward()
 
@@ -52,7 +54,10 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
     ``logits`` [B, T, V] or [N, V] on the GPU, fp32, bf16 or fp16, last dimension contiguous (a view such as
     ``outputs.logits[:, -T - 1 : -1]`` is read where it lies); ``token_ids`` [B, T] or [N], integers.  A negative
     id marks padding: its row of logits is not read, results and gradient are 0 whatever it holds.  An id that
-    is not below V gives NaN.  Differentiable in ``logits`` (the gradient has their type); rows whose incoming
+    is not below V gives NaN.  Where a gradient follows, hand over the whole logits with -1 at the positions that do not
+    count: the gradient is then written in one pass.  That of a slice is autograd's, which fills the whole logits'
+    gradient with 0 and copies this one's into it (bf16, V = 152,640, forward and gradient: 5 of 6 positions of 64 rows 72
+    and 109 us, 128 of 129 1.18 and 2.38 ms, 5 of 40 211 and 226 us).  Differentiable in ``logits`` (the gradient has their type); rows whose incoming
     gradient is 0 cost one write.  A pass recorded into a HIP graph needs leaves of its own: take
     ``logits.detach().requires_grad_()`` inside the recording (gradients that would leave it are refused)."""
     return (_ops_module or _ops()).token_logps(logits, token_ids, temperature, return_entropy)

@@ -130,3 +130,24 @@ def test_statistics_may_be_written_over_before_the_backward_pass(kind):
     assert torch.equal(got, want)
     with torch.inference_mode():
         assert torch.equal(step()[1].kl, values[0])
+
+
+@pytest.mark.parametrize("L,T", [(6, 5), (40, 5), (17, 16)])
+def test_whole_logits_with_padding_where_a_slice_would_cut(L, T):
+    """The same log-probabilities and gradient as from the slice: two runs of a row differ by the order of its sums, twice
+    (V / 256 + 160) u of a probability, and by 8 u of what is multiplied with it."""
+    B, V = 6, 1003
+    x, _, _ = _logits(B, L, V)
+    ids = torch.randint(0, V, (B, T), device=x.device)
+    ids[0, 2:] = -1
+    g = torch.randn((B, T), device=x.device)
+    cut = token_logps(x[:, -T - 1 : -1], ids)
+    every = ids.new_full((B, L), -1)
+    every[:, -T - 1 : -1] = ids
+    whole = token_logps(x, every)[:, -T - 1 : -1]
+    bound = (2 * (V / 256 + 160) + 12) * 2.0 ** -24
+    assert ((cut - whole).abs() <= bound + 2.0 ** -23 * cut.abs()).all()
+    (want,), (got,) = torch.autograd.grad(cut, x, g), torch.autograd.grad(whole, x, g)
+    assert (got[:, : L - T - 1] == 0).all() and (got[:, -1] == 0).all()
+    off = (got - want).abs()[:, -T - 1 : -1]
+    assert (off <= bound * 2 * g.abs()[..., None]).all()

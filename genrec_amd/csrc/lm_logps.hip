@@ -698,7 +698,9 @@ static int64_t ll_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 // Rows per tile of the products with the logits' shape (m_tiles x n tiles of 256 x BN): what counts is whole rounds over
 // the CUs.  At H = 2048 a round takes 54 us with tiles of 256 rows, 45 with 192, 34 with 128, 41 with 64 (two to a CU).
 // At V = 152,640 320 rows take 230 us in 5 rounds of 192, 237 in 7 of 128 and 270 in 5 of 256; 576 rows 310, 374 and 380;
-// 400 rows 270 in 5 rounds of 256 and 309 in 10 of 128.
+// 400 rows 270 in 5 rounds of 256 and 309 in 10 of 128.  Whole calls from 32 to 1403 rows at H = 576, 1536, 2048 and 3584: what is chosen
+// is at most 8 % behind the best of the four (H = 3584: 320 rows 379 us, 476, 403, 380 and 437 with 64, 128, 192 and 256; 64 rows
+// 236 with 64, 223 with 128); at V = 40,000 at most 18 % (H = 2048, 150 and 192 rows: 51 us with 64 and 44 with 192).
 static double ll_cost(int bn) { return bn == 64 ? 0.4 : bn == 128 ? 0.64 : bn == 192 ? 0.84 : 1.0; }
 
 static int ll_bn(int N, int64_t m_tiles) {
@@ -735,7 +737,7 @@ struct LlLayout {
 };
 
 // Rows up to which each workgroup counts those in front of it by itself (8192 rows of H = 2048: 31 us with the copy); more
-// take a launch for it (20,000 rows: 22 us, the copy 36).
+// take a launch for it (20,000 rows: 24 us, the copy 33).  The counting does not depend on H, and hides behind the copy.
 #define LL_COUNT_ROWS (1 << 14)
 static int64_t ll_offsets_bytes(int N) { return N > LL_COUNT_ROWS ? (int64_t)((N + 15) / 16) * 4 : 0; }
 

@@ -314,10 +314,16 @@ __global__ __launch_bounds__(TL_THREADS) void token_logps_grad_kernel(TlArgs a) 
 
 // ---- host ------------------------------------------------------------------------------------------
 // Rows that fill the CUs once, or twice to three quarters and more (a CU holds two workgroups of 1024 threads), and are
-// long enough for a turn of the loop: whole, in one launch.  V = 152,640 bf16, whole and split: 112 rows 12.9 and 12.6 us, 160
-// rows 13.1 and 15.9, 256 rows 16.6 and 21.0, 320 rows 24.4 and 24.0, 400 rows 25.3 and 27.9, 512 rows 27.9 and 31.6; V =
-// 16,000 512 rows 7.6 and 7.1.  With more rows, half of them padding, workgroups that find nothing to do cost more than
-// what is won (1280 rows 52 and 49).
+// long enough for a turn of the loop: whole, in one launch.  Kernel times in us, whole and split:
+//   rows                             112          160          256          320          384          512
+//   V = 152,640 bf16           13.3 12.0    14.0 14.8    16.1 19.5    24.5 24.4    25.5 27.7    29.2 32.3
+//     with entropies           15.2 12.9    16.0 16.0    17.7 21.4    27.3 26.7    27.8 30.2    30.9 34.8
+//     40 % of them padding     12.9 11.4    13.1 12.7    13.5 14.9    21.4 17.4    21.8 19.5    23.2 23.7
+//   V = 152,640 fp32           16.3 14.6    19.8 22.1    26.3 28.7    37.7 35.9    41.1 41.6    50.3 54.8
+//   V =  33,000 bf16            6.6  7.7     6.7  8.0     7.0  9.2     9.6  9.8     9.6 10.8     9.9 12.1
+//   V =  80,000 fp32, entropies 11.0 11.5   12.7 13.8    15.1 21.0    22.2 24.9    23.6 28.5    28.2 31.3
+// With padding workgroups that find nothing to do cost a part of what is won, and with more rows all of it (1280 rows, half of
+// them padding: 52 and 49).
 static bool tl_wide(int64_t rows, int V, int dtype) {
     const int64_t bytes = (int64_t)V * (dtype == GRX_F32 ? 4 : 2);
     return rows >= 128 && rows <= 512 && (rows <= 256 || rows >= 384) && bytes >= TL_WIDE * TL_UNROLL * 16;

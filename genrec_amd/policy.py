@@ -78,7 +78,9 @@ def lm_head_token_logps(hidden: torch.Tensor, weight: torch.Tensor, token_ids: t
     nothing.  The logits' gradient reaches the two products in two bf16 pieces (16 bits of each element, where autograd's bf16
     logits would hold 8), so that rows whose gradients cancel leave nothing but the rounding of 32-bit sums.
     Rows of padding, and in the backward pass rows whose gradients are 0, take no part in the products.  Scratch
-    tensors: about V / 16 bytes a row forward; up to 1 GB and 12 bytes per element of ``hidden`` backward.  A pass
+    tensors: forward, per row, V / 16 (many rows) to V / 4 bytes (few), half as much again with entropies; backward up to
+    1 GB for a chunk of the logits' gradient (above 2^20 rows 1 KB a row), and up to 64 copies of ``hidden``'s gradient in
+    fp32 where there are few rows, one where there are many; both a copy or two of ``hidden``.  A pass
     recorded into a HIP graph needs leaves of its own (``detach().requires_grad_()`` inside the recording)."""
     return (_ops_module or _ops()).lm_head_token_logps(hidden, weight, token_ids, temperature, return_entropy, keep_bytes)
 

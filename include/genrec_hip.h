@@ -749,9 +749,12 @@ GRX_API int grx_token_logps_backward(const grx_token_logps_args* args, void* str
  * contiguous, 16-byte aligned, all of them (a null one is not computed); the logits' gradient in
  * between is the sum of two bf16 numbers, within 2^-16 of each element.  Hidden rows of padding, and of rows whose gradients are 0, may hold anything.
  * H a multiple of 64, at most 2^34 elements of hidden in the backward pass, operand rows 16-byte
- * aligned.  scratch: the bytes that the matching size function names (forward: about V / 16 per row
- * and 2 per element of hidden; backward: a chunk of the logits' gradient, up to 1 GB, and about 12
- * per element of hidden), 16-byte aligned, contents need no initialisation; calls that may overlap
+ * aligned.  scratch: the bytes that the matching size function names, 16-byte aligned, contents need no
+ * initialisation (forward: 2 per element of hidden and, per row, V / 16 with row tiles of 256, V / 8 with
+ * 128 and 192, V / 4 with 64, rows rounded up to tiles, half as much again with entropies; backward: 2 per
+ * element of hidden, 4 with grad_weight, a chunk of the logits' gradient -- 4 per element, up to 1 GB, above
+ * 2^20 rows 256 columns of all rows -- and for grad_hidden as many fp32 copies of it as fill the CUs, up
+ * to 64 of few rows); calls that may overlap
  * must not share it.  kept (or null; grx_lm_token_logps_kept_bytes(N, V) bytes, 16-byte aligned, up
  * to 2^20 rows): the forward pass leaves its products there in fp32, and the backward pass of the
  * same N, V and token ids takes them instead of forming them again.

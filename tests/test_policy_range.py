@@ -46,3 +46,23 @@ def test_libraries_of_different_builds_are_refused(monkeypatch):
     monkeypatch.setattr(ops, "struct_bytes", (sizes[0], sizes[1] - 8, sizes[2]))
     with pytest.raises(_lib.GenrecHipError, match="different builds"):
         policy.token_logps(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("N,H,V", [(1, 64, 1), (5, 2048, 152640), (64, 2048, 152640), (100, 128, 151669), (320, 2048, 152640), (400, 1536, 152640),
+                                   (1403, 3584, 151669), (8192, 2048, 152640), (1 << 21, 64, 1000), (1 << 23, 64, 1000)])
+def test_scratch_sizes_are_what_the_header_says(N, H, V):
+    lib = _lib.lib()
+    up = lambda n, to: (n + to - 1) // to * to
+    columns, small = up(V, 256), 16 << 10  # small: what is rounded up to 256 bytes
+    per_row = lambda bn: columns * {64: 1 / 4, 128: 1 / 8, 192: 1 / 8, 256: 1 / 16}[bn]
+    for entropy in (0, 1):
+        most = max(up(N, bn) * per_row(bn) for bn in (64, 128, 192, 256)) * (1.5 if entropy else 1)
+        least = min(up(N, bn) * per_row(bn) for bn in (64, 128, 192, 256)) * (1.5 if entropy else 1)
+        have = lib.grx_lm_token_logps_scratch_bytes(N, H, V, entropy) - 2 * N * H
+        assert least <= have <= most + 16 * N + small
+    chunk = max(1 << 30, 4 * up(N, 64) * 256)
+    for want_h, want_w in ((1, 0), (0, 1), (1, 1)):
+        copies = (2 + 2 * want_w) * up(N, 64) * H
+        have = lib.grx_lm_token_logps_backward_scratch_bytes(N, H, V, want_h, want_w)
+        assert have <= copies + chunk + want_h * 64 * up(N, 256) * H * 4 + 64 * N + small
+    assert lib.grx_lm_token_logps_kept_bytes(N, V) <= up(N, 256) * columns * 4

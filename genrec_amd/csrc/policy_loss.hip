@@ -342,7 +342,7 @@ __global__ __launch_bounds__(PL_THREADS) void policy_loss_grad_kernel(const floa
 
 // ---- host ------------------------------------------------------------------------------------------
 // Lanes per row; a lane's share of a row of up to 1024 tokens stays in registers (4096 rows of 1001 tokens, one ratio a
-// row: 33 us with 256 lanes; 64 lanes with 16 tokens each 45 us, for 174 registers leave two waves on a SIMD).
+// row: 30 us with 256 lanes; 64 lanes with 16 tokens each 45 us, for 174 registers leave two waves on a SIMD).
 static int pl_lanes(int T) { return T <= 8 ? 8 : T <= 16 ? 16 : T <= 32 ? 32 : T <= 256 ? 64 : T <= 1024 ? PL_THREADS : PL_BIG; }
 
 static int pl_groups(int R, int T) {

@@ -57,8 +57,8 @@ def token_logps(logits: torch.Tensor, token_ids: torch.Tensor, temperature: floa
     is not below V gives NaN.  Where a gradient follows, hand over the whole logits with -1 at the positions that do not
     count: the gradient is then written in one pass.  That of a slice is autograd's, which fills the whole logits'
     gradient with 0 and copies this one's into it (bf16, V = 152,640, forward and gradient: 5 of 6 positions of 64 rows 72
-    and 109 us, 128 of 129 1.18 and 2.38 ms, 5 of 40 211 and 226 us).  Differentiable in ``logits`` (the gradient has their type); rows whose incoming
-    gradient is 0 cost one write.  A pass recorded into a HIP graph needs leaves of its own: take
+    and 109 us, 128 of 129 1.18 and 2.38 ms, 5 of 40 211 and 226 us).  Differentiable in ``logits`` (the gradient has their type); rows
+    whose incoming gradient is 0 cost one write.  A pass recorded into a HIP graph needs leaves of its own: take
     ``logits.detach().requires_grad_()`` inside the recording (gradients that would leave it are refused)."""
     return (_ops_module or _ops()).token_logps(logits, token_ids, temperature, return_entropy)
 

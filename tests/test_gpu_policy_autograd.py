@@ -151,3 +151,36 @@ def test_whole_logits_with_padding_where_a_slice_would_cut(L, T):
     assert (got[:, : L - T - 1] == 0).all() and (got[:, -1] == 0).all()
     off = (got - want).abs()[:, -T - 1 : -1]
     assert (off <= bound * 2 * g.abs()[..., None]).all()
+
+
+@pytest.mark.parametrize("keep_bytes", [8 << 30, 0])
+def test_entropies_alone_and_other_integer_types(keep_bytes):
+    """No gradient of the log-probabilities is a gradient of 0; token ids of any integer type are the same tokens."""
+    h, w, ids = _head()
+    ids[::5] = -1
+    g = torch.randn(ids.shape, device=ids.device)
+    lp, ent = lm_head_token_logps(h, w, ids, 0.9, True, keep_bytes)
+    want = torch.autograd.grad([lp, ent], [h, w], [torch.zeros_like(g), g], retain_graph=True)
+    got = torch.autograd.grad(ent, [h, w], g, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[1].any()
+    half = torch.autograd.grad(lp[::2], [h, w], g[::2], retain_graph=True)  # an incoming gradient with gaps
+    some = torch.where(torch.arange(ids.numel(), device=ids.device) % 2 == 0, g, 0.0)
+    assert all(torch.equal(a, b) for a, b in zip(half, torch.autograd.grad(lp, [h, w], some)))
+    for kind in (torch.int32, torch.int16):
+        assert torch.equal(lm_head_token_logps(h, w, ids.to(kind), 0.9, keep_bytes=keep_bytes), lp)
+
+
+@pytest.mark.parametrize("shape", [(5, 1), (1, 1), (1, 4097), (4097, 1), (3, 1025)])
+def test_advantages_of_single_positions_and_rows(shape):
+    """[R, T] and [R] say the same where a row's advantages are equal, at the borders between the kernels."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    x = (torch.randn(shape, generator=gen, device="cuda") - 2).requires_grad_()
+    old = x.detach() + 0.1 * torch.randn(shape, generator=gen, device="cuda")
+    adv = torch.randn(shape[:1], generator=gen, device="cuda")
+    mask = torch.ones(shape, device="cuda")
+    for level in ("token", "sequence"):
+        made = []
+        for a in (adv, adv[:, None].expand(shape), adv[:, None].expand(shape).contiguous()):
+            loss = policy_loss(x, a, mask, old, importance_sampling_level=level).loss
+            made.append((loss.detach(), torch.autograd.grad(loss, x)[0]))
+        assert all(torch.equal(p, q) for m in made[1:] for p, q in zip(m, made[0]))
